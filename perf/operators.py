@@ -220,8 +220,8 @@ def prepare(case, seed):
     if own:
         from santa_amd.paged import PagedPlan
 
-        st["plan"] = PagedPlan(st["lens"], heads=H, kv_heads=KVH, head_dim=D, page_size=page, new_tokens=st["new"],
-                               prefixes=st["prefixes"], device="cuda")
+        st["plan"] = PagedPlan(st["lens"], heads=H, kv_heads=KVH, new_tokens=st["new"], prefixes=st["prefixes"],
+                               device="cuda")
     return st
 
 
