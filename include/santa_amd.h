@@ -326,6 +326,119 @@ int santa_rt_exact_decode(const void* q, const void* k, const void* v, void* out
                           int KVH, int D, const long long* strides, void* workspace, size_t workspace_bytes,
                           hipStream_t stream);
 
+/* ------------------------------------------------------- shared paged caches */
+
+/* A paged KV cache that sequences share, and the exact attention that reads it
+ * (santa_amd/paged.py).  No counterpart in the reference, whose caches are
+ * contiguous and one per sequence (tutorial_code/runtime_common.py:340-397).
+ * Pages and block tables are those of santa_flash_decode_paged: K and V pools
+ * [num_pages, page_size, KVH, D], token n of sequence s in row n % page_size of
+ * page table[s][n / page_size], page_size a power of two in [8, 2^20].
+ *
+ * santa_pages: host bookkeeping of max_seqs sequences over num_pages pages, a
+ * sequence holding at most row_pages of them.  An object is used by one host
+ * thread at a time.  Every call either does all it is asked or fails and
+ * changes nothing.
+ *   _add: n new sequences of lengths[i] tokens, in the lowest free rows of the
+ *     table, written to seqs; pages are taken lowest number first.
+ *   _extend: tokens[i] more tokens for seqs[i] (each named once).  A last page
+ *     that is partly filled and held by other sequences too is replaced by a
+ *     copy.
+ *   _fork: n new sequences that hold every page of seq.
+ *   _free: the sequences end; a page that none holds is free.
+ *   _compact: with n pages in use, those numbered n and above move to the
+ *     numbers below n that are free, both in ascending order.
+ * What a call asks of the device is returned by _changes until the next call:
+ * page copies [n][2] (source, destination), edits of the block table [n][4]
+ * (row, first entry, count, value: entry first + i becomes value + i or, for a
+ * negative value, entry first + i of row -1 - value), and whether every table
+ * entry that is a copy's source becomes its destination.
+ * _length: tokens of a sequence (-1: no such sequence); _used: pages in use;
+ * _row: a sequence's pages, returns how many.
+ * _shared: groups of the sequences seqs whose first tokens lie in the same pages,
+ * the last own[i] tokens of each apart: group[i] is a group or -1, shared[g] the
+ * tokens that group g has in common (shared: room for n / 2). */
+typedef struct santa_pages santa_pages;
+int santa_pages_create(int num_pages, int page_size, int max_seqs, int row_pages, santa_pages** out);
+void santa_pages_destroy(santa_pages* p);
+int santa_pages_add(santa_pages* p, const int* lengths, int n, int* seqs);
+int santa_pages_extend(santa_pages* p, const int* seqs, const int* tokens, int n);
+int santa_pages_fork(santa_pages* p, int seq, int n, int* seqs);
+int santa_pages_free(santa_pages* p, const int* seqs, int n);
+int santa_pages_compact(santa_pages* p);
+int santa_pages_changes(const santa_pages* p, const int** copies, int* n_copies, const int** edits, int* n_edits,
+                        int* remap);
+int santa_pages_length(const santa_pages* p, int seq);
+int santa_pages_used(const santa_pages* p);
+int santa_pages_row(const santa_pages* p, int seq, const int** pages);
+int santa_pages_shared(const santa_pages* p, const int* seqs, const int* own, int n, int* group, int* shared,
+                       int* n_groups);
+
+/* Page copies: in each of n_pools pools (page i page_stride bytes from page
+ * i - 1), pairs[j][0] to pairs[j][1] for j < n.  pools and pairs are host
+ * arrays, read before the call returns.  No page is written twice or both read
+ * and written; page_bytes, page_stride and the pools' addresses are multiples
+ * of 16. */
+int santa_paged_copy(const void* const* pools, int n_pools, long long page_bytes, long long page_stride, int num_pages,
+                     const int* pairs, int n, hipStream_t stream);
+/* The last call's page copies in the pools and its edits in the device block
+ * table [max_seqs, table_stride], on `stream`. */
+int santa_pages_apply(const santa_pages* p, const void* const* pools, int n_pools, long long page_bytes,
+                      long long page_stride, int* table, long long table_stride, int max_seqs, hipStream_t stream);
+
+/* Attention plan: how the work of santa_paged_attention is cut up for one set
+ * of lengths, built on the host once and used by every layer.  Sequence b
+ * holds lens[b] tokens, the last new_tokens[b] of which have queries, in block
+ * table row rows[b] (rows NULL: b).  The sequences with group[b] = g >= 0
+ * (group NULL: none) have their first shared[g] tokens in common, no more than
+ * precede every member's queries; the pages of one of the members are
+ * read for all.  fixed != 0: items and the workspace are sized so that any
+ * other lengths with the same new_tokens and groups give a plan of the same
+ * info (for captured graphs whose plan changes between replays).  info is
+ * always written; plan (info->ints ints, 16-byte aligned, to be copied to the
+ * device as it is) where it is not NULL. */
+typedef struct santa_paged_plan_info {
+  int tokens;       /* queries: the sum of new_tokens */
+  int items;        /* workgroups per KV head */
+  int merge_tokens; /* tokens whose output is joined from parts */
+  int max_len, max_row; /* what the block table has to hold */
+  int heads, kv_heads;
+  long long records; /* parts: rows of the workspace */
+  long long ints, pos_at, merge_at, parts_at, list_at; /* ints of the plan, and where its sections start */
+} santa_paged_plan_info;
+int santa_paged_plan(const int* lens, const int* new_tokens, const int* rows, int B, const int* group,
+                     const int* shared, int n_groups, int heads, int kv_heads, int fixed, santa_paged_plan_info* info,
+                     int* plan, long long plan_ints);
+
+/* Exact attention over pages, D = 64 or 128: query i of sequence b (row
+ * sum of the earlier new_tokens + i of q [tokens, H, D]) attends to the tokens
+ * 0 .. lens[b] - new_tokens[b] + i of its sequence; one that has none gives
+ * zeros.  out [tokens, H, D] contiguous.  strides: 8 host values, q's token and
+ * head strides, K's page, row and head strides and V's, in elements (multiples
+ * of 8, the last dimension contiguous, the tensors 16-byte aligned).  plan: the
+ * device copy of a plan with this info.  Page numbers are clamped to the pool.
+ * Scores, softmax and sums in float32; the probabilities enter the second
+ * product rounded to the 16-bit type or, where at most 16 rows share a pass
+ * over a KV head's tokens, as the sum of two such values.  workspace:
+ * santa_paged_workspace_size(info, D) bytes, 16-byte aligned, no initialization
+ * needed. */
+size_t santa_paged_workspace_size(const santa_paged_plan_info* info, int D);
+int santa_paged_attention(const void* q, const void* k_pages, const void* v_pages, void* out, int dtype, int D,
+                          int num_pages, int page_size, const long long* strides, const int* table,
+                          long long table_stride, int table_rows, const santa_paged_plan_info* info, const int* plan,
+                          float scale, void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/* RoPE of new tokens with their write into pages: qkv [tokens, H + 2 KVH, D]
+ * contiguous, cos_, sin_ [tokens, D], one 16-bit type; q heads rotated into
+ * q_out [tokens, H, D], k heads rotated and v heads copied into the pages of
+ * their tokens (tokens of a plan; strides: K's page, row and head strides and
+ * V's, as above).  Rotate-half convention, float32, rounded once.  D a multiple of 16, every
+ * tensor 16-byte aligned.  A token of a negative position is not written. */
+int santa_paged_rope_append(const void* qkv, const void* cos_, const void* sin_, void* q_out, void* k_pages,
+                            void* v_pages, int dtype, int D, int num_pages, int page_size, const long long* strides,
+                            const int* table, long long table_stride, int table_rows,
+                            const santa_paged_plan_info* info, const int* plan, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

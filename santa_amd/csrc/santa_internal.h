@@ -24,6 +24,8 @@ struct PageTable {
 int set_error(int code, const char* fmt, ...) __attribute__((format(printf, 2, 3)));
 // Clears the calling thread's last error and returns SANTA_OK.
 int clear_error();
+// page_size: a power of two in [8, 2^20].
+int check_page_size(int page_size);
 // Checks a paged cache's geometry (page_size a power of two in [8, 2^20],
 // num_pages > 0, table_stride >= ceil(max_len / page_size)) and fills pt.
 int check_page_table(const int* table, int num_pages, int page_size, int table_stride, int max_len, PageTable* pt);
@@ -49,6 +51,17 @@ struct DenseCut {
   int S;      // samples per sequence and head, at most 2^20 (beyond that every tile is dense anyway)
 };
 constexpr int kDenseChunks = 7;
+
+// What the host bookkeeping of a paged cache asks of the device: a page copied
+// in every pool; entries col .. col + count - 1 of a block table row set to
+// value, value + 1, ... or, where value < 0, to the same entries of row
+// -1 - value.
+struct PageCopy {
+  int src, dst;
+};
+struct TableEdit {
+  int row, col, count, value;
+};
 
 constexpr size_t kWsAlign = 256;
 inline size_t align_up(size_t x) { return (x + kWsAlign - 1) & ~(kWsAlign - 1); }

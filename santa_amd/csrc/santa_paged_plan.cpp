@@ -1,0 +1,243 @@
+// santa_paged_plan.cpp -- how the work of the paged attention
+// (santa_paged.hip) is cut into workgroups.
+#include <algorithm>
+#include <climits>
+#include <cstdint>
+#include <cstring>
+#include <new>
+#include <vector>
+
+#include "santa_amd.h"
+#include "santa_internal.h"
+#include "santa_paged.h"
+
+namespace santa {
+namespace paged {
+namespace {
+
+// Rows (token, query head of one KV head) that pass over the same tokens
+// together: those of the tokens tok0 .. tok0 + ntok - 1 of the batch, or of
+// the list.
+struct Block {
+  int flags, row, begin, end, tok0, ntok, pos0;
+  int tiles() const { return (end - begin + kTile - 1) / kTile; }
+};
+
+int div_up(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
+
+// Workgroups that are resident at once, two per compute unit (their LDS).
+int resident() {
+  int dev = 0, cus = 0;
+  if (hipGetDevice(&dev) != hipSuccess ||
+      hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
+    cus = 256;
+  return 2 * cus;
+}
+
+struct Input {
+  const int *lens, *new_tokens, *rows;
+  int B;
+  const int *group, *shared;
+  int n_groups, heads, kv_heads, fixed;
+};
+
+int build(const Input& in, santa_paged_plan_info* info, int* plan, long long plan_ints) {
+  const int GH = in.heads / in.kv_heads;
+  const int block_tokens = std::max(1, kBlockRows / GH);
+  *info = santa_paged_plan_info{};
+  info->heads = in.heads;
+  info->kv_heads = in.kv_heads;
+  info->max_row = -1;
+  long long tokens = 0;
+  std::vector<int> first(static_cast<size_t>(in.B));       // first token of each sequence
+  std::vector<int> prefix(static_cast<size_t>(in.B), 0);   // tokens read with the group
+  std::vector<int> lead(static_cast<size_t>(in.n_groups), -1), members(static_cast<size_t>(in.n_groups), 0);
+  std::vector<long long> group_tokens(static_cast<size_t>(in.n_groups), 0);
+  for (int b = 0; b < in.B; ++b) {
+    const int n = in.lens[b], t = in.new_tokens[b], row = in.rows ? in.rows[b] : b;
+    if (n < 0 || t < 0) return set_error(SANTA_ERR_INVALID, "a sequence has 0 or more tokens and new tokens");
+    if (row < 0) return set_error(SANTA_ERR_INVALID, "bad block table row %d", row);
+    first[b] = static_cast<int>(tokens);
+    tokens += t;
+    if (tokens > (1 << 30) / GH) return set_error(SANTA_ERR_INVALID, "too many new tokens");
+    info->max_len = std::max(info->max_len, n);
+    info->max_row = std::max(info->max_row, row);
+    const int g = in.group ? in.group[b] : -1;
+    if (g < 0) continue;
+    if (g >= in.n_groups) return set_error(SANTA_ERR_INVALID, "sequence %d names group %d of %d", b, g, in.n_groups);
+    if (in.shared[g] < 0 || in.shared[g] > std::max(0, n - t))
+      return set_error(SANTA_ERR_INVALID, "%d tokens are not common to sequence %d: %d precede its new tokens",
+                       in.shared[g], b, std::max(0, n - t));
+    if (t == 0) continue;
+    if (lead[g] < 0) lead[g] = row;
+    ++members[g];
+    group_tokens[g] += t;
+  }
+  info->tokens = static_cast<int>(tokens);
+
+  // the passes: whole tiles of each group's common tokens for all its rows, and
+  // the rest of each sequence for its own
+  std::vector<Block> blocks;
+  std::vector<int> list;
+  std::vector<int> token_pos(static_cast<size_t>(tokens)), token_row(static_cast<size_t>(tokens));
+  std::vector<int> group_list(static_cast<size_t>(in.n_groups), 0);
+  for (int g = 0; g < in.n_groups; ++g) {
+    const int common = in.shared[g] / kTile * kTile;
+    if (members[g] < 2 || common == 0) {
+      members[g] = 0;
+      continue;
+    }
+    group_list[g] = static_cast<int>(list.size());
+    for (int b = 0; b < in.B; ++b)
+      if (in.group[b] == g) {
+        prefix[b] = common;
+        for (int i = 0; i < in.new_tokens[b]; ++i) list.push_back(first[b] + i);
+      }
+    const int n = static_cast<int>(list.size()) - group_list[g];
+    for (int i = 0; i < n; i += block_tokens)
+      blocks.push_back({kFromList, lead[g], 0, common, group_list[g] + i, std::min(block_tokens, n - i), INT_MAX / 2});
+  }
+  for (int b = 0; b < in.B; ++b) {
+    const int n = in.lens[b], t = in.new_tokens[b], row = in.rows ? in.rows[b] : b;
+    for (int i = 0; i < t; ++i) {
+      token_pos[first[b] + i] = n - t + i;
+      token_row[first[b] + i] = row;
+    }
+    for (int i = 0; i < t; i += block_tokens) {
+      const int k = std::min(block_tokens, t - i);
+      blocks.push_back({0, row, prefix[b], std::max(prefix[b], std::min(n, n - t + i + k)), first[b] + i, k, n - t + i});
+    }
+  }
+
+  // tiles per item: the fewest with which one resident round holds all items,
+  // or thirds of a round's worth where the blocks alone are more than that
+  const int slots = std::max(1, resident() / in.kv_heads);
+  long long total = 0;
+  int most = 1;
+  for (const Block& k : blocks) {
+    total += k.tiles();
+    most = std::max(most, k.tiles());
+  }
+  auto count = [&](int c) {
+    long long n = 0;
+    for (const Block& k : blocks) n += std::max(1, div_up(k.tiles(), c));
+    return n;
+  };
+  int chunk = std::max(kMinChunk, div_up(total, 3LL * slots));
+  if (count(most) <= slots) {
+    int lo = 1, hi = most;
+    while (lo < hi) {
+      const int mid = lo + (hi - lo) / 2;
+      if (count(mid) <= slots) hi = mid;
+      else lo = mid + 1;
+    }
+    chunk = std::max(kMinChunk, lo);
+  }
+  const long long max_items = static_cast<long long>(blocks.size()) + 3LL * slots;
+  if (max_items > (1 << 26)) return set_error(SANTA_ERR_INVALID, "too many sequences");
+
+  struct Parts {
+    int base = 0, rows = 0, local = 0, splits = 0;
+  };
+  std::vector<Parts> common_parts(static_cast<size_t>(tokens)), own_parts(static_cast<size_t>(tokens));
+  struct Piece {
+    int block, begin, end, base;
+    bool direct;
+  };
+  std::vector<Piece> pieces;
+  long long records = 0, most_rows = 0;
+  for (size_t i = 0; i < blocks.size(); ++i) {
+    const Block& k = blocks[i];
+    const int tiles = k.tiles(), splits = std::max(1, div_up(tiles, chunk));
+    const int rows = k.ntok * GH;
+    const bool from_list = (k.flags & kFromList) != 0;
+    const bool direct = splits == 1 && !from_list && k.begin == 0;
+    most_rows = std::max<long long>(most_rows, rows);
+    for (int j = 0; j < k.ntok && !direct; ++j) {
+      Parts& p = from_list ? common_parts[list[k.tok0 + j]] : own_parts[k.tok0 + j];
+      p.base = static_cast<int>(records);
+      p.rows = rows;
+      p.local = j * GH;
+      p.splits = splits;
+    }
+    for (int s = 0; s < splits; ++s) {
+      const int t0 = static_cast<int>(static_cast<long long>(tiles) * s / splits);
+      const int t1 = static_cast<int>(static_cast<long long>(tiles) * (s + 1) / splits);
+      pieces.push_back({static_cast<int>(i), k.begin + kTile * t0, std::min(k.end, k.begin + kTile * t1),
+                        static_cast<int>(records), direct});
+      if (!direct) records += static_cast<long long>(rows) * in.kv_heads;
+      if (records > INT_MAX) return set_error(SANTA_ERR_INVALID, "too many new tokens");
+    }
+  }
+  // the longest first
+  std::stable_sort(pieces.begin(), pieces.end(),
+                   [](const Piece& a, const Piece& b) { return a.end - a.begin > b.end - b.begin; });
+
+  info->items = static_cast<int>(in.fixed ? max_items : static_cast<long long>(pieces.size()));
+  info->records = in.fixed ? max_items * most_rows * in.kv_heads : records;
+  if (info->records > INT_MAX) return set_error(SANTA_ERR_INVALID, "too many new tokens");
+  std::vector<int> joined;
+  for (long long t = 0; t < tokens; ++t)
+    if (own_parts[t].splits > 0) joined.push_back(static_cast<int>(t));
+  info->merge_tokens = in.fixed ? info->tokens : static_cast<int>(joined.size());
+  info->pos_at = static_cast<long long>(info->items) * kItemInts;
+  info->parts_at = info->pos_at + 2 * tokens + (tokens & 1) * 2;
+  info->merge_at = info->parts_at + 8 * tokens;
+  info->list_at = info->merge_at + info->merge_tokens;
+  info->ints = info->list_at + static_cast<long long>(list.size());
+  if (!plan) return clear_error();
+  if (plan_ints < info->ints) return set_error(SANTA_ERR_INVALID, "the plan does not fit its buffer");
+
+  std::memset(plan, 0, static_cast<size_t>(info->ints) * sizeof(int));
+  for (size_t i = 0; i < pieces.size(); ++i) {
+    const Piece& p = pieces[i];
+    const Block& k = blocks[p.block];
+    Item it{};
+    it.flags = k.flags | (p.direct ? kDirect : 0);
+    it.row = k.row;
+    it.begin = p.begin;
+    it.end = p.end;
+    it.tok0 = k.tok0;
+    it.rows = k.ntok * GH;
+    it.pos0 = k.pos0;
+    it.base = p.base;
+    std::memcpy(plan + i * kItemInts, &it, sizeof it);
+  }
+  int* pos = plan + info->pos_at;
+  int* parts = plan + info->parts_at;
+  for (long long t = 0; t < tokens; ++t) {
+    pos[2 * t] = token_pos[t];
+    pos[2 * t + 1] = token_row[t];
+    const Parts &a = common_parts[t], &b = own_parts[t];
+    const int v[8] = {a.base, a.rows, a.local, a.splits, b.base, b.rows, b.local, b.splits};
+    std::memcpy(parts + 8 * t, v, sizeof v);
+  }
+  for (int t = 0; t < info->merge_tokens; ++t)
+    plan[info->merge_at + t] = t < static_cast<int>(joined.size()) ? joined[t] : -1;
+  std::copy(list.begin(), list.end(), plan + info->list_at);
+  return clear_error();
+}
+
+}  // namespace
+}  // namespace paged
+}  // namespace santa
+
+extern "C" int santa_paged_plan(const int* lens, const int* new_tokens, const int* rows, int B, const int* group,
+                                const int* shared, int n_groups, int heads, int kv_heads, int fixed,
+                                santa_paged_plan_info* info, int* plan, long long plan_ints) {
+  using namespace santa;
+  if (!info || B < 0 || (B > 0 && (!lens || !new_tokens)) || n_groups < 0 || (n_groups > 0 && (!group || !shared)))
+    return set_error(SANTA_ERR_INVALID, "bad santa_paged_plan arguments");
+  if (kv_heads <= 0 || heads <= 0 || heads % kv_heads != 0)
+    return set_error(SANTA_ERR_INVALID, "H must be divisible by KVH. Got H=%d KVH=%d", heads, kv_heads);
+  if (heads / kv_heads > paged::kBlockRows)
+    return set_error(SANTA_ERR_UNSUPPORTED, "the paged attention takes up to %d query heads per KV head. Got %d",
+                     paged::kBlockRows, heads / kv_heads);
+  try {
+    return paged::build({lens, new_tokens, rows, B, n_groups > 0 ? group : nullptr, shared, n_groups, heads, kv_heads,
+                         fixed},
+                        info, plan, plan_ints);
+  } catch (const std::bad_alloc&) {
+    return set_error(SANTA_ERR_INVALID, "out of host memory");
+  }
+}
