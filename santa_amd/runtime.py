@@ -21,7 +21,7 @@ import math
 import os
 import time
 from dataclasses import dataclass
-from typing import Dict, List, Optional
+from typing import Dict, List, Optional, Sequence, Union
 
 import torch
 import torch.autograd.forward_ad as fwAD
@@ -403,6 +403,18 @@ class ExactDecodeBackend:
         o = torch.bmm(p, v)                                                                  # [B*KVH, GH, D]
         return o.reshape(B, H, D).to(q_bhd.dtype)
 
+    def decode_paged(self, q_bhd: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                     block_table: torch.Tensor, seq_lens) -> torch.Tensor:
+        """Exact decode over a paged cache, with the arguments of the sampled
+        backends' decode_paged: k_pages / v_pages [num_pages, page_size, KVH, D],
+        block_table int32 [B, pages per sequence], seq_lens an int or one length
+        per sequence (santa_amd.paged.paged_attention, which also reads shared
+        prefixes once)."""
+        from .paged import paged_attention
+
+        lens = [seq_lens] * q_bhd.shape[0] if isinstance(seq_lens, int) else seq_lens
+        return paged_attention(q_bhd, k_pages, v_pages, block_table, lens)
+
     def info(self) -> Dict[str, object]:
         return {"backend": self.name, "exact_attention": True, "supports_true_batch_decode": True}
 
@@ -598,6 +610,80 @@ class RandomLlama:
             nxt = self.layers[li + 1]["ln1"] if li + 1 < len(self.layers) else self.norm
             x = _FusedOps.add_rms_norm(h, m, nxt, s.rms_eps)  # h += m, then the next layer's (or final) norm
         return _FusedOps.logits(x, self.lm_head)
+
+    # ------------------------------------------------------ shared paged caches
+    @torch.inference_mode()
+    def extend(self, tokens: torch.Tensor, cache, seqs: Sequence[int],
+               new_tokens: Union[None, int, Sequence[int]] = None, *, backend=None,
+               mlp_chunk: int = 8192) -> torch.Tensor:
+        """New tokens of sequences of a santa_amd.paged.PagedKVCache: prompts of
+        new sequences, more tokens behind what a sequence holds (a prompt behind
+        one it was forked from), or one decoded token each.  tokens: [len(seqs),
+        T], or the sequences' tokens one after the other with new_tokens (an int
+        or one count per sequence, at least 1).  Lengthens the sequences, writes
+        the tokens' K and V into their pages and returns the logits of each
+        sequence's last token [len(seqs), V] (float32, as prefill's).  Attention
+        is exact, tokens that sequences hold in the same pages being read once;
+        or, for one new token each, that of a backend with decode_paged."""
+        from .paged import paged_attention, rope_append
+
+        s, D = self.shape, self.shape.head_dim
+        B = len(seqs)
+        if new_tokens is None:
+            if tokens.dim() != 2 or tokens.shape[0] != B:
+                raise ValueError(f"tokens must be [{B}, T], or come with new_tokens; got {tuple(tokens.shape)}")
+            new_tokens = tokens.shape[1]
+        new = [new_tokens] * B if isinstance(new_tokens, int) else [int(n) for n in new_tokens]
+        if len(new) != B or B == 0 or min(new) < 1 or tokens.numel() != sum(new):
+            raise ValueError(f"{tokens.numel()} tokens do not give {B} sequences {new} new ones, at least 1 each")
+        if (cache.layers, cache.kv_heads, cache.head_dim) != (s.layers, s.kv_heads, D) or cache.dtype != self.dtype:
+            raise ValueError("the cache does not have the model's layers, KV heads, head_dim and dtype")
+        if backend is not None and max(new) > 1:
+            raise ValueError("a backend decodes one new token per sequence")
+        cache.extend(seqs, new)
+        plan = cache.plan(seqs, s.heads, new)
+        cos, sin = _rope_cos_sin(plan.positions, D, s.rope_theta, self.dtype)  # [N, D]
+        table, tables = cache.block_table, None
+        if backend is not None:
+            tables = cache.tables(seqs).contiguous()
+
+        def attend(li, qkv):
+            q = rope_append(qkv.view(len(qkv), -1, D), cos, sin, cache.k[li], cache.v[li], table, plan)
+            if backend is not None:
+                a = backend.decode_paged(q, cache.k[li], cache.v[li], tables, plan.seq_lens)
+            else:
+                a = paged_attention(q, cache.k[li], cache.v[li], table, plan)
+            return a.reshape(len(q), s.heads * D)
+
+        h = self.embed[tokens.reshape(-1)]  # [N, hidden]
+        fused = self.device.type == "cuda" and self.dtype == torch.bfloat16
+        if fused:
+            lin = _FusedOps.linear
+            h = h.contiguous()
+            x = _FusedOps.add_rms_norm(h, None, self.layers[0]["ln1"] if self.layers else self.norm, s.rms_eps)
+            for li, L in enumerate(self.layers):
+                o = lin(attend(li, lin(x, L["wqkv"])), L["wo"])
+                x = _FusedOps.add_rms_norm(h, o, L["ln2"], s.rms_eps)  # h += o
+                if len(h) <= mlp_chunk:
+                    o = lin(lin(x, L["wgu"], swiglu=True), L["wd"])
+                else:
+                    for c in range(0, len(h), mlp_chunk):
+                        o[c:c + mlp_chunk] = lin(lin(x[c:c + mlp_chunk], L["wgu"], swiglu=True), L["wd"])
+                nxt = self.layers[li + 1]["ln1"] if li + 1 < len(self.layers) else self.norm
+                x = _FusedOps.add_rms_norm(h, o, nxt, s.rms_eps)  # h += the MLP's, then the next layer's (or final) norm
+        else:
+            for li, L in enumerate(self.layers):
+                h = h + F.linear(attend(li, F.linear(_rms_norm(h, L["ln1"], s.rms_eps), L["wqkv"])), L["wo"])
+                for c in range(0, len(h), mlp_chunk):
+                    hc = h[c:c + mlp_chunk]
+                    hc += self._mlp(L, _rms_norm(hc, L["ln2"], s.rms_eps))
+            x = _rms_norm(h, self.norm, s.rms_eps)
+        if max(new) > 1:
+            last = torch.tensor(new).cumsum(0) - 1
+            if x.is_cuda:
+                last = last.pin_memory().to(x.device, non_blocking=True)
+            x = x.index_select(0, last)
+        return _FusedOps.logits(x, self.lm_head) if fused else F.linear(x, self.lm_head).float()
 
 
 @torch.inference_mode()

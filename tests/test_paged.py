@@ -12,6 +12,7 @@ import torch
 
 from santa_amd import paged
 from santa_amd.paged import PagedKVCache, PagedPlan, copy_pages, paged_attention, rope_append
+from santa_amd.runtime import ExactDecodeBackend, LlamaShape, NHDCache, RandomLlama
 
 
 class Model:
@@ -527,3 +528,68 @@ def test_library_refusals():
     small = (ctypes.c_int * 4)()
     out = paged._PlanInfo()
     assert lib.santa_paged_plan(small, small, None, 2, None, None, 0, 4, 2, 0, ctypes.byref(out), small, 1) != 0 or out.ints <= 1
+
+
+# -------------------------------------------------------------------- model
+TINY = LlamaShape(hidden=128, intermediate=256, heads=8, kv_heads=2, layers=2, vocab=97)
+
+
+def _model_cache(shape, device="cpu", dtype=torch.float32, **kw):
+    args = dict(num_pages=60, page_size=8, max_seqs=8, max_len=120, kv_heads=shape.kv_heads, head_dim=shape.head_dim)
+    return PagedKVCache(shape.layers, dtype=dtype, device=device, **{**args, **kw})
+
+
+def test_model_extends():
+    """Prompts, prompts behind a forked one and single tokens, after pages have
+    moved: the logits are those of each sequence prefilled by itself."""
+    model = RandomLlama(TINY, seed=3, std=0.05, dtype=torch.float32, device="cpu")
+    g = torch.Generator().manual_seed(2)
+    toks = torch.randint(0, TINY.vocab, (4, 100), generator=g)
+    toks[1:, :30] = toks[0, :30]  # three sequences share 30 tokens with the first
+
+    def alone(s, n):
+        return model.prefill(toks[s:s + 1, :n], NHDCache(TINY, 1, n, torch.float32, "cpu"))[0]
+
+    cache = _model_cache(TINY)
+    gone, a = cache.add([40, 0])
+    close = lambda x, y: (x - y).abs().max() < 1e-5  # noqa: E731
+    assert close(model.extend(toks[:1, :30], cache, [a])[0], alone(0, 30))
+    b, c = cache.fork(a, 2)
+    logits = model.extend(torch.cat([toks[2, 30:49], toks[0, 30:31], toks[1, 30:37]]), cache, [c, a, b], [19, 1, 7],
+                          mlp_chunk=5)
+    assert all(close(x, alone(s, n)) for x, s, n in zip(logits, (2, 0, 1), (49, 31, 37)))
+    d, = cache.fork(b)
+    toks[3, :37] = toks[1, :37]
+    cache.free([gone])
+    cache.compact()
+    lens = dict(zip((a, b, c, d), (31, 37, 49, 37)))
+    for i in range(4):
+        order = [d, a, c, b]
+        backend = ExactDecodeBackend() if i == 2 else None
+        logits = model.extend(torch.stack([toks[(a, b, c, d).index(s), lens[s]] for s in order]), cache, order, 1,
+                              backend=backend)
+        for s, x in zip(order, logits):
+            lens[s] += 1
+            assert close(x, alone((a, b, c, d).index(s), lens[s]))
+    assert cache.lengths([a, b, c, d]) == [lens[s] for s in (a, b, c, d)]
+    used = cache.used_pages
+    for bad in (lambda: model.extend(toks[:2, :3], cache, [a]), lambda: model.extend(toks[0, :3], cache, [a, b], [3, 0]),
+                lambda: model.extend(toks[0, :3], cache, [a, b], [1, 1]), lambda: model.extend(toks[0, :0], cache, [], []),
+                lambda: model.extend(toks[:1, :3], cache, [a], backend=ExactDecodeBackend()),
+                lambda: model.extend(toks[:1, :3], _model_cache(TINY, page_size=16, head_dim=32), [0])):
+        with pytest.raises(ValueError):
+            bad()
+    with pytest.raises(RuntimeError, match="would hold"):
+        model.extend(toks[:1, :99], cache, [a])
+    assert cache.used_pages == used
+
+
+def test_backend_decodes_pages():
+    lens = [20, 9, 64]
+    k, v, table = _shared_pools(lens, [], 8, 2, 32, 3, dtype=torch.float32)
+    q = torch.randn(3, 4, 32, generator=torch.Generator().manual_seed(1))
+    want = paged_attention(q, k, v, table, lens)
+    for x in (lens, torch.tensor(lens)):
+        assert torch.equal(ExactDecodeBackend().decode_paged(q, k, v, table, x), want)
+    same = ExactDecodeBackend().decode_paged(q, k, v, table, 9)
+    assert torch.equal(same, paged_attention(q, k, v, table, [9, 9, 9]))

@@ -18,7 +18,9 @@ import pytest
 import torch
 
 from santa_amd.paged import PagedKVCache, PagedPlan, copy_pages, paged_attention, rope_append
-from test_paged import _shared_pools
+from santa_amd import attention_backends as ab
+from santa_amd.runtime import ExactDecodeBackend, LlamaShape, NHDCache, RandomLlama
+from test_paged import _model_cache, _shared_pools
 
 pytestmark = pytest.mark.gpu
 BF, F16 = torch.bfloat16, torch.float16
@@ -421,3 +423,68 @@ def test_copy_pages():
         copy_pages(torch.zeros(4, 3, device="cuda"), [0], [1])
     with pytest.raises(ValueError, match="host integers"):
         copy_pages(x, torch.tensor([0], device="cuda"), [1])
+
+
+# -------------------------------------------------------------------- model
+SMALL = LlamaShape(hidden=512, intermediate=1024, heads=4, kv_heads=1, layers=2, vocab=1000)
+
+
+@pytest.mark.parametrize("dtype", [BF, F16])
+def test_model_extends(dtype):
+    """A prompt, samples of it with prompts of their own, decode steps and a
+    compaction between them: the logits are those of each sequence prefilled by
+    itself, to the tolerance of the runtime's decode against its prefill."""
+    print(f"\n[case] model over a shared cache, {dtype}", flush=True)
+    model = RandomLlama(SMALL, seed=11, std=0.05, device="cuda", dtype=dtype)
+    g = torch.Generator().manual_seed(5)
+    toks = torch.randint(0, SMALL.vocab, (6, 700), generator=g).cuda()
+    toks[:, :400] = toks[0, :400]
+
+    def check(logits, order, lens):
+        for x, s in zip(logits, order):
+            want = model.prefill(toks[s:s + 1, :lens[s]], NHDCache(SMALL, 1, lens[s], dtype, "cuda"))[0]
+            assert (x - want).abs().max() <= 0.05 * want.abs().max()
+
+    cache = _model_cache(SMALL, "cuda", dtype, num_pages=400, page_size=16, max_len=700)
+    gone, first = cache.add([500, 0])
+    check(model.extend(toks[:1, :400], cache, [first]), [0], [400])
+    seqs = [first, *cache.fork(first, 5)]
+    new = [1, 150, 40, 7, 64, 3]
+    lens = [400 + n for n in new]
+    packed = torch.cat([toks[s, 400:n] for s, n in enumerate(lens)])
+    check(model.extend(packed, cache, seqs, new, mlp_chunk=100), range(6), lens)
+    cache.free([gone])
+    assert cache.compact() == cache.used_pages == 25 + sum(-(-n // 16) - 25 for n in lens)
+    for i in range(3):
+        logits = model.extend(torch.stack([toks[s, n] for s, n in enumerate(lens)]), cache, seqs, 1,
+                              backend=ExactDecodeBackend() if i == 1 else None)
+        lens = [n + 1 for n in lens]
+        check(logits, range(6), lens)
+
+
+def test_sampled_backends_read_the_cache():
+    """santa_flash over the rows of a forked cache gives the bits it gives on the
+    same tokens stored contiguously, also through the model."""
+    print("\n[case] santa_flash over a forked cache", flush=True)
+    backend = ab.build_backends(["santa_flash"], santa_s=128, santa_seed=3, santa_block_n=None, flashinfer_mode="auto",
+                                flashinfer_use_tensor_cores=False)[0]
+    cache = PagedKVCache(1, 300, 16, kv_heads=2, head_dim=128, max_seqs=4, max_len=1200)
+    a, = cache.add([1000])
+    cache.k[0].normal_()
+    cache.v[0].normal_()
+    b, = cache.fork(a)
+    cache.extend([b], 37)
+    q = torch.randn(2, 8, 128, device="cuda").bfloat16()
+    got = backend.decode_paged(q, cache.k[0], cache.v[0], cache.tables([b, a]), [1037, 1000])
+    at = torch.arange(1037, device="cuda")
+    flat = [torch.stack([t[cache.block_table[s, at.clamp_max(n - 1) // 16].long(), at.clamp_max(n - 1) % 16]
+                         for s, n in ((b, 1037), (a, 1000))]) for t in (cache.k[0], cache.v[0])]
+    want = backend._unwrap_tensor_out(backend.module.decode_systematic_batched(q, *flat, 128, seed=3,
+                                                                               valid_len=[1037, 1000]))
+    assert torch.equal(got, want)
+    model = RandomLlama(SMALL, seed=1, std=0.05, device="cuda")
+    held = _model_cache(SMALL, "cuda", BF, num_pages=100, page_size=16, max_len=600)
+    s, = held.add([0])
+    model.extend(torch.arange(300, device="cuda")[None], held, [s])
+    logits = model.extend(torch.tensor([[5], [6]], device="cuda"), held, [s, *held.fork(s)], backend=backend)
+    assert logits.shape == (2, SMALL.vocab) and torch.isfinite(logits).all() and backend.actual_mode == "paged"
