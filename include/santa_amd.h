@@ -399,7 +399,8 @@ int santa_pages_apply(const santa_pages* p, const void* const* pools, int n_pool
  * device as it is) where it is not NULL. */
 typedef struct santa_paged_plan_info {
   int tokens;       /* queries: the sum of new_tokens */
-  int items;        /* workgroups per KV head */
+  int groups;       /* workgroups per KV head, and the items they work through */
+  int items;
   int merge_tokens; /* tokens whose output is joined from parts */
   int max_len, max_row; /* what the block table has to hold */
   int heads, kv_heads;
@@ -416,7 +417,8 @@ int santa_paged_plan(const int* lens, const int* new_tokens, const int* rows, in
  * zeros.  out [tokens, H, D] contiguous.  strides: 8 host values, q's token and
  * head strides, K's page, row and head strides and V's, in elements (multiples
  * of 8, the last dimension contiguous, the tensors 16-byte aligned).  plan: the
- * device copy of a plan with this info.  Page numbers are clamped to the pool.
+ * device copy of a plan with this info.  scale: positive and finite.  Page
+ * numbers are clamped to the pool.
  * Scores, softmax and sums in float32; the probabilities enter the second
  * product rounded to the 16-bit type or, where at most 16 rows share a pass
  * over a KV head's tokens, as the sum of two such values.  workspace:

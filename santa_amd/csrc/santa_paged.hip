@@ -184,25 +184,75 @@ __global__ __launch_bounds__(256) void rope_append_kernel(const uint16_t* __rest
 }
 
 // ----------------------------------------------------------------- attention
-constexpr int kWaves = 4;
-// Above this a maximum in log2 units is subtracted from the scores before they
-// are scaled: fma(score, scale, -round(max * scale)) is off by half an ulp of
-// the product, a factor common to a row's probabilities that up to here (2^-15)
-// leaves the largest of them 1 in either 16-bit type.
+constexpr int kWaves = 8;
+// Above this a row's reference in log2 units is subtracted from the scores before
+// they are scaled: fma(score, scale, -round(m * scale)) is off by half an ulp of
+// the product, up to here 2^-15, a factor common to the row's probabilities that
+// hardly moves what they are rounded to.
 constexpr float kExactMax = 512.0f;
-constexpr int kWaitVmem = 0x0f70;  // s_waitcnt vmcnt(0) alone
+constexpr int kBufWord3 = 0x00020000;  // raw buffer descriptor, gfx9 family
 
-// What invalid rows of a tile are read from.
-__device__ u32x4 g_zero_row[16];
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+
+// 16 bytes per lane from rs + off (this lane's byte offset) to LDS, 1 KiB from
+// byte `at` on in lane order.  As asm, because with the builtin the compiler
+// makes the next read of LDS wait for it, whatever it reads; it has no result in
+// registers, and the waits are the tile loop's own.
+__device__ __forceinline__ void load_lds16(i32x4 rs, uint32_t at, uint32_t off) {
+  uint32_t m0;  // kept as it was; the pause is the one that scalars written by the vector unit need before a load
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %1\n\ts_nop 4\n\tbuffer_load_dwordx4 %2, %3, 0 offen lds\n\t"
+               "s_mov_b32 m0, %0"
+               : "=&s"(m0)
+               : "s"(at), "v"(off), "s"(rs)
+               : "memory");
+}
 
 template <int D>
 struct Geometry {
-  static constexpr int kRow = 2 * D;               // bytes
-  static constexpr int kLanes = D / 8;             // lanes per row
-  static constexpr int kRows = 64 / kLanes;        // rows per load instruction
-  static constexpr int kGroups = kTile / kRows;    // load instructions per tile
-  static constexpr int kVecs = kTile * kLanes;     // 16-byte pieces per tile
+  static constexpr int kRow = 2 * D;                   // bytes
+  static constexpr int kLanes = D / 8;                 // lanes per row
+  static constexpr int kRows = 64 / kLanes;            // rows per load instruction
+  static constexpr int kLoads = 8 / kRows;             // load instructions per wave, tile and tensor
+  static constexpr int kVecs = kTile * kLanes;         // 16-byte pieces per K or V tile
+  static constexpr int kStages = 512 / D;              // tiles in LDS, 128 KiB of them
+  static constexpr int kStage = 2 * kVecs;             // pieces per stage: the K tile, the V tile
 };
+
+// Waits until at most N of this wave's loads are in flight (they land in order;
+// loads and stores the compiler has issued since only make it wait for more).
+template <int N>
+__device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"i"(N) : "memory");
+}
+
+// How far a row's largest score may exceed the one that its sums are relative to
+// before they are rescaled: with none, new maxima among 32 rows rescale most
+// tiles (a quarter more vector work); probabilities up to 2^8 round as well as
+// those up to 1.
+constexpr float kHeadroom = 8.0f;
+
+// acc + the eight 16-bit values of v.
+template <bool BF16>
+__device__ __forceinline__ float sum8(u32x4 v, float acc) {
+  typedef typename attn::Half8<BF16>::T H8;
+  const H8 x = __builtin_bit_cast(H8, v);
+  constexpr uint32_t kOnes = BF16 ? 0x3f803f80u : 0x3c003c00u;
+  const H8 one = __builtin_bit_cast(H8, u32x4{kOnes, kOnes, kOnes, kOnes});
+  if constexpr (BF16) {
+    acc = __builtin_amdgcn_fdot2_f32_bf16(x.s01, one.s01, acc, false);
+    acc = __builtin_amdgcn_fdot2_f32_bf16(x.s23, one.s01, acc, false);
+    acc = __builtin_amdgcn_fdot2_f32_bf16(x.s45, one.s01, acc, false);
+    return __builtin_amdgcn_fdot2_f32_bf16(x.s67, one.s01, acc, false);
+  } else {
+    acc = __builtin_amdgcn_fdot2(x.s01, one.s01, acc, false);
+    acc = __builtin_amdgcn_fdot2(x.s23, one.s01, acc, false);
+    acc = __builtin_amdgcn_fdot2(x.s45, one.s01, acc, false);
+    return __builtin_amdgcn_fdot2(x.s67, one.s01, acc, false);
+  }
+}
+
+template <class T>
+using Const = const __attribute__((address_space(4))) T;  // read through the scalar cache
 
 struct AttnArgs {
   const uint16_t* q;
@@ -212,89 +262,155 @@ struct AttnArgs {
   const Item* items;
   const int* list;
   Pages pg;
-  long long sq_t, sq_h;                  // elements
-  long long sk_p, sk_r, sk_h, sv_p, sv_r, sv_h;  // bytes
+  long long sq_t, sq_h;              // elements
+  long long sk_h, sv_h;              // bytes
+  uint32_t sk_p, sk_r, sv_p, sv_r;
   int KVH, GH;
   float scale_log2;
 };
 
-// What a lane loads of a tile: its piece of the rows n, n + 1, ... from the
-// tile's row0 on, one per load instruction.
-struct TileLoad {
-  const char *k, *v;         // this KV head in the pools
-  const int* table;          // the block table row
-  int row0, lrow, lslot;
-  int begin, end, last;
+// Where a workgroup's loads are: tile t of an item (in scalar registers), and
+// where this wave's eight tokens of 64 tiles lie in K and V, one tile a lane:
+// looked up tile by tile as scalars they would be waited for with the loop's
+// reads of LDS, and their addresses be formed by every wave.
+struct Cursor {
+  int begin, end, row, next;      // of the item
+  int begin2, end2, row2, next2;  // of the next one
+  int t, tiles;                   // of the item
+  int left;                       // tokens from this wave's first one of the tile to the end
+  uint32_t k_lo, k_hi, v_lo, v_hi;
+  bool more;                      // there is a tile
 };
 
-// Issues the loads of tile t into dst; nothing waits for them here.  A row's
-// 16-byte pieces are swizzled so that the reads of both tiles are without bank
-// conflicts.  Eight tokens from a multiple of eight on lie in one page.
-template <int D>
-__device__ __forceinline__ void load_tile(const AttnArgs& a, const TileLoad& w, u32x4* __restrict__ dst, int wave, int t,
-                                          int page) {
-  using G = Geometry<D>;
-  constexpr int GPW = G::kGroups / kWaves;
-  const int n = w.begin + t * kTile + w.row0;
-  page = in_pool(a.pg, page);
-  const int in_page = n & ((1 << a.pg.shift) - 1);
-  const char* kp = w.k + page * a.sk_p + in_page * a.sk_r;
-  const char* vp = w.v + page * a.sv_p + in_page * a.sv_r;
-#pragma unroll
-  for (int c = 0; c < GPW; ++c) {
-    const int g = GPW * wave + c;
-    const int pr = G::kRows * g + w.lrow;  // row of the tile in LDS
-    const int ks = 16 * (w.lslot ^ (D == 128 ? pr & 15 : (pr >> 1) & 7));
-    const int vs = 16 * (w.lslot ^ (D == 128 ? 4 * (pr & 3) : 4 * ((pr >> 1) & 1)));
-    const bool in = n + c < w.end;
-    const char* zero = reinterpret_cast<const char*>(g_zero_row);
-    const char* ka = in ? kp + c * a.sk_r + ks : zero + ks;
-    const char* va = in ? vp + c * a.sv_r + vs : zero + vs;
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)ka,
-                                     (__attribute__((address_space(3))) void*)(dst + 64 * g), 16, 0, 0);
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)va,
-                                     (__attribute__((address_space(3))) void*)(dst + G::kVecs + 64 * g), 16, 0, 0);
+struct Loader {
+  const char *k, *v;      // this KV head in the pools
+  Const<Item>* items;
+  const int* table;
+  long long stride;
+  int shift, num_pages, limit;  // limit: tokens a block table row can name
+  uint32_t sk_p, sk_r, sv_p, sv_r;
+  uint32_t stages;  // LDS byte address of this wave's part of the first stage
+  int wave;
+};
+
+__device__ __forceinline__ int tiles_of(int begin, int end) { return (end - begin + kTile - 1) / kTile; }
+
+__device__ __forceinline__ void look_up(const Loader& w, Cursor& c) {
+  const int n = min(c.begin + (c.t + static_cast<int>(threadIdx.x & 63)) * kTile + 8 * w.wave, min(c.end, w.limit) - 1);
+  const uint32_t page = min(max(w.table[c.row * w.stride + (n >> w.shift)], 0), w.num_pages - 1);
+  const uint32_t r = n & ((1 << w.shift) - 1) & ~7;
+  const uint64_t k = reinterpret_cast<uint64_t>(w.k) + static_cast<uint64_t>(page) * w.sk_p + static_cast<uint64_t>(r) * w.sk_r;
+  const uint64_t v = reinterpret_cast<uint64_t>(w.v) + static_cast<uint64_t>(page) * w.sv_p + static_cast<uint64_t>(r) * w.sv_r;
+  c.k_lo = static_cast<uint32_t>(k), c.k_hi = static_cast<uint32_t>(k >> 32) & 0xffff;
+  c.v_lo = static_cast<uint32_t>(v), c.v_hi = static_cast<uint32_t>(v >> 32) & 0xffff;
+  // waited for here, once in 64 tiles, and not at every use
+  asm volatile("" : "+v"(c.k_lo), "+v"(c.k_hi), "+v"(c.v_lo), "+v"(c.v_hi));
+}
+__device__ __forceinline__ void read_next(const Loader& w, Cursor& c) {
+  if (c.next < 0) return;
+  Const<Item>* it = w.items + c.next;
+  c.begin2 = it->begin, c.end2 = it->end, c.row2 = it->row, c.next2 = it->next;
+}
+// To the first tile of the next item that has one.
+__device__ __forceinline__ void enter_next(const Loader& w, Cursor& c) {
+  c.more = false;
+  while (c.next >= 0) {
+    c.begin = c.begin2, c.end = c.end2, c.row = c.row2, c.next = c.next2;
+    read_next(w, c);
+    if (c.end > c.begin) {
+      c.t = 0;
+      c.tiles = tiles_of(c.begin, c.end);
+      c.left = c.end - c.begin - 8 * w.wave;
+      c.more = true;
+      look_up(w, c);
+      return;
+    }
   }
 }
 
-// Running softmax of a wave's rows (one per lane of each half): the sum of
-// MB x 32 dims, the maximum of the raw scores and the mass of this half's
-// tokens.  mc: the maximum in log2 units, or 0 where the scores have it
-// subtracted (kExactMax); grows: the maximum, or -inf there, so that every tile's
-// scores pass that way.
+// Issues this wave's loads of the cursor's tile into a stage (tokens 8 wave ..
+// 8 wave + 7 of it, which lie in one page, so that their address is a scalar's)
+// and moves the cursor on; nothing waits for them here.  Rows past the end read
+// as zeros.  A row's 16-byte pieces are swizzled so that the reads of both
+// tiles are without bank conflicts.
+template <int D>
+__device__ __forceinline__ void load_tile(const Loader& w, Cursor& c, uint32_t stage, const uint32_t (&ko)[2],
+                                          const uint32_t (&vo)[2]) {
+  using G = Geometry<D>;
+  const int lane = c.t & 63;
+  int k_bytes = 7 * w.sk_r + 2 * D, v_bytes = 7 * w.sv_r + 2 * D;
+  if (c.left < 8) {
+    k_bytes = c.left > 0 ? (c.left - 1) * w.sk_r + 2 * D : 0;
+    v_bytes = c.left > 0 ? (c.left - 1) * w.sv_r + 2 * D : 0;
+  }
+  const i32x4 rk{static_cast<int>(__builtin_amdgcn_readlane(c.k_lo, lane)),
+                 static_cast<int>(__builtin_amdgcn_readlane(c.k_hi, lane)), k_bytes, kBufWord3};
+  const i32x4 rv{static_cast<int>(__builtin_amdgcn_readlane(c.v_lo, lane)),
+                 static_cast<int>(__builtin_amdgcn_readlane(c.v_hi, lane)), v_bytes, kBufWord3};
+  const uint32_t at = w.stages + 16 * G::kStage * stage;
+#pragma unroll
+  for (int i = 0; i < G::kLoads; ++i) {
+    load_lds16(rk, at + 1024 * i, ko[i]);
+    load_lds16(rv, at + 1024 * i + 16 * G::kVecs, vo[i]);
+  }
+  c.left -= kTile;
+  if (++c.t == c.tiles) enter_next(w, c);
+  else if ((c.t & 63) == 0) look_up(w, c);
+}
+
+// Running softmax of a wave's rows (one per lane of each half): the sum of MB x
+// 32 dims and the mass of this half's tokens, relative to m, a score that the
+// row's largest exceeds by less than kHeadroom (log2 units).  mc: m in log2
+// units; grows: the score above which m moves up; exact: some row's mc is too
+// large to scale the scores before m is subtracted (kExactMax).
 template <int MB>
 struct State {
   f32x16 o[MB];
   float m, l, mc, grows;
+  bool exact;
 };
 
-// One tile: scores S^T = K Q^T of 32 KB tokens x 32 rows, softmax, and
-// O^T += V^T P^T.  n0 and lim: the tile's first token and the last one that the
-// lane's row attends to.
-template <bool BF16, int D, int KB, int MB>
-__device__ __forceinline__ void attend_tile(const char* __restrict__ buf, const u32x4 (&qf)[D / 16],
-                                            const uint32_t (&ko)[D / 16], const uint32_t (&vo)[MB], int kh, int n0,
-                                            int lim, int lim_lo, bool dup, float scale_log2, State<MB>& st) {
-  using G = Geometry<D>;
-  const int lane = threadIdx.x & 63, half = lane >> 5;
-  f32x16 s[KB];
+// Scores S^T = K Q^T of a tile's 32 KB tokens x 32 rows.  The first fragments of
+// K are all asked for before the first product, the rest one by one beside the
+// products: left to itself the compiler reads, waits and multiplies in turn.
+template <bool BF16, int D, int KB>
+__device__ __forceinline__ void scores(const char* buf, const u32x4 (&qf)[D / 16], const uint32_t (&ko)[D / 16],
+                                       f32x16 (&s)[KB]) {
+  u32x4 k[KB][D / 16];
+#pragma unroll
+  for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+    for (int c = 0; c < D / 16; ++c)
+      k[kb][c] = *reinterpret_cast<const u32x4*>(buf + ko[c] + 32 * Geometry<D>::kRow * kb);
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) s[kb][e] = 0.0f;
 #pragma unroll
-    for (int c = 0; c < D / 16; ++c)
-      s[kb] = mfma32<BF16>(*reinterpret_cast<const u32x4*>(buf + ko[c] + 32 * G::kRow * kb), qf[c], s[kb]);
+    for (int c = 0; c < D / 16; ++c) s[kb] = mfma32<BF16>(k[kb][c], qf[c], s[kb]);
   }
-  if (n0 + kTile - 1 > lim_lo) {  // tokens that some row does not attend to
+  __builtin_amdgcn_sched_group_barrier(0x100, D / 16, 0);  // LDS reads
+#pragma unroll
+  for (int i = 0; i < D / 16 * (KB - 1); ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix products
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x008, D / 16, 0);
+}
+
+// Their softmax: P^T in the 16-bit type, the running state moved on.  n0: the
+// first token; lim: the last one that the lane's row attends to, lim_lo the least
+// of the wave's rows.  dup: up to 16 rows.
+template <bool BF16, int KB, int MB>
+__device__ __forceinline__ void softmax(f32x16 (&s)[KB], u32x4 (&p)[2 * KB], int n0, int lim, int lim_lo, bool dup,
+                                        float scale_log2, State<MB>& st) {
+  const int lane = threadIdx.x & 63, half = lane >> 5;
+  if (n0 + 32 * KB - 1 > lim_lo) {  // tokens that some row does not attend to
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int pr = 32 * (kh + kb) + 8 * (e >> 2) + 4 * half + (e & 3);
-        const int n = n0 + G::kGroups * (pr % G::kRows) + pr / G::kRows;
-        if (n > lim) s[kb][e] = -__builtin_inff();
-      }
+      for (int e = 0; e < 16; ++e)
+        if (n0 + 32 * kb + 8 * (e >> 2) + 4 * half + (e & 3) > lim) s[kb][e] = -__builtin_inff();
   }
   float mx = s[0][0];
 #pragma unroll
@@ -302,34 +418,33 @@ __device__ __forceinline__ void attend_tile(const char* __restrict__ buf, const 
 #pragma unroll
     for (int e = 0; e < 16; ++e) mx = fmaxf(mx, s[kb][e]);
   mx = fmaxf(mx, other_half(mx));
-  const float m_new = fmaxf(st.m, mx);
-  if (__any(m_new > st.grows)) {
-    const float w = __builtin_amdgcn_exp2f((st.m - m_new) * scale_log2);
+  const bool up = mx > st.grows;
+  if (__any(up)) {
+    const float m = up ? fmaxf(st.m, mx) : st.m;
+    const float w = __builtin_amdgcn_exp2f((st.m - m) * scale_log2);
     st.l *= w;
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
       for (int e = 0; e < 16; ++e) st.o[mb][e] *= w;
-    st.grows = st.m = m_new;
-    st.mc = st.m * scale_log2;
-    if (__any(fabsf(st.mc) > kExactMax)) {
-#pragma unroll
-      for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) s[kb][e] -= st.m;
-      st.mc = 0.0f;
-      st.grows = -__builtin_inff();
-    }
+    st.m = m;
+    st.mc = m * scale_log2;
+    if (up) st.grows = m + kHeadroom / scale_log2;
+    st.exact = __any(fabsf(st.mc) > kExactMax);
   }
-  u32x4 p[2 * KB];
+  float mc = st.mc;
+  if (st.exact) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) s[kb][e] -= st.m;
+    mc = 0.0f;
+  }
 #pragma unroll
   for (int kc = 0; kc < 2 * KB; ++kc) {
     float e[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      e[j] = __builtin_amdgcn_exp2f(fmaf(s[kc >> 1][8 * (kc & 1) + j], scale_log2, -st.mc));
-      st.l += e[j];
-    }
+    for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(s[kc >> 1][8 * (kc & 1) + j], scale_log2, -mc));
     p[kc] = pack8<BF16>(e);
     // up to 16 rows leave lanes 16 .. 31 of the wave free: they hold the same
     // rows again, and carry what rounding took from their probabilities
@@ -342,73 +457,81 @@ __device__ __forceinline__ void attend_tile(const char* __restrict__ buf, const 
       const u32x4 low = pack8<BF16>(e);
       if (lane & 16) p[kc] = low;
     }
+    // the mass of the probabilities as rounded: a row's weights sum to 1, and one
+    // that attends to one token gives its value
+    st.l = sum8<BF16>(p[kc], st.l);
   }
+}
+
+// O^T += V^T P^T over MB x 32 dims; the reads of V run ahead of the products as
+// those of K do.
+template <bool BF16, int D, int KB, int MB>
+__device__ __forceinline__ void sums(const char* buf, const uint32_t (&vo)[MB], const u32x4 (&p)[2 * KB],
+                                     State<MB>& st) {
+  using G = Geometry<D>;
+  constexpr int N = 2 * KB * MB, kAhead = N < 4 ? N : 4;
+  u32x4 v[2 * KB][MB];
 #pragma unroll
   for (int kc = 0; kc < 2 * KB; ++kc)
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb)
-      st.o[mb] = mfma32<BF16>(read_tr8<G::kRow>(buf + vo[mb] + 16 * G::kRow * kc), p[kc], st.o[mb]);
-}
-
-// The next tile's loads and this tile's work.  The buffers are told apart by
-// their restrict qualifiers: without them the compiler makes the first read of
-// this tile wait for the loads of the next.
-template <bool BF16, int D, int KB, int MB>
-__device__ __forceinline__ void step(const char* __restrict__ cur, u32x4* __restrict__ next, bool more,
-                                     const AttnArgs& a, const TileLoad& w, int wave, int t, int& page, bool busy,
-                                     const u32x4 (&qf)[D / 16], const uint32_t (&ko)[D / 16], const uint32_t (&vo)[MB],
-                                     int kh, int lim, int lim_lo, bool dup, State<MB>& st) {
-  if (more) {
-    load_tile<D>(a, w, next, wave, t + 1, page);
-    page = w.table[min(w.begin + (t + 2) * kTile + w.row0, w.last) >> a.pg.shift];
+    for (int mb = 0; mb < MB; ++mb) v[kc][mb] = read_tr8<G::kRow>(buf + vo[mb] + 16 * G::kRow * kc);
+#pragma unroll
+  for (int kc = 0; kc < 2 * KB; ++kc)
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) st.o[mb] = mfma32<BF16>(v[kc][mb], p[kc], st.o[mb]);
+  __builtin_amdgcn_sched_group_barrier(0x100, 2 * kAhead, 0);  // LDS reads
+#pragma unroll
+  for (int i = 0; i < N - kAhead; ++i) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix products
+    __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
   }
-  if (busy)
-    attend_tile<BF16, D, KB, MB>(cur, qf, ko, vo, kh, w.begin + t * kTile, lim, lim_lo, dup, a.scale_log2, st);
+  __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
 }
 
-// The passes of one wave over its item's tiles, and its output.  SPLIT: the four
-// waves hold the same rows (up to 32) and take two halves of each tile's
-// tokens times two halves of the dims; else each has its own 32 rows.
-template <bool BF16, int D, bool SPLIT>
-__device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv,
-                                       u32x4 (*s_kv)[2 * Geometry<D>::kVecs]) {
+// The workgroup's barrier alone: no wave waits for its loads here.
+__device__ __forceinline__ void barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// LDS beside the stages, for what the waves of the same rows and dims hold of
+// different tokens.
+struct Shares {
+  float o[6][16][64], m[6][64], l[6][64];
+};
+
+// One item.  Its rows are RG groups of 32, each held by 8 / RG waves.  RG 8: one
+// wave has all of a tile.  4: two waves, each a half of its tokens.  2: four
+// waves, each a half of its tokens and of the dims.  1: eight waves, each a half
+// of the dims and a quarter of the tokens of two tiles (with four waves to a
+// tile, its latency, not HBM, would bound the pass).  tile: the number of the
+// item's first tile, loaded: that of the next one to be loaded, counted over the
+// workgroup's items.
+template <bool BF16, int D, int RG>
+__device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv, const Loader& w, Cursor& cur,
+                                       const uint32_t (&lk)[2], const uint32_t (&lv)[2], uint32_t& tile, uint32_t& loaded,
+                                       u32x4* stages, Shares* x) {
   using G = Geometry<D>;
-  constexpr int KB = SPLIT ? 1 : 2;
-  constexpr int MB = SPLIT ? D / 64 : D / 32;
-  const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int half = lane >> 5, ql = lane & 31;
-  const int kh = SPLIT ? wave & 1 : 0, dh = SPLIT ? wave >> 1 : 0;
-  const bool dup = SPLIT && it.rows <= 16;
+  constexpr int KB = RG == 8 ? 2 : 1;                       // 32s of a tile's tokens that a wave takes
+  constexpr int DH = RG >= 4 ? 1 : 2, MB = D / 32 / DH;     // parts of the dims, 32s of them in each
+  constexpr int TG = RG == 8 ? 1 : RG == 1 ? 4 : 2;         // parts of the tokens
+  constexpr int kStep = RG == 1 ? 2 : 1;                    // tiles at once
+  const int lane = threadIdx.x & 63, half = lane >> 5, ql = lane & 31;
+  const int wave = w.wave;
+  const int dh = DH == 1 ? 0 : wave & 1, tg = wave / DH % TG, rg = wave / (DH * TG);
+  const int kh = TG == 1 ? 0 : tg & 1;                      // half of a tile
+  const bool dup = RG == 1 && it.rows <= 16;
 
   // this lane's row
-  const int r = dup ? ql & 15 : SPLIT ? ql : 32 * wave + ql;
-  const bool active = r < it.rows;
+  const int r = dup ? ql & 15 : 32 * rg + ql;
   const int rc = min(r, it.rows - 1);
   const int i = rc / a.GH, h = kv * a.GH + (rc - i * a.GH);
   const int tok = it.flags & kFromList ? a.list[it.tok0 + i] : it.tok0 + i;
   const int pos = it.pos0 + i;
   const int lim = min(it.end - 1, pos);  // last position this row attends to here
   const int lim_lo = __builtin_amdgcn_readlane(lim, 0), lim_hi = __builtin_amdgcn_readlane(lim, 31);
-  const bool any = SPLIT || 32 * wave < it.rows;
-
-  TileLoad w;
-  w.k = a.k + kv * a.sk_h;
-  w.v = a.v + kv * a.sv_h;
-  w.table = a.pg.table + it.row * a.pg.stride;
-  w.lrow = lane / G::kLanes;
-  w.lslot = lane % G::kLanes;
-  w.row0 = G::kGroups * w.lrow + G::kGroups / kWaves * wave;
-  w.begin = it.begin;
-  w.end = it.end;
-  w.last = static_cast<int>(min(static_cast<long long>(it.end), a.pg.stride << a.pg.shift)) - 1;
-  const int nt = (it.end - it.begin + kTile - 1) / kTile;
-  int page = 0;
-  if (nt > 0) {
-    page = w.table[min(w.begin + w.row0, w.last) >> a.pg.shift];
-    load_tile<D>(a, w, s_kv[0], wave, 0, page);
-    page = w.table[min(w.begin + kTile + w.row0, w.last) >> a.pg.shift];
-  }
+  const bool any = 32 * rg < it.rows;
 
   // Q fragments: dims 16c + 8 half .. + 7 of this lane's row
   u32x4 qf[D / 16];
@@ -417,7 +540,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) qf[c] = *reinterpret_cast<const u32x4*>(qr + 16 * c);
   }
-  // LDS byte offsets of this lane's fragments inside a buffer
+  // LDS byte offsets of this lane's fragments inside a stage
   uint32_t ko[D / 16], vo[MB];
 #pragma unroll
   for (int c = 0; c < D / 16; ++c)
@@ -438,45 +561,86 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv
   st.m = kLowest;
   st.l = st.mc = 0.0f;
   st.grows = -__builtin_inff();
-  for (int t = 0; t < nt; ++t) {
-    __builtin_amdgcn_s_waitcnt(kWaitVmem);
-    __syncthreads();  // tile t is in LDS, and no wave reads the other buffer any more
-    step<BF16, D, KB, MB>(reinterpret_cast<const char*>(s_kv[t & 1]), s_kv[(t + 1) & 1], t + 1 < nt, a, w, wave, t,
-                          page, any && w.begin + t * kTile <= lim_hi, qf, ko, vo, kh, lim, lim_lo, dup, st);
+  st.exact = false;
+  // Q has landed: known here, it is not waited for in every tile
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0) alone
+  const int nt = tiles_of(it.begin, it.end);
+  // tiles in which a row of this wave attends to a token
+  const int busy = any && lim_hi >= it.begin ? min(nt, (lim_hi - it.begin) / kTile + 1) : 0;
+  for (int t = 0; t < nt; t += kStep) {
+    // this wave's loads of the step's tiles have landed (those of newer ones need
+    // not have), then all waves' have, and no wave reads the tiles before any more
+    const int newer = static_cast<int>(loaded - tile) - min(kStep, nt - t);
+    constexpr int kMost = G::kStages - 1 - kStep, kSome = kMost / 2;
+    if (newer >= kMost) wait_loads<2 * G::kLoads * kMost>();
+    else if (newer >= kSome) wait_loads<2 * G::kLoads * kSome>();
+    else wait_loads<0>();
+    barrier();
+    while (cur.more && loaded - tile < G::kStages)
+      load_tile<D>(w, cur, loaded++ % G::kStages, lk, lv);
+    const int mine = kStep == 1 ? 0 : tg >> 1;
+    if (t + mine < busy) {
+      const char* stage = reinterpret_cast<const char*>(stages + ((tile + mine) % G::kStages) * G::kStage);
+      f32x16 s[KB];
+      u32x4 p[2 * KB];
+      scores<BF16, D, KB>(stage, qf, ko, s);
+      softmax<BF16, KB, MB>(s, p, it.begin + (t + mine) * kTile + 32 * kh, lim, lim_lo, dup, a.scale_log2, st);
+      sums<BF16, D, KB, MB>(stage, vo, p, st);
+    }
+    tile += min(kStep, nt - t);
   }
   float m = st.m, l = st.l + other_half(st.l);
   f32x16(&o)[MB] = st.o;
-  if constexpr (SPLIT) {
-    if (dup) {
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[mb][e] += fxor<16>(o[mb][e], lane);
-    }
-    // the two halves of the tokens
-    float* const x = reinterpret_cast<float*>(s_kv) + dh * (16 * MB + 2) * 64 + lane;
-    __syncthreads();  // no wave reads a tile any more
-    if (kh == 1) {
-#pragma unroll
-      for (int mb = 0; mb < MB; ++mb)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) x[(16 * mb + e) * 64] = o[mb][e];
-      x[16 * MB * 64] = m;
-      x[(16 * MB + 1) * 64] = l;
-    }
-    __syncthreads();
-    if (kh == 1) return;
-    const float m2 = x[16 * MB * 64], top = fmaxf(m, m2);
-    const float w1 = __builtin_amdgcn_exp2f((m - top) * a.scale_log2), w2 = __builtin_amdgcn_exp2f((m2 - top) * a.scale_log2);
-    m = top;
-    l = l * w1 + x[(16 * MB + 1) * 64] * w2;
+  if (dup) {  // an infinite value is whole in the first part, and times 0 or less in the second
+    l += fxor<16>(l, lane);
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) o[mb][e] = o[mb][e] * w1 + x[(16 * mb + e) * 64] * w2;
-    if (dup && (ql & 16)) return;
+      for (int e = 0; e < 16; ++e) {
+        const float low = fxor<16>(o[mb][e], lane);
+        o[mb][e] += fabsf(low) < __builtin_inff() ? low : 0.0f;
+      }
   }
-  if (!active) return;
+  if constexpr (TG > 1) {  // the parts of the tokens
+    const int first = (wave % DH + DH * rg) * (TG - 1);
+    if (tg > 0) {
+      x->m[first + tg - 1][lane] = m;
+      x->l[first + tg - 1][lane] = l;
+    }
+    float own = 0.0f, weight[TG - 1];
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      if (tg > 0) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) x->o[first + tg - 1][e][lane] = o[mb][e];
+      }
+      __syncthreads();
+      if (tg == 0) {
+        if (mb == 0) {
+          float top = m;
+#pragma unroll
+          for (int i = 0; i < TG - 1; ++i) top = fmaxf(top, x->m[first + i][lane]);
+          own = __builtin_amdgcn_exp2f((m - top) * a.scale_log2);
+          l *= own;
+          m = top;
+#pragma unroll
+          for (int i = 0; i < TG - 1; ++i) {
+            weight[i] = __builtin_amdgcn_exp2f((x->m[first + i][lane] - top) * a.scale_log2);
+            l = fmaf(x->l[first + i][lane], weight[i], l);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          o[mb][e] *= own;
+#pragma unroll
+          for (int i = 0; i < TG - 1; ++i) o[mb][e] = fmaf(x->o[first + i][e][lane], weight[i], o[mb][e]);
+        }
+      }
+      __syncthreads();
+    }
+    if (tg > 0 || (dup && (ql & 16))) return;
+  }
+  if (!any || r >= it.rows) return;
   if (it.flags & kDirect) {
     const float inv = pos < 0 ? 0.0f : 1.0f / l;
     uint16_t* orow = a.out + (static_cast<size_t>(tok) * (a.KVH * a.GH) + h) * D + 32 * MB * dh;
@@ -484,10 +648,10 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
-        uint2 w;
-        w.x = f32_to_h16<BF16>(o[mb][e] * inv) | (static_cast<uint32_t>(f32_to_h16<BF16>(o[mb][e + 1] * inv)) << 16);
-        w.y = f32_to_h16<BF16>(o[mb][e + 2] * inv) | (static_cast<uint32_t>(f32_to_h16<BF16>(o[mb][e + 3] * inv)) << 16);
-        *reinterpret_cast<uint2*>(orow + 32 * mb + 2 * e + 4 * half) = w;
+        uint2 v;
+        v.x = f32_to_h16<BF16>(o[mb][e] * inv) | (static_cast<uint32_t>(f32_to_h16<BF16>(o[mb][e + 1] * inv)) << 16);
+        v.y = f32_to_h16<BF16>(o[mb][e + 2] * inv) | (static_cast<uint32_t>(f32_to_h16<BF16>(o[mb][e + 3] * inv)) << 16);
+        *reinterpret_cast<uint2*>(orow + 32 * mb + 2 * e + 4 * half) = v;
       }
     return;
   }
@@ -502,84 +666,140 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv
   if (dh == 0 && half == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * rec) = make_float2(m, l);
 }
 
-template <bool BF16, int D>
-__global__ __launch_bounds__(256, 2) void paged_attention_kernel(AttnArgs a, int first_item) {
-  __shared__ u32x4 s_kv[2][2 * Geometry<D>::kVecs];  // per buffer: the K tile, the V tile
-  const int kv = blockIdx.x % a.KVH;
-  const Item it = a.items[first_item + blockIdx.x / a.KVH];
-  if (it.rows <= 0) return;
-  if (it.rows <= 32)
-    attend<BF16, D, true>(a, it, kv, s_kv);
-  else
-    attend<BF16, D, false>(a, it, kv, s_kv);
+__device__ __forceinline__ Item read_item(const Loader& w, int i) {
+  Const<Item>* p = w.items + i;
+  Item it;
+  it.flags = p->flags, it.row = p->row, it.begin = p->begin, it.end = p->end, it.tok0 = p->tok0, it.rows = p->rows;
+  it.pos0 = p->pos0, it.base = p->base, it.next = p->next;
+  return it;
 }
 
-// Joins the parts of one (token, head): 256 threads, the parts spread over
-// them for the maximum and the weights, then 256 / (D / 2) groups of D / 2
-// threads, two dims each, over the parts in turn.
-constexpr int kMergeThreads = 256;
-
 template <bool BF16, int D>
-__global__ __launch_bounds__(kMergeThreads) void merge_kernel(const float* __restrict__ part,
-                                                              const float2* __restrict__ part_ml,
-                                                              const int* __restrict__ tokens,
-                                                              const int4* __restrict__ parts,
-                                                              const int2* __restrict__ pos, int first_token, int H,
-                                                              int KVH, float scale_log2, uint16_t* __restrict__ out) {
-  constexpr int kThreads = D / 2, kTeams = kMergeThreads / kThreads;
-  __shared__ float s_w[kMergeThreads];
-  __shared__ float s_red[2][4];
-  __shared__ float2 s_o[kTeams][kThreads];
-  const int tok = tokens[first_token + blockIdx.x / H];
-  if (tok < 0) return;
-  const int h = blockIdx.x % H, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int kv = h / (H / KVH), g = h % (H / KVH);
-  const int4 pa = parts[2 * tok], pb = parts[2 * tok + 1];  // base, rows, local, splits
-  const int n = pb.w > 0 ? pa.w + pb.w : 0;
-  if (n == 0) return;  // written by its item
-  auto record = [&](int j) {
-    const int4 p = j < pa.w ? pa : pb;
-    return static_cast<size_t>(p.x) + (static_cast<size_t>(j < pa.w ? j : j - pa.w) * KVH + kv) * p.y + p.z + g;
-  };
-  float mx = kLowest;
-  for (int j = tid; j < n; j += kMergeThreads) mx = fmaxf(mx, part_ml[record(j)].x);
+__global__ __launch_bounds__(64 * kWaves, 2) void paged_attention_kernel(AttnArgs a) {
+  using G = Geometry<D>;
+  __shared__ u32x4 stages[G::kStages * G::kStage];
+  __shared__ Shares shares;
+  const int kv = blockIdx.x % a.KVH, group = blockIdx.x / a.KVH;
+  const int lane = threadIdx.x & 63;
+  Loader w;
+  w.wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  w.k = a.k + kv * a.sk_h;
+  w.v = a.v + kv * a.sv_h;
+  w.items = (Const<Item>*)a.items;
+  w.table = a.pg.table;
+  w.stride = a.pg.stride;
+  w.shift = a.pg.shift;
+  w.num_pages = a.pg.num_pages;
+  w.limit = static_cast<int>(min(a.pg.stride << a.pg.shift, 0x7fffffffLL));
+  w.sk_p = a.sk_p, w.sk_r = a.sk_r, w.sv_p = a.sv_p, w.sv_r = a.sv_r;
+  w.stages = __builtin_amdgcn_readfirstlane(
+                 static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) void*)stages))) +
+             1024 * G::kLoads * w.wave;
+  uint32_t lk[2], lv[2];
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
-  if (lane == 0) s_red[0][wave] = mx;
-  __syncthreads();
-  mx = fmaxf(fmaxf(s_red[0][0], s_red[0][1]), fmaxf(s_red[0][2], s_red[0][3]));
-  const int team = tid / kThreads, d2 = tid % kThreads;
-  float z = 0.0f;
-  float2 acc = make_float2(0.0f, 0.0f);
-  for (int j0 = 0; j0 < n; j0 += kMergeThreads) {
-    __syncthreads();  // the weights of the parts before are used up
-    if (j0 + tid < n) {
-      const float2 ml = part_ml[record(j0 + tid)];
-      const float w = __builtin_amdgcn_exp2f((ml.x - mx) * scale_log2);
-      s_w[tid] = w;
-      z = fmaf(w, ml.y, z);
-    }
-    __syncthreads();
-    const int k = min(kMergeThreads, n - j0);
-#pragma unroll 8
-    for (int j = team; j < k; j += kTeams) {
-      const float2 v = *reinterpret_cast<const float2*>(part + record(j0 + j) * D + 2 * d2);
-      acc.x = fmaf(s_w[j], v.x, acc.x);
-      acc.y = fmaf(s_w[j], v.y, acc.y);
+  for (int i = 0; i < 2; ++i) {
+    const int row = G::kRows * i + lane / G::kLanes, slot = lane % G::kLanes;
+    const int pr = 8 * w.wave + row;  // row of the tile
+    lk[i] = row * a.sk_r + 16 * (slot ^ (D == 128 ? pr & 15 : (pr >> 1) & 7));
+    lv[i] = row * a.sv_r + 16 * (slot ^ (D == 128 ? 4 * (pr & 3) : 4 * ((pr >> 1) & 1)));
+  }
+  Cursor c;
+  c.next = group;
+  const int item = c.next;
+  uint32_t tile = 0, loaded = 0;
+  read_next(w, c);
+  enter_next(w, c);
+  for (; loaded < G::kStages - 1 && c.more; ++loaded)
+    load_tile<D>(w, c, loaded, lk, lv);
+  Item it = read_item(w, item);
+  for (bool last = false; !last && it.rows > 0;) {
+    const Item now = it;
+    last = now.next < 0;
+    if (!last) it = read_item(w, now.next);  // while this one is worked on
+    if (now.rows <= 32) attend<BF16, D, 1>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares);
+    else if (now.rows <= 64) attend<BF16, D, 2>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares);
+    else if (now.rows <= 128) attend<BF16, D, 4>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares);
+    else attend<BF16, D, 8>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares);
+  }
+}
+
+// Joins the parts of one (token, head): W waves, each every W-th part, a lane two
+// dims (D 64: the two halves of a wave take parts in turn).
+template <bool BF16, int D, int W>
+__global__ __launch_bounds__(256) void merge_kernel(const float* __restrict__ part, const float2* __restrict__ part_ml,
+                                                    const int* __restrict__ tokens, const int4* __restrict__ parts,
+                                                    const int2* __restrict__ pos, int first_row, int rows, int H,
+                                                    int KVH, float scale_log2, uint16_t* __restrict__ out) {
+  constexpr int kTeam = D / 2, kTeams = 64 / kTeam;  // lanes per part, parts per wave at once
+  __shared__ float s_m[4], s_z[4];
+  __shared__ float2 s_o[4][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int row = W == 1 ? 4 * blockIdx.x + wave : blockIdx.x;
+  int tok = -1, n = 0, h = 0;
+  int4 pa{}, pb{};  // base, rows, local, splits
+  if (row < rows) {
+    tok = tokens[(first_row + row) / H];
+    h = (first_row + row) % H;
+    if (tok >= 0) {
+      pa = parts[2 * tok], pb = parts[2 * tok + 1];
+      n = pb.w > 0 ? pa.w + pb.w : 0;  // 0: written by its item
     }
   }
+  const int kv = h / (H / KVH), g = h % (H / KVH);
+  auto record = [&](int j) {
+    const bool first = j < pa.w;
+    return static_cast<size_t>(first ? pa.x : pb.x) +
+           (static_cast<size_t>(first ? j : j - pa.w) * KVH + kv) * (first ? pa.y : pb.y) + (first ? pa.z : pb.z) + g;
+  };
+  const int w = W == 1 ? 0 : wave, team = lane / kTeam, d2 = lane % kTeam;
+  float mx = kLowest;
+  for (int j = lane * W + w; j < n; j += 64 * W) mx = fmaxf(mx, part_ml[record(j)].x);
 #pragma unroll
-  for (int d = 32; d > 0; d >>= 1) z += __shfl_xor(z, d, 64);
-  if (lane == 0) s_red[1][wave] = z;
-  s_o[team][d2] = acc;
-  __syncthreads();
-  if (team > 0) return;
-  z = (s_red[1][0] + s_red[1][1]) + (s_red[1][2] + s_red[1][3]);
+  for (int d = 32; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
+  if constexpr (W > 1) {
+    if (lane == 0) s_m[wave] = mx;
+    __syncthreads();
+    mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+  }
+  float z = 0.0f;
+  float2 acc = make_float2(0.0f, 0.0f);
+  constexpr int kBatch = 8;
+  for (int j0 = w + team * W; j0 < n; j0 += kBatch * kTeams * W) {
+    float2 ml[kBatch], v[kBatch];
 #pragma unroll
-  for (int k = 1; k < kTeams; ++k) acc.x += s_o[k][d2].x, acc.y += s_o[k][d2].y;
+    for (int b = 0; b < kBatch; ++b) {
+      const int j = j0 + b * kTeams * W;
+      const size_t rec = record(min(j, n - 1));
+      ml[b] = part_ml[rec];
+      v[b] = *reinterpret_cast<const float2*>(part + rec * D + 2 * d2);
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b)
+      if (j0 + b * kTeams * W < n) {
+        const float e = __builtin_amdgcn_exp2f((ml[b].x - mx) * scale_log2);
+        z = fmaf(e, ml[b].y, z);
+        acc.x = fmaf(e, v[b].x, acc.x);
+        acc.y = fmaf(e, v[b].y, acc.y);
+      }
+  }
+  if constexpr (kTeams == 2) {
+    z += other_half(z);
+    acc.x += other_half(acc.x);
+    acc.y += other_half(acc.y);
+  }
+  if constexpr (W > 1) {
+    if (lane == 0) s_z[wave] = z;
+    s_o[wave][lane] = acc;
+    __syncthreads();
+    if (wave > 0) return;
+    z = (s_z[0] + s_z[1]) + (s_z[2] + s_z[3]);
+#pragma unroll
+    for (int k = 1; k < W; ++k) acc.x += s_o[k][lane].x, acc.y += s_o[k][lane].y;
+  }
+  if (n == 0 || team > 0) return;
   const float inv = pos[tok].x < 0 ? 0.0f : 1.0f / z;
-  const uint32_t w = f32_to_h16<BF16>(acc.x * inv) | (static_cast<uint32_t>(f32_to_h16<BF16>(acc.y * inv)) << 16);
-  *reinterpret_cast<uint32_t*>(out + (static_cast<size_t>(tok) * H + h) * D + 2 * d2) = w;
+  const uint32_t v = f32_to_h16<BF16>(acc.x * inv) | (static_cast<uint32_t>(f32_to_h16<BF16>(acc.y * inv)) << 16);
+  *reinterpret_cast<uint32_t*>(out + (static_cast<size_t>(tok) * H + h) * D + 2 * d2) = v;
 }
 
 // A block table, pools and plan that belong together.
@@ -747,29 +967,49 @@ extern "C" int santa_paged_attention(const void* q, const void* k_pages, const v
   a.list = plan + info->list_at;
   a.pg = pg;
   a.sq_t = strides[0], a.sq_h = strides[1];
-  a.sk_p = 2 * strides[2], a.sk_r = 2 * strides[3], a.sk_h = 2 * strides[4];
-  a.sv_p = 2 * strides[5], a.sv_r = 2 * strides[6], a.sv_h = 2 * strides[7];
+  if (strides[2] >= 1LL << 31 || strides[5] >= 1LL << 31)
+    return set_error(SANTA_ERR_UNSUPPORTED, "paged_attention: pages must lie less than 4 GiB apart");
+  // rows past the end are told by their offset from the first of eight
+  if (strides[3] < D || strides[6] < D || strides[3] >= 1LL << 26 || strides[6] >= 1LL << 26)
+    return set_error(SANTA_ERR_UNSUPPORTED, "paged_attention: the rows of a page must lie at least D and less than 2^26 "
+                                            "elements apart");
+  a.sk_p = static_cast<uint32_t>(2 * strides[2]), a.sk_r = static_cast<uint32_t>(2 * strides[3]), a.sk_h = 2 * strides[4];
+  a.sv_p = static_cast<uint32_t>(2 * strides[5]), a.sv_r = static_cast<uint32_t>(2 * strides[6]), a.sv_h = 2 * strides[7];
   a.KVH = KVH;
   a.GH = H / KVH;
   a.scale_log2 = 1.44269504088896340736f * scale;
-  auto run = [&](auto attention, auto merge) {
-    // a launch holds fewer than 2^32 threads
-    const int step = (1 << 23) / std::max(H, KVH);
-    for (int i = 0; i < info->items; i += step)
-      hipLaunchKernelGGL(attention, dim3(static_cast<unsigned>(std::min(step, info->items - i) * KVH)), dim3(256), 0,
-                         stream, a, i);
-    for (int t = 0; t < info->merge_tokens; t += step)
-      hipLaunchKernelGGL(merge, dim3(static_cast<unsigned>(std::min(step, info->merge_tokens - t) * H)),
-                         dim3(kMergeThreads), 0, stream, a.part, reinterpret_cast<const float2*>(a.part_ml),
-                         plan + info->merge_at, reinterpret_cast<const int4*>(plan + info->parts_at),
-                         reinterpret_cast<const int2*>(plan + info->pos_at), t, H, KVH, a.scale_log2, a.out);
+  // maxima are those of the raw scores, and kHeadroom is divided by the scale
+  if (!(scale > 0.0f) || !std::isnormal(scale) || !std::isnormal(a.scale_log2))
+    return set_error(SANTA_ERR_INVALID, "paged_attention: scale must be positive and finite. Got scale=%g",
+                     static_cast<double>(scale));
+  auto run = [&](auto bf, auto dim) {
+    constexpr bool BF16 = decltype(bf)::value;
+    constexpr int kD = decltype(dim)::value;
+    if (info->groups > 0)  // one resident round
+      hipLaunchKernelGGL((paged_attention_kernel<BF16, kD>), dim3(static_cast<unsigned>(info->groups) * KVH),
+                         dim3(64 * kWaves), 0, stream, a);
+    const long long rows = static_cast<long long>(info->merge_tokens) * H;
+    // four waves a row while that leaves them one resident round
+    const bool wide = rows <= 2048;
+    for (long long r = 0; r < rows; r += 1 << 22) {  // a launch holds fewer than 2^32 threads
+      const int n = static_cast<int>(std::min<long long>(rows - r, 1 << 22));
+      auto merge = [&](auto kernel, int wgs) {
+        hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(wgs)), dim3(256), 0, stream, a.part,
+                           reinterpret_cast<const float2*>(a.part_ml), plan + info->merge_at,
+                           reinterpret_cast<const int4*>(plan + info->parts_at),
+                           reinterpret_cast<const int2*>(plan + info->pos_at), static_cast<int>(r), n, H, KVH,
+                           a.scale_log2, a.out);
+      };
+      if (wide) merge(merge_kernel<BF16, kD, 4>, n);
+      else merge(merge_kernel<BF16, kD, 1>, (n + 3) / 4);
+    }
   };
   if (dtype == SANTA_BF16) {
-    if (D == 128) run(paged_attention_kernel<true, 128>, merge_kernel<true, 128>);
-    else run(paged_attention_kernel<true, 64>, merge_kernel<true, 64>);
+    if (D == 128) run(std::true_type{}, std::integral_constant<int, 128>{});
+    else run(std::true_type{}, std::integral_constant<int, 64>{});
   } else {
-    if (D == 128) run(paged_attention_kernel<false, 128>, merge_kernel<false, 128>);
-    else run(paged_attention_kernel<false, 64>, merge_kernel<false, 64>);
+    if (D == 128) run(std::false_type{}, std::integral_constant<int, 128>{});
+    else run(std::false_type{}, std::integral_constant<int, 64>{});
   }
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(SANTA_ERR_HIP, "paged_attention launch failed: %s", hipGetErrorString(e));

@@ -2,6 +2,7 @@
 // (santa_paged.hip) is cut into workgroups.
 #include <algorithm>
 #include <climits>
+#include <cstddef>
 #include <cstdint>
 #include <cstring>
 #include <new>
@@ -23,15 +24,23 @@ struct Block {
   int tiles() const { return (end - begin + kTile - 1) / kTile; }
 };
 
-int div_up(long long a, long long b) { return static_cast<int>((a + b - 1) / b); }
+// What a tile costs a workgroup, by the rows of its block, and what a piece does
+// besides (its first loads, its output), in units of about 0.25 us.  With 64 or
+// fewer rows a tile takes as long as its 32 KiB do from HBM, with 256 as long as
+// its products.  All tiles alike and a piece like one: 122 us for 64 sequences
+// behind 32k tokens and 232 for 32 behind 128k (113 and 219 with these).
+constexpr int kPieceCost = 20;
+int tile_cost(int rows) { return rows > 128 ? 10 : rows > 64 ? 7 : 6; }
+// The fewest tiles that a block is cut off after.
+constexpr int kLeastCut = 2;
 
-// Workgroups that are resident at once, two per compute unit (their LDS).
+// Workgroups that are resident at once, one per compute unit (their LDS).
 int resident() {
   int dev = 0, cus = 0;
   if (hipGetDevice(&dev) != hipSuccess ||
       hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || cus <= 0)
     cus = 256;
-  return 2 * cus;
+  return cus;
 }
 
 struct Input {
@@ -68,7 +77,7 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
     if (in.shared[g] < 0 || in.shared[g] > std::max(0, n - t))
       return set_error(SANTA_ERR_INVALID, "%d tokens are not common to sequence %d: %d precede its new tokens",
                        in.shared[g], b, std::max(0, n - t));
-    if (t == 0) continue;
+    if (t == 0 || static_cast<long long>(t) * GH >= kBlockRows) continue;  // fills workgroups by itself
     if (lead[g] < 0) lead[g] = row;
     ++members[g];
     group_tokens[g] += t;
@@ -89,7 +98,7 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
     }
     group_list[g] = static_cast<int>(list.size());
     for (int b = 0; b < in.B; ++b)
-      if (in.group[b] == g) {
+      if (in.group[b] == g && static_cast<long long>(in.new_tokens[b]) * GH < kBlockRows) {
         prefix[b] = common;
         for (int i = 0; i < in.new_tokens[b]; ++i) list.push_back(first[b] + i);
       }
@@ -109,70 +118,74 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
     }
   }
 
-  // tiles per item: the fewest with which one resident round holds all items,
-  // or thirds of a round's worth where the blocks alone are more than that
+  // one resident round of workgroups, each with a run of whole tiles of about
+  // the same cost: the least with which they hold everything
   const int slots = std::max(1, resident() / in.kv_heads);
-  long long total = 0;
-  int most = 1;
-  for (const Block& k : blocks) {
-    total += k.tiles();
-    most = std::max(most, k.tiles());
-  }
-  auto count = [&](int c) {
-    long long n = 0;
-    for (const Block& k : blocks) n += std::max(1, div_up(k.tiles(), c));
-    return n;
+  struct Piece {
+    int block, t0, t1, slot;
   };
-  int chunk = std::max(kMinChunk, div_up(total, 3LL * slots));
-  if (count(most) <= slots) {
-    int lo = 1, hi = most;
-    while (lo < hi) {
-      const int mid = lo + (hi - lo) / 2;
-      if (count(mid) <= slots) hi = mid;
-      else lo = mid + 1;
+  std::vector<Piece> pieces;
+  auto pack = [&](long long budget, bool keep) {
+    int slot = 0;
+    long long left = budget;
+    for (size_t i = 0; i < blocks.size(); ++i) {
+      const int tiles = blocks[i].tiles(), cost = tile_cost(blocks[i].ntok * GH);
+      for (int t = 0; t < tiles || t == 0;) {
+        long long k = std::min<long long>(tiles - t, (left - kPieceCost) / cost);
+        if (left < budget && (k < 1 ? tiles > 0 || left < kPieceCost : k < tiles - t && k < kLeastCut)) {
+          if (++slot == slots) return false;
+          left = budget;
+          continue;
+        }
+        k = std::max<long long>(k, std::min(1, tiles));
+        if (keep) pieces.push_back({static_cast<int>(i), t, t + static_cast<int>(k), slot});
+        left -= kPieceCost + cost * k;
+        t += std::max(1, static_cast<int>(k));
+      }
     }
-    chunk = std::max(kMinChunk, lo);
+    return true;
+  };
+  long long total = 0;
+  for (const Block& k : blocks) total += kPieceCost + static_cast<long long>(tile_cost(k.ntok * GH)) * k.tiles();
+  long long lo = std::max<long long>(total / slots, kPieceCost + tile_cost(1) * kLeastCut), hi = lo;
+  while (!pack(hi, false)) lo = hi + 1, hi += std::max(1LL, hi / 4);
+  while (lo < hi) {
+    const long long mid = lo + (hi - lo) / 2;
+    if (pack(mid, false)) hi = mid;
+    else lo = mid + 1;
   }
-  const long long max_items = static_cast<long long>(blocks.size()) + 3LL * slots;
+  pack(hi, true);
+  const long long used = pieces.empty() ? 0 : pieces.back().slot + 1;
+  const long long max_items = static_cast<long long>(blocks.size()) + slots;
   if (max_items > (1 << 26)) return set_error(SANTA_ERR_INVALID, "too many sequences");
 
   struct Parts {
     int base = 0, rows = 0, local = 0, splits = 0;
   };
   std::vector<Parts> common_parts(static_cast<size_t>(tokens)), own_parts(static_cast<size_t>(tokens));
-  struct Piece {
-    int block, begin, end, base;
-    bool direct;
-  };
-  std::vector<Piece> pieces;
+  std::vector<int> base(pieces.size());
+  std::vector<char> direct(pieces.size());
   long long records = 0, most_rows = 0;
-  for (size_t i = 0; i < blocks.size(); ++i) {
-    const Block& k = blocks[i];
-    const int tiles = k.tiles(), splits = std::max(1, div_up(tiles, chunk));
+  for (size_t i = 0; i < pieces.size();) {
+    const Block& k = blocks[pieces[i].block];
+    size_t end = i;
+    while (end < pieces.size() && pieces[end].block == pieces[i].block) ++end;
     const int rows = k.ntok * GH;
     const bool from_list = (k.flags & kFromList) != 0;
-    const bool direct = splits == 1 && !from_list && k.begin == 0;
+    const bool whole = end - i == 1 && !from_list && k.begin == 0;
     most_rows = std::max<long long>(most_rows, rows);
-    for (int j = 0; j < k.ntok && !direct; ++j) {
-      Parts& p = from_list ? common_parts[list[k.tok0 + j]] : own_parts[k.tok0 + j];
-      p.base = static_cast<int>(records);
-      p.rows = rows;
-      p.local = j * GH;
-      p.splits = splits;
-    }
-    for (int s = 0; s < splits; ++s) {
-      const int t0 = static_cast<int>(static_cast<long long>(tiles) * s / splits);
-      const int t1 = static_cast<int>(static_cast<long long>(tiles) * (s + 1) / splits);
-      pieces.push_back({static_cast<int>(i), k.begin + kTile * t0, std::min(k.end, k.begin + kTile * t1),
-                        static_cast<int>(records), direct});
-      if (!direct) records += static_cast<long long>(rows) * in.kv_heads;
+    for (int j = 0; j < k.ntok && !whole; ++j)
+      (from_list ? common_parts[list[k.tok0 + j]] : own_parts[k.tok0 + j]) = {static_cast<int>(records), rows, j * GH,
+                                                                              static_cast<int>(end - i)};
+    for (; i < end; ++i) {
+      base[i] = static_cast<int>(records);
+      direct[i] = whole;
+      if (!whole) records += static_cast<long long>(rows) * in.kv_heads;
       if (records > INT_MAX) return set_error(SANTA_ERR_INVALID, "too many new tokens");
     }
   }
-  // the longest first
-  std::stable_sort(pieces.begin(), pieces.end(),
-                   [](const Piece& a, const Piece& b) { return a.end - a.begin > b.end - b.begin; });
 
+  info->groups = static_cast<int>(in.fixed ? slots : used);
   info->items = static_cast<int>(in.fixed ? max_items : static_cast<long long>(pieces.size()));
   info->records = in.fixed ? max_items * most_rows * in.kv_heads : records;
   if (info->records > INT_MAX) return set_error(SANTA_ERR_INVALID, "too many new tokens");
@@ -189,19 +202,27 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
   if (plan_ints < info->ints) return set_error(SANTA_ERR_INVALID, "the plan does not fit its buffer");
 
   std::memset(plan, 0, static_cast<size_t>(info->ints) * sizeof(int));
+  for (int i = 0; i < info->items; ++i) plan[static_cast<size_t>(i) * kItemInts + offsetof(Item, next) / sizeof(int)] = -1;
+  // a slot's first piece at the slot's number, the others behind them
+  int more = static_cast<int>(used), last = -1;
   for (size_t i = 0; i < pieces.size(); ++i) {
     const Piece& p = pieces[i];
     const Block& k = blocks[p.block];
     Item it{};
-    it.flags = k.flags | (p.direct ? kDirect : 0);
+    it.flags = k.flags | (direct[i] ? kDirect : 0);
     it.row = k.row;
-    it.begin = p.begin;
-    it.end = p.end;
+    it.begin = k.begin + kTile * p.t0;
+    it.end = std::min(k.end, k.begin + kTile * p.t1);
     it.tok0 = k.tok0;
     it.rows = k.ntok * GH;
     it.pos0 = k.pos0;
-    it.base = p.base;
-    std::memcpy(plan + i * kItemInts, &it, sizeof it);
+    it.base = base[i];
+    it.next = -1;
+    const bool first = i == 0 || pieces[i - 1].slot != p.slot;
+    const int at = first ? p.slot : more++;
+    if (!first) plan[static_cast<size_t>(last) * kItemInts + offsetof(Item, next) / sizeof(int)] = at;
+    std::memcpy(plan + static_cast<size_t>(at) * kItemInts, &it, sizeof it);
+    last = at;
   }
   int* pos = plan + info->pos_at;
   int* parts = plan + info->parts_at;
@@ -230,6 +251,7 @@ extern "C" int santa_paged_plan(const int* lens, const int* new_tokens, const in
     return set_error(SANTA_ERR_INVALID, "bad santa_paged_plan arguments");
   if (kv_heads <= 0 || heads <= 0 || heads % kv_heads != 0)
     return set_error(SANTA_ERR_INVALID, "H must be divisible by KVH. Got H=%d KVH=%d", heads, kv_heads);
+  if (heads > 1 << 16) return set_error(SANTA_ERR_UNSUPPORTED, "too many heads");
   if (heads / kv_heads > paged::kBlockRows)
     return set_error(SANTA_ERR_UNSUPPORTED, "the paged attention takes up to %d query heads per KV head. Got %d",
                      paged::kBlockRows, heads / kv_heads);

@@ -43,8 +43,8 @@ _IP = ctypes.POINTER(ctypes.c_int)
 
 
 class _PlanInfo(ctypes.Structure):
-    _fields_ = [(n, _I) for n in ("tokens", "items", "merge_tokens", "max_len", "max_row", "heads", "kv_heads")] + [
-        (n, _L) for n in ("records", "ints", "pos_at", "merge_at", "parts_at", "list_at")]
+    _fields_ = [(n, _I) for n in ("tokens", "groups", "items", "merge_tokens", "max_len", "max_row", "heads",
+                                  "kv_heads")] + [(n, _L) for n in ("records", "ints", "pos_at", "merge_at", "parts_at", "list_at")]
 
 
 _lib_ready = None
@@ -83,14 +83,14 @@ def _lib():
 _check = _FusedOps._check
 
 
-def _launch(device: torch.device, fn: str, *args):
-    """santa_<fn>(*args, stream) on device and its current stream."""
-    call = getattr(_lib(), "santa_" + fn)
-    if torch.cuda.current_device() == device.index:
-        _check(call(*args, torch.cuda.current_stream(device).cuda_stream))
+def _launch(device: torch.device, call, *args):
+    """call(*args, stream) on device and its current stream (the raw handle: an
+    object of it costs as much as a launch)."""
+    if torch._C._cuda_getDevice() == device.index:
+        _check(call(*args, torch._C._cuda_getCurrentRawStream(device.index)))
         return
     with torch.cuda.device(device):
-        _check(call(*args, torch.cuda.current_stream(device).cuda_stream))
+        _check(call(*args, torch._C._cuda_getCurrentRawStream(device.index)))
 
 
 def _device(device) -> torch.device:
@@ -268,7 +268,7 @@ class PagedKVCache:
         """What the last call asks of the pools and the block table."""
         table = self.block_table
         if self.device.type == "cuda":
-            _launch(self.device, "pages_apply", self._pages, self._pools, len(self._pools), self._page_bytes,
+            _launch(self.device, _lib().santa_pages_apply, self._pages, self._pools, len(self._pools), self._page_bytes,
                     self._page_bytes, table.data_ptr(), table.shape[1], self.max_seqs)
             return
         copies, edits = _IP(), _IP()
@@ -316,7 +316,7 @@ def copy_pages(pools: Union[torch.Tensor, Iterable[torch.Tensor]], src: Sequence
         for (size, stride), ts in groups.items():
             if size == 0 and all(0 <= p < num_pages for p in pairs):
                 continue
-            _launch(device, "paged_copy", (_P * len(ts))(*[t.data_ptr() for t in ts]), len(ts), size, stride, num_pages,
+            _launch(device, _lib().santa_paged_copy, (_P * len(ts))(*[t.data_ptr() for t in ts]), len(ts), size, stride, num_pages,
                     pairs, len(src))
         return
     for p in (*src, *dst):
@@ -419,44 +419,49 @@ class PagedPlan:
 
 
 def _check_pools(k_pages, v_pages, block_table, plan: PagedPlan, like: torch.Tensor) -> None:
-    if k_pages.dim() != 4 or k_pages.shape != v_pages.shape:
+    shape, device = k_pages.shape, like.device
+    if len(shape) != 4 or shape != v_pages.shape:
         raise ValueError("k_pages and v_pages must be [num_pages, page_size, KVH, D] tensors of one shape")
     if k_pages.dtype != like.dtype or v_pages.dtype != like.dtype:
         raise ValueError("k_pages and v_pages must have the dtype of the new tokens")
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or (block_table.shape[1] > 1
                                                                       and block_table.stride(1) != 1):
         raise ValueError("block_table must be an int32 [sequences, pages] tensor with contiguous rows")
-    for t in (k_pages, v_pages, block_table):
-        if t.device != like.device:
-            raise ValueError("device mismatch")
-    if plan.device != like.device:
-        raise ValueError(f"the plan is for {plan.device}, the tensors are on {like.device}")
-    page_size = k_pages.shape[1]
+    if k_pages.device != device or v_pages.device != device or block_table.device != device:
+        raise ValueError("device mismatch")
+    if plan.device != device:
+        raise ValueError(f"the plan is for {plan.device}, the tensors are on {device}")
+    num_pages, page_size, kv_heads, _ = shape
     if page_size < 8 or page_size & (page_size - 1) or page_size > 1 << 20:
         raise ValueError(f"page_size must be a power of two in [8, 1048576]. Got page_size={page_size}")
-    if k_pages.shape[0] == 0:
+    if num_pages == 0:
         raise ValueError("num_pages must be > 0")
-    if k_pages.shape[2] != plan.kv_heads:
-        raise ValueError(f"the plan is for {plan.kv_heads} KV heads, the pages hold {k_pages.shape[2]}")
-    info = plan._info
-    if info.max_row >= block_table.shape[0]:
-        raise ValueError(f"the plan names block table row {info.max_row} of {block_table.shape[0]}")
-    if info.max_len > block_table.shape[1] * page_size:
-        raise ValueError(f"seq_lens exceeds the block table's capacity: {info.max_len} > "
-                         f"{block_table.shape[1] * page_size}")
+    if kv_heads != plan.kv_heads:
+        raise ValueError(f"the plan is for {plan.kv_heads} KV heads, the pages hold {kv_heads}")
+    info, (rows, width) = plan._info, block_table.shape
+    if info.max_row >= rows:
+        raise ValueError(f"the plan names block table row {info.max_row} of {rows}")
+    if info.max_len > width * page_size:
+        raise ValueError(f"seq_lens exceeds the block table's capacity: {info.max_len} > {width * page_size}")
 
 
-def _strides(t: torch.Tensor, what: str) -> Tuple[int, ...]:
+def _strides(t: torch.Tensor, what: str) -> Sequence[int]:
     """The leading strides of [.., D]; those of dimensions of size 1, which are
     never used and can be any number, as if packed."""
-    out, packed = [], 1
-    for size, stride in zip(reversed(t.shape), reversed(t.stride())):
-        out.append(packed if size == 1 else stride)
-        packed *= size
-    if out[0] != 1 or any(s % 8 or s < 0 for s in out[1:]) or t.data_ptr() % 16:
+    strides = t.stride()
+    if 1 in t.shape:
+        strides, packed = list(strides), 1
+        for i in range(t.dim() - 1, -1, -1):
+            if t.shape[i] == 1:
+                strides[i] = packed
+            packed *= t.shape[i]
+    bad = strides[-1] != 1 or t.data_ptr() % 16
+    for s in strides[:-1]:
+        bad = bad or s % 8 or s < 0
+    if bad:
         raise ValueError(f"{what} must be 16-byte aligned, its last dimension contiguous and its other strides "
                          "multiples of 8 elements")
-    return tuple(reversed(out[1:]))
+    return strides[:-1]
 
 
 def _table_rows(table: torch.Tensor) -> Tuple[torch.Tensor, int]:
@@ -511,7 +516,7 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages
         q = torch.empty(plan.tokens, H, D, dtype=qkv.dtype, device=qkv.device)
         table, row = _table_rows(block_table)
         if plan.tokens:
-            _launch(qkv.device, "paged_rope_append", qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), q.data_ptr(),
+            _launch(qkv.device, _lib().santa_paged_rope_append, qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), q.data_ptr(),
                     k_pages.data_ptr(), v_pages.data_ptr(), int(qkv.dtype == torch.float16), D, k_pages.shape[0],
                     k_pages.shape[1], (_L * 6)(*strides), table.data_ptr(), row, table.shape[0],
                     ctypes.byref(plan._info), plan._data.data_ptr())
@@ -560,7 +565,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     block_table int32 [sequences, pages] -> [tokens, H, D].  A token attends to
     the tokens of its sequence up to itself; one at a negative position gives
     zeros.  plan: a PagedPlan, or the lengths of the sequences, each with one
-    new token.  scale: of the scores, 1 / sqrt(D) by default.
+    new token.  scale: of the scores, positive, 1 / sqrt(D) by default.
 
     bf16 and f16 of head_dim 64 and 128 on a GPU run as one kernel over all
     sequences (and one that joins parts, where the tokens of a sequence are
@@ -579,10 +584,12 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if k_pages.shape[3] != D:
         raise ValueError(f"D mismatch: q {D}, pages {k_pages.shape[3]}")
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not 1e-37 < scale < 1e37:  # normal in float32, times log2(e) too
+        raise ValueError(f"scale must be positive and finite; got {scale}")
     if not (q.is_cuda and q.dtype in (torch.bfloat16, torch.float16) and D in (64, 128)
             and _plain(q, k_pages, v_pages)):
         return _attention_expressions(q, k_pages, v_pages, block_table, plan, scale)
-    out = torch.empty(N, H, D, dtype=q.dtype, device=q.device)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if N == 0:
         return out
     try:
@@ -594,7 +601,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     table, row = _table_rows(block_table)
     info = ctypes.byref(plan._info)
     workspace = torch.empty(_lib().santa_paged_workspace_size(info, D), dtype=torch.uint8, device=q.device)
-    _launch(q.device, "paged_attention", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(),
+    _launch(q.device, _lib().santa_paged_attention, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(),
             int(q.dtype == torch.float16), D, k_pages.shape[0], k_pages.shape[1], strides, table.data_ptr(), row,
             table.shape[0], info, plan._data.data_ptr(), scale, workspace.data_ptr(), workspace.numel())
     return out

@@ -273,11 +273,17 @@ def _carry_out(q, k, v, table, plan):
     out = torch.full((N, H, D), math.nan, dtype=torch.float64)
     part = {}
     written = set()
-    for i in range(info.items):
-        flags, row, begin, end, tok0, rows, pos0, base = data[16 * i:16 * i + 8].tolist()
+    items, seen = [], set()
+    for w in range(info.groups):
+        while w >= 0:
+            assert w < info.items and w not in seen
+            seen.add(w)
+            items.append(data[16 * w:16 * w + 9].tolist())
+            w = items[-1][8]
+    for flags, row, begin, end, tok0, rows, pos0, base, _ in items:
         if rows == 0:
             continue
-        assert begin % 64 == 0 and begin <= end and 0 < rows <= 128 and rows % GH == 0
+        assert begin % 64 == 0 and begin <= end and 0 < rows <= 256 and rows % GH == 0
         at = torch.arange(begin, end)
         kk, vv = (x[table[row, at // page].long(), at % page] for x in (k, v))
         for kv in range(KVH):
@@ -331,6 +337,7 @@ PLANS = [
     ([5000], [1], [], 2, 2, 64),
     ([700, 3], [300, 2], [], 8, 2, 16),
     ([260], [2], [], 128, 1, 64),
+    ([100], [3], [], 256, 1, 8),
 ]
 
 
@@ -358,7 +365,7 @@ def test_plan_update():
     for fixed in (False, True):
         plan = PagedPlan(lens, heads=4, kv_heads=2, new_tokens=new, prefixes=shared, device="cpu", fixed=fixed)
         held = plan._data
-        size = lambda i: (i.tokens, i.items, i.merge_tokens, i.records, i.ints)  # noqa: E731
+        size = lambda i: (i.tokens, i.groups, i.items, i.merge_tokens, i.records, i.ints)  # noqa: E731
         first = size(plan._info)
         for other in ([129, 2, 140], [4000, 9000, 129], [200, 300, 180]):
             plan.update(other)
@@ -381,7 +388,7 @@ def test_plan_refusals():
                            ([4], {"kv_heads": 0}, "divisible"), ([4], {"rows": [-2]}, "row -2"),
                            ([9, 9], {"prefixes": [([0, 1], 9)]}, "are not common"),
                            ([9, 9], {"prefixes": [([0, 1], -1)]}, "are not common"),
-                           ([4], {"heads": 129, "kv_heads": 1}, "up to 128 query heads"),
+                           ([4], {"heads": 257, "kv_heads": 1}, "up to 256 query heads"),
                            ([4], {"new_tokens": [1 << 30]}, "too many new tokens")]:
         with pytest.raises(RuntimeError, match=text):
             PagedPlan(lens, **{**ok, **kw})
@@ -489,6 +496,9 @@ def test_call_refusals():
         lambda: paged_attention(q, k, v, table.t().contiguous().t(), plan),
         lambda: paged_attention(q, k, v, table, short), lambda: paged_attention(q, k, v, table, far),
         lambda: paged_attention(q, k[:0], v[:0], table, plan),
+        lambda: paged_attention(q, k, v, table, plan, scale=0.0), lambda: paged_attention(q, k, v, table, plan, scale=-1.0),
+        lambda: paged_attention(q, k, v, table, plan, scale=float("inf")),
+        lambda: paged_attention(q, k, v, table, plan, scale=float("nan")),
         lambda: rope_append(qkv[:1], cs, cs, k, v, table, plan), lambda: rope_append(qkv, cs[:1], cs, k, v, table, plan),
         lambda: rope_append(qkv, cs.float(), cs, k, v, table, plan), lambda: rope_append(qkv, cs, cs, k, v, table, short),
         lambda: rope_append(qkv.float(), cs.float(), cs.float(), k, v, table, plan),
@@ -505,14 +515,16 @@ def test_library_refusals():
     info, one = ctypes.byref(plan._info), ctypes.c_void_p(16)
     strides = (ctypes.c_longlong * 8)(512, 128, 2048, 256, 128, 2048, 256, 128)
 
-    def attend(q=one, dtype=0, D=128, pages=4, page=8, st=strides, width=4, rows=2, ws=one, size=1 << 30):
-        return lib.santa_paged_attention(q, one, one, one, dtype, D, pages, page, st, one, width, rows, info, one, 1.0, ws,
-                                         size, None)
+    def attend(q=one, dtype=0, D=128, pages=4, page=8, st=strides, width=4, rows=2, ws=one, size=1 << 30, scale=1.0):
+        return lib.santa_paged_attention(q, one, one, one, dtype, D, pages, page, st, one, width, rows, info, one, scale,
+                                         ws, size, None)
 
     odd = (ctypes.c_longlong * 8)(512, 128, 2048, 256, 4, 2048, 256, 128)
     for kw, text in [({"q": None}, "bad paged_attention"), ({"dtype": 3}, "bad paged_attention"), ({"D": 96}, "64 or 128"),
                      ({"pages": 0}, "num_pages"), ({"page": 12}, "power of two"), ({"st": odd}, "multiples of 8"),
-                     ({"width": 2}, "too narrow"), ({"rows": 1}, "row 1 of 1"), ({"q": ctypes.c_void_p(8)}, "16-byte")]:
+                     ({"width": 2}, "too narrow"), ({"rows": 1}, "row 1 of 1"),
+                     ({"scale": 0.0}, "positive"), ({"scale": -1.0}, "positive"), ({"scale": 3e38}, "positive"),
+                     ({"scale": float("nan")}, "positive"), ({"q": ctypes.c_void_p(8)}, "16-byte")]:
         assert attend(**kw) != 0 and text in error(), (kw, error())
     if plan._info.records:
         assert attend(size=8) == 3 and attend(ws=None) == 1
@@ -527,7 +539,8 @@ def test_library_refusals():
     assert lib.santa_pages_length(None, 0) == -1 and lib.santa_pages_used(None) == -1
     small = (ctypes.c_int * 4)()
     out = paged._PlanInfo()
-    assert lib.santa_paged_plan(small, small, None, 2, None, None, 0, 4, 2, 0, ctypes.byref(out), small, 1) != 0 or out.ints <= 1
+    made = lib.santa_paged_plan(small, small, None, 2, None, None, 0, 4, 2, 0, ctypes.byref(out), small, 1)
+    assert made != 0 or out.ints <= 1
 
 
 # -------------------------------------------------------------------- model
