@@ -374,14 +374,14 @@ struct State {
 // K are all asked for before the first product, the rest one by one beside the
 // products: left to itself the compiler reads, waits and multiplies in turn.
 template <bool BF16, int D, int KB>
-__device__ __forceinline__ void scores(const char* buf, const u32x4 (&qf)[D / 16], const uint32_t (&ko)[D / 16],
-                                       f32x16 (&s)[KB]) {
+__device__ __forceinline__ void scores(const char* buf, const u32x4 (&qf)[D / 16], uint32_t ko, f32x16 (&s)[KB]) {
+  asm volatile("" : "+v"(ko));  // its parts are formed here and not kept over the loop
   u32x4 k[KB][D / 16];
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
     for (int c = 0; c < D / 16; ++c)
-      k[kb][c] = *reinterpret_cast<const u32x4*>(buf + ko[c] + 32 * Geometry<D>::kRow * kb);
+      k[kb][c] = *reinterpret_cast<const u32x4*>(buf + (ko ^ (32 * c)) + 32 * Geometry<D>::kRow * kb);
 #pragma unroll
   for (int kb = 0; kb < KB; ++kb) {
 #pragma unroll
@@ -398,19 +398,19 @@ __device__ __forceinline__ void scores(const char* buf, const u32x4 (&qf)[D / 16
   __builtin_amdgcn_sched_group_barrier(0x008, D / 16, 0);
 }
 
-// Their softmax: P^T in the 16-bit type, the running state moved on.  n0: the
-// first token; lim: the last one that the lane's row attends to, lim_lo the least
-// of the wave's rows.  dup: up to 16 rows.
-template <bool BF16, int KB, int MB>
-__device__ __forceinline__ void softmax(f32x16 (&s)[KB], u32x4 (&p)[2 * KB], int n0, int lim, int lim_lo, bool dup,
-                                        float scale_log2, State<MB>& st) {
-  const int lane = threadIdx.x & 63, half = lane >> 5;
-  if (n0 + 32 * KB - 1 > lim_lo) {  // tokens that some row does not attend to
+// Their softmax: P^T in the 16-bit type, the running state moved on.  kMasked:
+// the lane's row attends to the first lim + 1 of the tokens.  dup: up to 16 rows.
+template <bool BF16, int KB, int MB, bool kMasked>
+__device__ __forceinline__ void softmax(f32x16 (&s)[KB], u32x4 (&p)[2 * KB], int lim, bool dup, float scale_log2,
+                                        State<MB>& st) {
+  const int lane = threadIdx.x & 63;
+  if constexpr (kMasked) {
+    const int left = lim - 4 * (lane >> 5);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        if (n0 + 32 * kb + 8 * (e >> 2) + 4 * half + (e & 3) > lim) s[kb][e] = -__builtin_inff();
+        if (32 * kb + 8 * (e >> 2) + (e & 3) > left) s[kb][e] = -__builtin_inff();
   }
   float mx = s[0][0];
 #pragma unroll
@@ -466,15 +466,15 @@ __device__ __forceinline__ void softmax(f32x16 (&s)[KB], u32x4 (&p)[2 * KB], int
 // O^T += V^T P^T over MB x 32 dims; the reads of V run ahead of the products as
 // those of K do.
 template <bool BF16, int D, int KB, int MB>
-__device__ __forceinline__ void sums(const char* buf, const uint32_t (&vo)[MB], const u32x4 (&p)[2 * KB],
-                                     State<MB>& st) {
+__device__ __forceinline__ void sums(const char* buf, uint32_t vo, const u32x4 (&p)[2 * KB], State<MB>& st) {
+  asm volatile("" : "+v"(vo));
   using G = Geometry<D>;
   constexpr int N = 2 * KB * MB, kAhead = N < 4 ? N : 4;
   u32x4 v[2 * KB][MB];
 #pragma unroll
   for (int kc = 0; kc < 2 * KB; ++kc)
 #pragma unroll
-    for (int mb = 0; mb < MB; ++mb) v[kc][mb] = read_tr8<G::kRow>(buf + vo[mb] + 16 * G::kRow * kc);
+    for (int mb = 0; mb < MB; ++mb) v[kc][mb] = read_tr8<G::kRow>(buf + (vo ^ (64 * mb)) + 16 * G::kRow * kc);
 #pragma unroll
   for (int kc = 0; kc < 2 * KB; ++kc)
 #pragma unroll
@@ -488,6 +488,57 @@ __device__ __forceinline__ void sums(const char* buf, const uint32_t (&vo)[MB], 
   __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
 }
 
+// Whether 32 KB rows of a V tile hold an infinity or a NaN.
+template <bool BF16, int D, int KB>
+__device__ __forceinline__ bool not_finite(const char* rows) {
+  constexpr uint32_t kStep = BF16 ? 0x00800080 : 0x04000400;  // carries an exponent of all ones into the sign's bit
+  uint32_t bad = 0;
+#pragma unroll 4
+  for (int i = 0; i < 32 * KB * Geometry<D>::kRow / 1024; ++i) {
+    const u32x4 v = *reinterpret_cast<const u32x4*>(rows + 1024 * i + 16 * (threadIdx.x & 63));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) bad |= (v[j] & 0x7fff7fff) + kStep;
+  }
+  return __any((bad & 0x80008000) != 0);
+}
+
+// sums() for a tile of which some rows do not attend to all tokens.  Where a
+// value there is not finite (apart), and would not vanish with a probability of
+// 0: for one last token after the other, the values behind it left out, and the
+// result kept by the rows that end there.
+template <bool BF16, int D, int KB, int MB>
+__device__ __forceinline__ void sums_masked(const char* buf, uint32_t vo, const u32x4 (&p)[2 * KB], int n0,
+                                            int last, int lim, int lim_lo, int lim_hi, bool apart, State<MB>& st) {
+  using G = Geometry<D>;
+  const int most = apart ? min(lim_hi, last) : last;
+  for (int end = apart ? max(lim_lo, n0) : last; end <= most; ++end) {
+    const int left = end - n0 - 4 * (static_cast<int>(threadIdx.x & 63) >> 5);
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      u32x4 v[2 * KB];
+#pragma unroll
+      for (int kc = 0; kc < 2 * KB; ++kc) v[kc] = read_tr8<G::kRow>(buf + (vo ^ (64 * mb)) + 16 * G::kRow * kc);
+      if (!apart) {
+#pragma unroll
+        for (int kc = 0; kc < 2 * KB; ++kc) st.o[mb] = mfma32<BF16>(v[kc], p[kc], st.o[mb]);
+      } else {
+        f32x16 o = st.o[mb];
+#pragma unroll
+        for (int kc = 0; kc < 2 * KB; ++kc) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const int n = 16 * kc + 8 * (j >> 1) + 2 * (j & 1);  // of the dword's first value
+            v[kc][j] = n < left ? v[kc][j] : n == left ? v[kc][j] & 0xffff : 0;
+          }
+          o = mfma32<BF16>(v[kc], p[kc], o);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) st.o[mb][e] = min(lim, last) == end ? o[e] : st.o[mb][e];
+      }
+    }
+  }
+}
+
 // The workgroup's barrier alone: no wave waits for its loads here.
 __device__ __forceinline__ void barrier() {
   asm volatile("" ::: "memory");
@@ -498,7 +549,8 @@ __device__ __forceinline__ void barrier() {
 // LDS beside the stages, for what the waves of the same rows and dims hold of
 // different tokens.
 struct Shares {
-  float o[6][16][64], m[6][64], l[6][64];
+  float4 o[6][4][64];
+  float m[6][64], l[6][64];
 };
 
 // One item.  Its rows are RG groups of 32, each held by 8 / RG waves.  RG 8: one
@@ -517,7 +569,11 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv
   constexpr int DH = RG >= 4 ? 1 : 2, MB = D / 32 / DH;     // parts of the dims, 32s of them in each
   constexpr int TG = RG == 8 ? 1 : RG == 1 ? 4 : 2;         // parts of the tokens
   constexpr int kStep = RG == 1 ? 2 : 1;                    // tiles at once
-  const int lane = threadIdx.x & 63, half = lane >> 5, ql = lane & 31;
+  // opaque, so that what depends on it is formed here: the offsets of all four
+  // forms, kept over all items, would not fit the registers
+  int lane = threadIdx.x & 63;
+  asm volatile("" : "+v"(lane));
+  const int half = lane >> 5, ql = lane & 31;
   const int wave = w.wave;
   const int dh = DH == 1 ? 0 : wave & 1, tg = wave / DH % TG, rg = wave / (DH * TG);
   const int kh = TG == 1 ? 0 : tg & 1;                      // half of a tile
@@ -540,18 +596,12 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv
 #pragma unroll
     for (int c = 0; c < D / 16; ++c) qf[c] = *reinterpret_cast<const u32x4*>(qr + 16 * c);
   }
-  // LDS byte offsets of this lane's fragments inside a stage
-  uint32_t ko[D / 16], vo[MB];
-#pragma unroll
-  for (int c = 0; c < D / 16; ++c)
-    ko[c] = (ql + 32 * kh) * G::kRow + 16 * ((2 * c + half) ^ (D == 128 ? ql & 15 : (ql >> 1) & 7));
-  const int r3 = (lane & 15) >> 2;
-#pragma unroll
-  for (int mb = 0; mb < MB; ++mb) {
-    const int piece = 4 * (mb + MB * dh) + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
-    vo[mb] = 16 * G::kVecs + (4 * half + r3 + 32 * kh) * G::kRow +
-             16 * (piece ^ (D == 128 ? 4 * r3 : 4 * (r3 >> 1))) + 8 * (lane & 1);
-  }
+  // LDS byte offsets inside a stage of this lane's first fragments; those of
+  // further dims lie at these numbers with some bits flipped (the swizzle)
+  const uint32_t ko = (ql + 32 * kh) * G::kRow + 16 * (half ^ (D == 128 ? ql & 15 : (ql >> 1) & 7));
+  const int r3 = (lane & 15) >> 2, piece = 4 * MB * dh + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+  const uint32_t vo = 16 * G::kVecs + (4 * half + r3 + 32 * kh) * G::kRow +
+                      16 * (piece ^ (D == 128 ? 4 * r3 : 4 * (r3 >> 1))) + 8 * (lane & 1);
 
   State<MB> st;
 #pragma unroll
@@ -565,11 +615,15 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv
   // Q has landed: known here, it is not waited for in every tile
   __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0) alone
   const int nt = tiles_of(it.begin, it.end);
-  // tiles in which a row of this wave attends to a token
+  const int mine = kStep == 1 ? 0 : tg >> 1, first = it.begin + 32 * kh;  // tile of the step, token of the tile 0
+  // tiles in which a row of this wave attends to a token; and those of them in
+  // which all rows attend to all
   const int busy = any && lim_hi >= it.begin ? min(nt, (lim_hi - it.begin) / kTile + 1) : 0;
-  for (int t = 0; t < nt; t += kStep) {
-    // this wave's loads of the step's tiles have landed (those of newer ones need
-    // not have), then all waves' have, and no wave reads the tiles before any more
+  const int whole = min(busy, (max(lim_lo + 1 - first - 32 * KB, -kTile) + kTile) / kTile);
+  // To the step of tile t: this wave's loads of its tiles have landed (those of
+  // newer ones need not have), then all waves' have, and no wave reads the tiles
+  // before any more, whose places are loaded anew.
+  auto enter = [&](int t) {
     const int newer = static_cast<int>(loaded - tile) - min(kStep, nt - t);
     constexpr int kMost = G::kStages - 1 - kStep, kSome = kMost / 2;
     if (newer >= kMost) wait_loads<2 * G::kLoads * kMost>();
@@ -578,16 +632,29 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv
     barrier();
     while (cur.more && loaded - tile < G::kStages)
       load_tile<D>(w, cur, loaded++ % G::kStages, lk, lv);
-    const int mine = kStep == 1 ? 0 : tg >> 1;
-    if (t + mine < busy) {
-      const char* stage = reinterpret_cast<const char*>(stages + ((tile + mine) % G::kStages) * G::kStage);
-      f32x16 s[KB];
-      u32x4 p[2 * KB];
-      scores<BF16, D, KB>(stage, qf, ko, s);
-      softmax<BF16, KB, MB>(s, p, it.begin + (t + mine) * kTile + 32 * kh, lim, lim_lo, dup, a.scale_log2, st);
-      sums<BF16, D, KB, MB>(stage, vo, p, st);
-    }
+    const uint32_t at = tile + mine;
     tile += min(kStep, nt - t);
+    return reinterpret_cast<const char*>(stages + (at % G::kStages) * G::kStage);
+  };
+  int t = 0;
+  for (; t + mine < whole; t += kStep) {
+    const char* stage = enter(t);
+    f32x16 s[KB];
+    u32x4 p[2 * KB];
+    scores<BF16, D, KB>(stage, qf, ko, s);
+    softmax<BF16, KB, MB, false>(s, p, 0, dup, a.scale_log2, st);
+    sums<BF16, D, KB, MB>(stage, vo, p, st);
+  }
+  for (; t < nt; t += kStep) {  // a loop of its own, or both would run short of registers
+    const char* stage = enter(t);
+    if (t + mine >= busy) continue;
+    f32x16 s[KB];
+    u32x4 p[2 * KB];
+    const int n0 = first + (t + mine) * kTile, last = min(it.end, n0 + 32 * KB) - 1;
+    scores<BF16, D, KB>(stage, qf, ko, s);
+    softmax<BF16, KB, MB, true>(s, p, lim - n0, dup, a.scale_log2, st);
+    const bool apart = last > lim_lo && not_finite<BF16, D, KB>(stage + 16 * G::kVecs + 32 * kh * G::kRow);
+    sums_masked<BF16, D, KB, MB>(stage, vo, p, n0, last, lim, lim_lo, lim_hi, apart, st);
   }
   float m = st.m, l = st.l + other_half(st.l);
   f32x16(&o)[MB] = st.o;
@@ -612,7 +679,8 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv
     for (int mb = 0; mb < MB; ++mb) {
       if (tg > 0) {
 #pragma unroll
-        for (int e = 0; e < 16; ++e) x->o[first + tg - 1][e][lane] = o[mb][e];
+        for (int e = 0; e < 16; e += 4)
+          x->o[first + tg - 1][e / 4][lane] = make_float4(o[mb][e], o[mb][e + 1], o[mb][e + 2], o[mb][e + 3]);
       }
       __syncthreads();
       if (tg == 0) {
@@ -630,11 +698,17 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv
           }
         }
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-          o[mb][e] *= own;
+        for (int e = 0; e < 16; ++e) o[mb][e] *= own;
 #pragma unroll
-          for (int i = 0; i < TG - 1; ++i) o[mb][e] = fmaf(x->o[first + i][e][lane], weight[i], o[mb][e]);
-        }
+        for (int i = 0; i < TG - 1; ++i)
+#pragma unroll
+          for (int e = 0; e < 16; e += 4) {
+            const float4 v = x->o[first + i][e / 4][lane];
+            o[mb][e] = fmaf(v.x, weight[i], o[mb][e]);
+            o[mb][e + 1] = fmaf(v.y, weight[i], o[mb][e + 1]);
+            o[mb][e + 2] = fmaf(v.z, weight[i], o[mb][e + 2]);
+            o[mb][e + 3] = fmaf(v.w, weight[i], o[mb][e + 3]);
+          }
       }
       __syncthreads();
     }
@@ -723,83 +797,75 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_attention_kernel(AttnArg
   }
 }
 
-// Joins the parts of one (token, head): W waves, each every W-th part, a lane two
-// dims (D 64: the two halves of a wave take parts in turn).
-template <bool BF16, int D, int W>
+// Joins the parts of a (token, head): D / 4 lanes, a team, hold four dims each of
+// every part that they take.  kOne: the teams of a workgroup take the parts of one
+// row in turn; otherwise each has a row of its own.
+template <bool BF16, int D, bool kOne>
 __global__ __launch_bounds__(256) void merge_kernel(const float* __restrict__ part, const float2* __restrict__ part_ml,
                                                     const int* __restrict__ tokens, const int4* __restrict__ parts,
                                                     const int2* __restrict__ pos, int first_row, int rows, int H,
                                                     int KVH, float scale_log2, uint16_t* __restrict__ out) {
-  constexpr int kTeam = D / 2, kTeams = 64 / kTeam;  // lanes per part, parts per wave at once
-  __shared__ float s_m[4], s_z[4];
-  __shared__ float2 s_o[4][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int row = W == 1 ? 4 * blockIdx.x + wave : blockIdx.x;
-  int tok = -1, n = 0, h = 0;
-  int4 pa{}, pb{};  // base, rows, local, splits
-  if (row < rows) {
-    tok = tokens[(first_row + row) / H];
-    h = (first_row + row) % H;
-    if (tok >= 0) {
-      pa = parts[2 * tok], pb = parts[2 * tok + 1];
-      n = pb.w > 0 ? pa.w + pb.w : 0;  // 0: written by its item
-    }
-  }
-  const int kv = h / (H / KVH), g = h % (H / KVH);
+  constexpr int kTeam = D / 4, kTeams = 256 / kTeam, kStep = kOne ? kTeams : 1, kBatch = 4;
+  __shared__ float s_m[kTeams], s_z[kTeams];
+  __shared__ float4 s_o[kTeams][kTeam];
+  const int team = threadIdx.x / kTeam, d4 = threadIdx.x % kTeam;
+  const int row = kOne ? static_cast<int>(blockIdx.x) : static_cast<int>(blockIdx.x) * kTeams + team;
+  if (row >= rows) return;  // of all the workgroup or, without a barrier below, of some teams
+  const int tok = tokens[(first_row + row) / H], h = (first_row + row) % H;
+  if (tok < 0) return;
+  const int4 pa = parts[2 * tok], pb = parts[2 * tok + 1];  // base, rows, local, splits
+  if (pb.w <= 0) return;                                    // written by its item
+  const bool blind = pos[tok].x < 0;
+  const int n = pa.w + pb.w, kv = h / (H / KVH), g = h % (H / KVH);
   auto record = [&](int j) {
     const bool first = j < pa.w;
     return static_cast<size_t>(first ? pa.x : pb.x) +
            (static_cast<size_t>(first ? j : j - pa.w) * KVH + kv) * (first ? pa.y : pb.y) + (first ? pa.z : pb.z) + g;
   };
-  const int w = W == 1 ? 0 : wave, team = lane / kTeam, d2 = lane % kTeam;
-  float mx = kLowest;
-  for (int j = lane * W + w; j < n; j += 64 * W) mx = fmaxf(mx, part_ml[record(j)].x);
-#pragma unroll
-  for (int d = 32; d > 0; d >>= 1) mx = fmaxf(mx, __shfl_xor(mx, d, 64));
-  if constexpr (W > 1) {
-    if (lane == 0) s_m[wave] = mx;
-    __syncthreads();
-    mx = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-  }
-  float z = 0.0f;
-  float2 acc = make_float2(0.0f, 0.0f);
-  constexpr int kBatch = 8;
-  for (int j0 = w + team * W; j0 < n; j0 += kBatch * kTeams * W) {
-    float2 ml[kBatch], v[kBatch];
+  float m = kLowest, z = 0.0f;
+  float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  auto add = [&](float mj, float zj, const float4& o) {
+    const float e = __builtin_amdgcn_exp2f((mj - m) * scale_log2);
+    z = fmaf(e, zj, z);
+    acc.x = fmaf(e, o.x, acc.x), acc.y = fmaf(e, o.y, acc.y);
+    acc.z = fmaf(e, o.z, acc.z), acc.w = fmaf(e, o.w, acc.w);
+  };
+  for (int j0 = kOne ? team : 0; j0 < n; j0 += kBatch * kStep) {
+    float2 ml[kBatch];
+    float4 v[kBatch];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      const int j = j0 + b * kTeams * W;
-      const size_t rec = record(min(j, n - 1));
+      const size_t rec = record(min(j0 + b * kStep, n - 1));
       ml[b] = part_ml[rec];
-      v[b] = *reinterpret_cast<const float2*>(part + rec * D + 2 * d2);
+      v[b] = *reinterpret_cast<const float4*>(part + rec * D + 4 * d4);
     }
+    float top = m;
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) top = fmaxf(top, ml[b].x);  // the last part stands for those past the end
+    const float w = __builtin_amdgcn_exp2f((m - top) * scale_log2);
+    z *= w, acc.x *= w, acc.y *= w, acc.z *= w, acc.w *= w;
+    m = top;
 #pragma unroll
     for (int b = 0; b < kBatch; ++b)
-      if (j0 + b * kTeams * W < n) {
-        const float e = __builtin_amdgcn_exp2f((ml[b].x - mx) * scale_log2);
-        z = fmaf(e, ml[b].y, z);
-        acc.x = fmaf(e, v[b].x, acc.x);
-        acc.y = fmaf(e, v[b].y, acc.y);
-      }
+      if (j0 + b * kStep < n) add(ml[b].x, ml[b].y, v[b]);
   }
-  if constexpr (kTeams == 2) {
-    z += other_half(z);
-    acc.x += other_half(acc.x);
-    acc.y += other_half(acc.y);
-  }
-  if constexpr (W > 1) {
-    if (lane == 0) s_z[wave] = z;
-    s_o[wave][lane] = acc;
+  if constexpr (kOne) {
+    if (d4 == 0) s_m[team] = m, s_z[team] = z;
+    s_o[team][d4] = acc;
     __syncthreads();
-    if (wave > 0) return;
-    z = (s_z[0] + s_z[1]) + (s_z[2] + s_z[3]);
+    if (team > 0) return;
 #pragma unroll
-    for (int k = 1; k < W; ++k) acc.x += s_o[k][lane].x, acc.y += s_o[k][lane].y;
+    for (int t = 1; t < kTeams; ++t) m = fmaxf(m, s_m[t]);
+    z = 0.0f;
+    acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+    for (int t = 0; t < kTeams; ++t) add(s_m[t], s_z[t], s_o[t][d4]);
   }
-  if (n == 0 || team > 0) return;
-  const float inv = pos[tok].x < 0 ? 0.0f : 1.0f / z;
-  const uint32_t v = f32_to_h16<BF16>(acc.x * inv) | (static_cast<uint32_t>(f32_to_h16<BF16>(acc.y * inv)) << 16);
-  *reinterpret_cast<uint32_t*>(out + (static_cast<size_t>(tok) * H + h) * D + 2 * d2) = v;
+  const float inv = blind ? 0.0f : 1.0f / z;
+  uint2 v;
+  v.x = f32_to_h16<BF16>(acc.x * inv) | (static_cast<uint32_t>(f32_to_h16<BF16>(acc.y * inv)) << 16);
+  v.y = f32_to_h16<BF16>(acc.z * inv) | (static_cast<uint32_t>(f32_to_h16<BF16>(acc.w * inv)) << 16);
+  *reinterpret_cast<uint2*>(out + (static_cast<size_t>(tok) * H + h) * D + 4 * d4) = v;
 }
 
 // A block table, pools and plan that belong together.
@@ -1000,8 +1066,9 @@ extern "C" int santa_paged_attention(const void* q, const void* k_pages, const v
                            reinterpret_cast<const int2*>(plan + info->pos_at), static_cast<int>(r), n, H, KVH,
                            a.scale_log2, a.out);
       };
-      if (wide) merge(merge_kernel<BF16, kD, 4>, n);
-      else merge(merge_kernel<BF16, kD, 1>, (n + 3) / 4);
+      constexpr int kTeams = 1024 / kD;
+      if (wide) merge(merge_kernel<BF16, kD, true>, n);
+      else merge(merge_kernel<BF16, kD, false>, (n + kTeams - 1) / kTeams);
     }
   };
   if (dtype == SANTA_BF16) {

@@ -532,6 +532,20 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages
 
 
 # ---------------------------------------------------------------- attention
+def _weighted(p, v, seen):
+    """p @ v [KVH, rows, D] over the tokens that a row attends to (seen [rows,
+    n]): an infinity or a NaN among a later token's values stays out, where its
+    product with a probability of 0 would be NaN."""
+    bad = ~torch.isfinite(v)
+    o = torch.bmm(p, v.masked_fill(bad, 0.0))
+    weighs, none = ((seen & (p.detach() > 0)).to(v.dtype), (seen & ~(p.detach() > 0)).to(v.dtype))
+    plus, minus = (torch.bmm(weighs, (v.detach() == x).to(v.dtype)) > 0 for x in (math.inf, -math.inf))
+    lost = torch.bmm(weighs, v.detach().isnan().to(v.dtype)) + torch.bmm(none, bad.to(v.dtype)) > 0
+    for where, value in ((plus, math.inf), (minus, -math.inf), (lost, math.nan)):
+        o = o + torch.where(where, value, 0.0).to(o.dtype)
+    return o
+
+
 def _attention_expressions(q, k_pages, v_pages, block_table, plan: PagedPlan, scale: float) -> torch.Tensor:
     """paged_attention sequence by sequence, float32 (float64 for float64)."""
     N, H, D = q.shape
@@ -551,7 +565,9 @@ def _attention_expressions(q, k_pages, v_pages, block_table, plan: PagedPlan, sc
             s = torch.bmm(x.reshape(KVH, -1, D).contiguous(), k) * scale                     # [KVH, tokens * GH, n]
             pos = torch.arange(n - t + blind, n, device=q.device).repeat_interleave(H // KVH)
             s = s.masked_fill(at[None, :] > pos[:, None], float("-inf"))
-            o = torch.bmm(torch.softmax(s, dim=-1), v).view(KVH, t - blind, H // KVH, D).permute(1, 0, 2, 3)
+            o = _weighted(torch.softmax(s, dim=-1), v, at[None, :] <= pos[:, None]) if t > 1 else \
+                torch.bmm(torch.softmax(s, dim=-1), v)
+            o = o.view(KVH, t - blind, H // KVH, D).permute(1, 0, 2, 3)
             out.append(o.reshape(t - blind, H, D).to(q.dtype))
         t0 += t
     return torch.cat(out) if out else torch.empty_like(q)

@@ -479,6 +479,31 @@ def test_rope_append_expressions(dtype):
     assert torch.equal(k.nan_to_num(9.0), k0.nan_to_num(9.0)) and torch.equal(v.nan_to_num(9.0), v0.nan_to_num(9.0))
 
 
+def test_later_values_stay_out():
+    """Infinities and NaN of tokens that a row does not attend to leave it as it
+    is; those that it attends to are in their own dims."""
+    g = torch.Generator().manual_seed(0)
+    lens, new = [20, 9, 2], [6, 9, 4]
+    k, v, table = _shared_pools(lens, [], 8, 2, 16, 1)
+    q = torch.randn(sum(new), 4, 16, generator=g, dtype=torch.float64)
+    plan = PagedPlan(lens, heads=4, kv_heads=2, new_tokens=new, device="cpu")
+    clean = paged_attention(q, k, v, table, plan)
+    at = {0: (17, 3, math.inf), 1: (4, 7, math.nan), 2: (1, 0, -math.inf)}
+    for b, (n, d, x) in at.items():
+        v[table[b, n // 8].long(), n % 8, 1, d] = x
+    out = paged_attention(q, k, v, table, plan)
+    t0 = 0
+    for b, (n, d, x) in at.items():
+        for i in range(new[b]):
+            sees = lens[b] - new[b] + i >= n
+            hit = torch.zeros(4, 16, dtype=torch.bool)
+            hit[2:, d] = sees
+            assert torch.equal(out[t0 + i][~hit], clean[t0 + i][~hit]), (b, i)
+            want = torch.full((2,), x, dtype=torch.float64)
+            assert not sees or torch.equal(out[t0 + i][hit].nan_to_num(9.0), want.nan_to_num(9.0)), (b, i)
+        t0 += new[b]
+
+
 def test_call_refusals():
     k, v, table = _shared_pools([20, 9], [], 8, 2, 16, 1)
     plan = PagedPlan([20, 9], heads=4, kv_heads=2, device="cpu")

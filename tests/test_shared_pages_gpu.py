@@ -169,6 +169,31 @@ def test_infinite_scores_and_values():
     assert out[:2].isfinite().sum() == 2 * 4 * 128 - 4
 
 
+@pytest.mark.parametrize("lens, new, H, KVH, D, dtype", [
+    ([70], [3], 4, 1, 128, BF), ([40, 129], [6, 7], 4, 1, 64, F16), ([130], [30], 2, 1, 128, F16),
+    ([100, 3], [50, 5], 4, 2, 64, BF), ([300], [64], 4, 1, 128, BF), ([200], [150], 1, 1, 64, F16)])
+def test_values_of_later_tokens_stay_out(lens, new, H, KVH, D, dtype):
+    """Infinities and NaN among the values of a token that a row does not attend
+    to leave the row as it is, bit for bit."""
+    print(f"\n[case] values of later tokens lens={lens} new={new} H={H} D={D} {dtype}", flush=True)
+    q, k, v, table, plan = _case(lens, new, [], H, KVH, D, 8, dtype)
+    clean = paged_attention(q, k, v, table, plan)
+    t0 = 0
+    marks = []
+    for b, (n, t) in enumerate(zip(lens, new)):
+        for i, x in ((t - 1, math.nan), (t // 2, math.inf), (max(1, t - n + 1), -math.inf)):
+            d = (7 * i + 5) % D
+            v[table[b, (n - t + i) // 8].long(), (n - t + i) % 8, KVH - 1, d] = x
+            marks.append((t0, t, i, d, x))
+        t0 += t
+    out = paged_attention(q, k, v, table, plan)
+    hit = torch.zeros(out.shape, dtype=torch.bool)
+    for at, t, i, d, _ in marks:
+        hit[at + i:at + t, H - H // KVH:, d] = True
+    assert torch.equal(out.cpu()[~hit], clean.cpu()[~hit])
+    assert not out.cpu()[hit].isfinite().any()
+
+
 def test_strides_and_views():
     """Pools interleaved in one tensor, head-major pages, a table that is part of a
     wider one or one row for all, q of a fused projection, odd addresses."""
