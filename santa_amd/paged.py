@@ -43,8 +43,9 @@ _IP = ctypes.POINTER(ctypes.c_int)
 
 
 class _PlanInfo(ctypes.Structure):
-    _fields_ = [(n, _I) for n in ("tokens", "groups", "items", "merge_tokens", "max_len", "max_row", "heads",
-                                  "kv_heads")] + [(n, _L) for n in ("records", "ints", "pos_at", "merge_at", "parts_at", "list_at")]
+    _fields_ = ([(n, _I) for n in ("tokens", "groups", "items", "merge_tokens", "max_len", "max_row", "heads",
+                                   "kv_heads")]
+                + [(n, _L) for n in ("records", "ints", "pos_at", "merge_at", "parts_at", "list_at")])
 
 
 _lib_ready = None
@@ -316,8 +317,8 @@ def copy_pages(pools: Union[torch.Tensor, Iterable[torch.Tensor]], src: Sequence
         for (size, stride), ts in groups.items():
             if size == 0 and all(0 <= p < num_pages for p in pairs):
                 continue
-            _launch(device, _lib().santa_paged_copy, (_P * len(ts))(*[t.data_ptr() for t in ts]), len(ts), size, stride, num_pages,
-                    pairs, len(src))
+            pointers = (_P * len(ts))(*[t.data_ptr() for t in ts])
+            _launch(device, _lib().santa_paged_copy, pointers, len(ts), size, stride, num_pages, pairs, len(src))
         return
     for p in (*src, *dst):
         if not 0 <= p < num_pages:
@@ -464,6 +465,24 @@ def _strides(t: torch.Tensor, what: str) -> Sequence[int]:
     return strides[:-1]
 
 
+def _overlaps(t: torch.Tensor) -> bool:
+    """Whether elements of t share memory, or dimensions interleave."""
+    span = 1
+    if not t.is_contiguous():
+        for stride, size in sorted((s, n) for s, n in zip(t.stride(), t.shape) if n > 1):
+            if stride < span:
+                return True
+            span += stride * (size - 1)
+    return False
+
+
+def _packed(t: torch.Tensor) -> torch.Tensor:
+    """t, contiguous and 16-byte aligned."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t)
+
+
 def _table_rows(table: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """The table as the kernels address it, and its row stride: rows that do
     not overlap."""
@@ -502,23 +521,21 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages
         raise ValueError(f"D mismatch: qkv {D}, pages {k_pages.shape[3]}")
     if D % 2 or cos.shape != (plan.tokens, D) or sin.shape != cos.shape:
         raise ValueError(f"cos and sin must be [{plan.tokens}, D], D even")
-    for t in (cos, sin):
-        if t.device != qkv.device or t.dtype != qkv.dtype:
-            raise ValueError("cos and sin must have the device and dtype of qkv")
-    if (qkv.is_cuda and qkv.dtype in (torch.bfloat16, torch.float16) and D % 16 == 0
+    device, dtype = qkv.device, qkv.dtype
+    if cos.device != device or sin.device != device or cos.dtype != dtype or sin.dtype != dtype:
+        raise ValueError("cos and sin must have the device and dtype of qkv")
+    if (device.type == "cuda" and dtype in (torch.bfloat16, torch.float16) and D % 16 == 0
             and _plain(qkv, cos, sin, k_pages, v_pages)):
         strides = (*_strides(k_pages, "k_pages"), *_strides(v_pages, "v_pages"))
-        for t in (k_pages, v_pages):
-            if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
-                raise ValueError("pages that are written must not overlap")
-        qkv, cos, sin = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else
-                         torch.empty(t.shape, dtype=t.dtype, device=t.device).copy_(t) for t in (qkv, cos, sin))
-        q = torch.empty(plan.tokens, H, D, dtype=qkv.dtype, device=qkv.device)
+        if _overlaps(k_pages) or _overlaps(v_pages):
+            raise ValueError("rows of pages that are written must not overlap")
+        qkv, cos, sin = _packed(qkv), _packed(cos), _packed(sin)
+        q = qkv.new_empty((plan.tokens, H, D))
         table, row = _table_rows(block_table)
         if plan.tokens:
-            _launch(qkv.device, _lib().santa_paged_rope_append, qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), q.data_ptr(),
-                    k_pages.data_ptr(), v_pages.data_ptr(), int(qkv.dtype == torch.float16), D, k_pages.shape[0],
-                    k_pages.shape[1], (_L * 6)(*strides), table.data_ptr(), row, table.shape[0],
+            _launch(device, _lib().santa_paged_rope_append, qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+                    q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), int(dtype == torch.float16), D,
+                    k_pages.shape[0], k_pages.shape[1], (_L * 6)(*strides), table.data_ptr(), row, table.shape[0],
                     ctypes.byref(plan._info), plan._data.data_ptr())
         return q
     wide = torch.float64 if qkv.dtype == torch.float64 else torch.float32
@@ -602,7 +619,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
     if not 1e-37 < scale < 1e37:  # normal in float32, times log2(e) too
         raise ValueError(f"scale must be positive and finite; got {scale}")
-    if not (q.is_cuda and q.dtype in (torch.bfloat16, torch.float16) and D in (64, 128)
+    device = q.device
+    if not (device.type == "cuda" and q.dtype in (torch.bfloat16, torch.float16) and D in (64, 128)
             and _plain(q, k_pages, v_pages)):
         return _attention_expressions(q, k_pages, v_pages, block_table, plan, scale)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
@@ -611,13 +629,14 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     try:
         sq = _strides(q, "q")
     except ValueError:
-        q = torch.empty(q.shape, dtype=q.dtype, device=q.device).copy_(q)
+        q = _packed(q)
         sq = _strides(q, "q")
     strides = (_L * 8)(*sq, *_strides(k_pages, "k_pages"), *_strides(v_pages, "v_pages"))
     table, row = _table_rows(block_table)
     info = ctypes.byref(plan._info)
-    workspace = torch.empty(_lib().santa_paged_workspace_size(info, D), dtype=torch.uint8, device=q.device)
-    _launch(q.device, _lib().santa_paged_attention, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(),
+    lib = _lib()
+    workspace = torch.empty(lib.santa_paged_workspace_size(info, D), dtype=torch.uint8, device=device)
+    _launch(device, lib.santa_paged_attention, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(),
             int(q.dtype == torch.float16), D, k_pages.shape[0], k_pages.shape[1], strides, table.data_ptr(), row,
             table.shape[0], info, plan._data.data_ptr(), scale, workspace.data_ptr(), workspace.numel())
     return out
