@@ -53,7 +53,10 @@ struct RemapArgs {
   int n;
 };
 
-// Workgroup (piece of the page, pair, pool).
+// Workgroup (piece of the page, pair, pool): 16 KiB in flight per workgroup, all
+// pairs and up to 64 pools of a launch at once.  Bound by HBM: 5.0 TB/s read and
+// written together where half of a batch's pages are closed up (898 MB in 180 us;
+// a plain copy of 2 GiB reaches 4.8 TB/s).
 __global__ __launch_bounds__(kCopyThreads) void copy_pages_kernel(CopyArgs a) {
   char* const pool = a.pool[blockIdx.z];
   const PageCopy c = a.pair[blockIdx.y];
@@ -69,6 +72,7 @@ __global__ __launch_bounds__(kCopyThreads) void copy_pages_kernel(CopyArgs a) {
     if (i0 + k * kCopyThreads < a.vecs) dst[i0 + k * kCopyThreads] = v[k];
 }
 
+// A workgroup per edit; a few us whatever it holds (64 rows of 2048 entries 3.7).
 __global__ __launch_bounds__(256) void edit_table_kernel(EditArgs a) {
   const TableEdit e = a.edit[blockIdx.x];
   int* dst = a.table + e.row * a.stride + e.col;
@@ -135,8 +139,12 @@ struct Pages {
 
 __device__ __forceinline__ int in_pool(const Pages& pg, int page) { return min(max(page, 0), pg.num_pages - 1); }
 
-// A thread takes dims d .. d + 7 and d + D/2 .. d + D/2 + 7 of one head of one
-// token, the two pieces that rotate-half combines.
+// y_d = x_d cos_d - x_{d + D/2} sin_d and y_{d + D/2} = x_{d + D/2} cos_{d + D/2}
+// + x_d sin_{d + D/2}: a thread takes dims d .. d + 7 and d + D/2 .. d + D/2 + 7
+// of one head of one token, the two pieces that the formula combines, so that qkv
+// is read and q, k and v are written once, in 16-byte pieces.  Bound by HBM: 27
+// thousand tokens of 32 + 2 x 8 heads of 128 in 69 us, 5.7 TB/s read and written;
+// one token for each of 64 sequences is latency (3.7 us).
 template <bool BF16>
 __global__ __launch_bounds__(256) void rope_append_kernel(const uint16_t* __restrict__ qkv,
                                                           const uint16_t* __restrict__ cos_,
@@ -184,6 +192,36 @@ __global__ __launch_bounds__(256) void rope_append_kernel(const uint16_t* __rest
 }
 
 // ----------------------------------------------------------------- attention
+// out = sum_n p_n v_n / sum_n p_n over the tokens n <= the row's position, p_n =
+// exp(scale q k_n - m), m a running reference near the largest score: one pass
+// over K and V.  A row is a (token, query head); the rows of a KV head that read
+// the same tokens form a block of up to 256, and read each tile of 64 tokens once:
+// the new tokens of a sequence or, over a prefix that sequences have in common,
+// those of all of them.  S^T = K Q^T and O^T += V^T P^T by 32x32x16 products, a
+// lane holding one row throughout, so that the softmax needs one exchange (with
+// the other half of the wave) and P^T never leaves the registers.
+//
+// One workgroup of 8 waves per compute unit, with a ring of tiles in LDS (128
+// KiB: 4 of K and V at D 128, 8 at D 64) that asynchronous loads fill ahead of
+// their use and across items.  The plan gives every workgroup a run of items of
+// about the same cost, one resident round; long blocks are cut between
+// workgroups, and their parts (sum, mass, reference) joined by merge_kernel.
+// KV head h's workgroups are those of numbers h modulo the KV heads, so that with
+// 8 of them an XCD's L2 holds one head (16 unshared sequences: 280 us, against
+// 294 with whole sequences side by side).
+//
+// What bounds it, at D 128 in bf16.  Few rows: HBM, 5.6 TB/s over 16-token pages
+// (16 sequences of 1000 to 40 000 tokens, 32 query and 8 KV heads, 1.55 GB:
+// 277 us; a ring of half or twice the depth, or two workgroups per compute unit,
+// change nothing).  256 rows: the matrix products and the softmax, each half of a
+// SIMD's cycles, and the clock, which is at 2.0 GHz then: 985 TFLOP/s behind
+// shared prompts (six sequences of 4000 shared, 100 to 1300 own and 1300 new
+// tokens, 318 us), where a plain product of 8192^3 reaches 1202; running the two
+// waves of a SIMD half a tile apart, products of one beside the softmax of the
+// other, or leaner steps, give back in clock what they save in cycles.  A batch
+// behind a long prompt has both: 64 sequences behind 32k tokens 110 us, 32 of 64
+// query heads behind 128k 216 us.  Little work: latency, about 10 us for the
+// first loads, one tile, the join of the waves and the output.
 constexpr int kWaves = 8;
 // Above this a row's reference in log2 units is subtracted from the scores before
 // they are scaled: fma(score, scale, -round(m * scale)) is off by half an ulp of
@@ -230,6 +268,12 @@ __device__ __forceinline__ void wait_loads() {
 // tiles (a quarter more vector work); probabilities up to 2^8 round as well as
 // those up to 1.
 constexpr float kHeadroom = 8.0f;
+
+template <bool BF16>
+__device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) {
+  return make_uint2(f32_to_h16<BF16>(a) | static_cast<uint32_t>(f32_to_h16<BF16>(b)) << 16,
+                    f32_to_h16<BF16>(c) | static_cast<uint32_t>(f32_to_h16<BF16>(d)) << 16);
+}
 
 // acc + the eight 16-bit values of v.
 template <bool BF16>
@@ -299,8 +343,9 @@ __device__ __forceinline__ void look_up(const Loader& w, Cursor& c) {
   const int n = min(c.begin + (c.t + static_cast<int>(threadIdx.x & 63)) * kTile + 8 * w.wave, min(c.end, w.limit) - 1);
   const uint32_t page = min(max(w.table[c.row * w.stride + (n >> w.shift)], 0), w.num_pages - 1);
   const uint32_t r = n & ((1 << w.shift) - 1) & ~7;
-  const uint64_t k = reinterpret_cast<uint64_t>(w.k) + static_cast<uint64_t>(page) * w.sk_p + static_cast<uint64_t>(r) * w.sk_r;
-  const uint64_t v = reinterpret_cast<uint64_t>(w.v) + static_cast<uint64_t>(page) * w.sv_p + static_cast<uint64_t>(r) * w.sv_r;
+  const uint64_t p64 = page, r64 = r;
+  const uint64_t k = reinterpret_cast<uint64_t>(w.k) + p64 * w.sk_p + r64 * w.sk_r;
+  const uint64_t v = reinterpret_cast<uint64_t>(w.v) + p64 * w.sv_p + r64 * w.sv_r;
   c.k_lo = static_cast<uint32_t>(k), c.k_hi = static_cast<uint32_t>(k >> 32) & 0xffff;
   c.v_lo = static_cast<uint32_t>(v), c.v_hi = static_cast<uint32_t>(v >> 32) & 0xffff;
   // waited for here, once in 64 tiles, and not at every use
@@ -562,8 +607,8 @@ struct Shares {
 // workgroup's items.
 template <bool BF16, int D, int RG>
 __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv, const Loader& w, Cursor& cur,
-                                       const uint32_t (&lk)[2], const uint32_t (&lv)[2], uint32_t& tile, uint32_t& loaded,
-                                       u32x4* stages, Shares* x) {
+                                       const uint32_t (&lk)[2], const uint32_t (&lv)[2], uint32_t& tile,
+                                       uint32_t& loaded, u32x4* stages, Shares* x) {
   using G = Geometry<D>;
   constexpr int KB = RG == 8 ? 2 : 1;                       // 32s of a tile's tokens that a wave takes
   constexpr int DH = RG >= 4 ? 1 : 2, MB = D / 32 / DH;     // parts of the dims, 32s of them in each
@@ -722,10 +767,8 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
       for (int e = 0; e < 16; e += 4) {
-        uint2 v;
-        v.x = f32_to_h16<BF16>(o[mb][e] * inv) | (static_cast<uint32_t>(f32_to_h16<BF16>(o[mb][e + 1] * inv)) << 16);
-        v.y = f32_to_h16<BF16>(o[mb][e + 2] * inv) | (static_cast<uint32_t>(f32_to_h16<BF16>(o[mb][e + 3] * inv)) << 16);
-        *reinterpret_cast<uint2*>(orow + 32 * mb + 2 * e + 4 * half) = v;
+        *reinterpret_cast<uint2*>(orow + 32 * mb + 2 * e + 4 * half) =
+            pack4<BF16>(o[mb][e] * inv, o[mb][e + 1] * inv, o[mb][e + 2] * inv, o[mb][e + 3] * inv);
       }
     return;
   }
@@ -798,8 +841,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_attention_kernel(AttnArg
 }
 
 // Joins the parts of a (token, head): D / 4 lanes, a team, hold four dims each of
-// every part that they take.  kOne: the teams of a workgroup take the parts of one
-// row in turn; otherwise each has a row of its own.
+// every part that they take, in one pass with a running maximum.  kOne: the teams
+// of a workgroup take the parts of one row in turn; otherwise each has a row of its
+// own.  Parts come in fixed order, so that the same call gives the same bits.
+// Latency bound with few rows (128 rows 3.7 us, 2048 of about 14 parts 6.6); 58
+// thousand rows of two parts, 75 MB: 19 us, 3.9 TB/s.
 template <bool BF16, int D, bool kOne>
 __global__ __launch_bounds__(256) void merge_kernel(const float* __restrict__ part, const float2* __restrict__ part_ml,
                                                     const int* __restrict__ tokens, const int4* __restrict__ parts,
@@ -862,10 +908,8 @@ __global__ __launch_bounds__(256) void merge_kernel(const float* __restrict__ pa
     for (int t = 0; t < kTeams; ++t) add(s_m[t], s_z[t], s_o[t][d4]);
   }
   const float inv = blind ? 0.0f : 1.0f / z;
-  uint2 v;
-  v.x = f32_to_h16<BF16>(acc.x * inv) | (static_cast<uint32_t>(f32_to_h16<BF16>(acc.y * inv)) << 16);
-  v.y = f32_to_h16<BF16>(acc.z * inv) | (static_cast<uint32_t>(f32_to_h16<BF16>(acc.w * inv)) << 16);
-  *reinterpret_cast<uint2*>(out + (static_cast<size_t>(tok) * H + h) * D + 4 * d4) = v;
+  *reinterpret_cast<uint2*>(out + (static_cast<size_t>(tok) * H + h) * D + 4 * d4) =
+      pack4<BF16>(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
 }
 
 // A block table, pools and plan that belong together.
@@ -979,7 +1023,8 @@ extern "C" int santa_paged_rope_append(const void* qkv, const void* cos_, const 
   if (rc != SANTA_OK) return rc;
   if (!cos_ || !sin_ || (reinterpret_cast<uintptr_t>(cos_) | reinterpret_cast<uintptr_t>(sin_)) % 16 != 0)
     return set_error(SANTA_ERR_INVALID, "rope_append: cos and sin must be 16-byte aligned");
-  if (D <= 0 || D % 16 != 0) return set_error(SANTA_ERR_UNSUPPORTED, "rope_append: D must be a multiple of 16. Got D=%d", D);
+  if (D <= 0 || D % 16 != 0)
+    return set_error(SANTA_ERR_UNSUPPORTED, "rope_append: D must be a multiple of 16. Got D=%d", D);
   const int H = info->heads, KVH = info->kv_heads;
   const long long total = static_cast<long long>(info->tokens) * (H + 2LL * KVH) * (D / 16);
   if (total >= 0x7fffff00LL) return set_error(SANTA_ERR_INVALID, "too many new tokens");
@@ -1037,10 +1082,11 @@ extern "C" int santa_paged_attention(const void* q, const void* k_pages, const v
     return set_error(SANTA_ERR_UNSUPPORTED, "paged_attention: pages must lie less than 4 GiB apart");
   // rows past the end are told by their offset from the first of eight
   if (strides[3] < D || strides[6] < D || strides[3] >= 1LL << 26 || strides[6] >= 1LL << 26)
-    return set_error(SANTA_ERR_UNSUPPORTED, "paged_attention: the rows of a page must lie at least D and less than 2^26 "
-                                            "elements apart");
-  a.sk_p = static_cast<uint32_t>(2 * strides[2]), a.sk_r = static_cast<uint32_t>(2 * strides[3]), a.sk_h = 2 * strides[4];
-  a.sv_p = static_cast<uint32_t>(2 * strides[5]), a.sv_r = static_cast<uint32_t>(2 * strides[6]), a.sv_h = 2 * strides[7];
+    return set_error(SANTA_ERR_UNSUPPORTED,
+                     "paged_attention: the rows of a page must lie at least D and less than 2^26 elements apart");
+  a.sk_p = static_cast<uint32_t>(2 * strides[2]), a.sk_r = static_cast<uint32_t>(2 * strides[3]);
+  a.sv_p = static_cast<uint32_t>(2 * strides[5]), a.sv_r = static_cast<uint32_t>(2 * strides[6]);
+  a.sk_h = 2 * strides[4], a.sv_h = 2 * strides[7];
   a.KVH = KVH;
   a.GH = H / KVH;
   a.scale_log2 = 1.44269504088896340736f * scale;
@@ -1055,7 +1101,9 @@ extern "C" int santa_paged_attention(const void* q, const void* k_pages, const v
       hipLaunchKernelGGL((paged_attention_kernel<BF16, kD>), dim3(static_cast<unsigned>(info->groups) * KVH),
                          dim3(64 * kWaves), 0, stream, a);
     const long long rows = static_cast<long long>(info->merge_tokens) * H;
-    // four waves a row while that leaves them one resident round
+    // a workgroup per row up to one resident round of them (2048 rows of 14 parts
+    // 6.6 us, against 7.6 with a team each, and of 24 parts 8.9 against 11.4); above
+    // it the rows have few parts (58 thousand of two 57 us, against 19.5)
     const bool wide = rows <= 2048;
     for (long long r = 0; r < rows; r += 1 << 22) {  // a launch holds fewer than 2^32 threads
       const int n = static_cast<int>(std::min<long long>(rows - r, 1 << 22));

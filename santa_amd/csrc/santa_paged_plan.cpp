@@ -114,7 +114,8 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
     }
     for (int i = 0; i < t; i += block_tokens) {
       const int k = std::min(block_tokens, t - i);
-      blocks.push_back({0, row, prefix[b], std::max(prefix[b], std::min(n, n - t + i + k)), first[b] + i, k, n - t + i});
+      const int end = std::max(prefix[b], std::min(n, n - t + i + k));
+      blocks.push_back({0, row, prefix[b], end, first[b] + i, k, n - t + i});
     }
   }
 
@@ -202,7 +203,8 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
   if (plan_ints < info->ints) return set_error(SANTA_ERR_INVALID, "the plan does not fit its buffer");
 
   std::memset(plan, 0, static_cast<size_t>(info->ints) * sizeof(int));
-  for (int i = 0; i < info->items; ++i) plan[static_cast<size_t>(i) * kItemInts + offsetof(Item, next) / sizeof(int)] = -1;
+  for (int i = 0; i < info->items; ++i)
+    plan[static_cast<size_t>(i) * kItemInts + offsetof(Item, next) / sizeof(int)] = -1;
   // a slot's first piece at the slot's number, the others behind them
   int more = static_cast<int>(used), last = -1;
   for (size_t i = 0; i < pieces.size(); ++i) {

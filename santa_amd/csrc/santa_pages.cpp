@@ -34,7 +34,9 @@ struct santa_pages {
   bool remap = false;
 
   int num_pages() const { return static_cast<int>(refs.size()); }
-  int pages_for(int tokens) const { return static_cast<int>((static_cast<int64_t>(tokens) + page_size - 1) / page_size); }
+  int pages_for(int tokens) const {
+    return static_cast<int>((static_cast<int64_t>(tokens) + page_size - 1) / page_size);
+  }
   // The free page of the lowest number (there is one).
   int take() {
     while (!open[hint]) ++hint;
@@ -123,8 +125,8 @@ int extend(santa_pages* p, const int* seqs, const int* tokens, int n) {
     }
     const int64_t len = static_cast<int64_t>(s.len) + tokens[i];
     if (len > static_cast<int64_t>(p->row_pages) * p->page_size) {
-      rc = set_error(SANTA_ERR_INVALID, "sequence %d would hold %lld tokens; the block table has room for %lld", seqs[i],
-                     static_cast<long long>(len), static_cast<long long>(p->row_pages) * p->page_size);
+      rc = set_error(SANTA_ERR_INVALID, "sequence %d would hold %lld tokens; the block table has room for %lld",
+                     seqs[i], static_cast<long long>(len), static_cast<long long>(p->row_pages) * p->page_size);
       break;
     }
     need += p->pages_for(static_cast<int>(len)) - static_cast<int>(s.pages.size());
@@ -219,7 +221,8 @@ extern "C" int santa_pages_create(int num_pages, int page_size, int max_seqs, in
 extern "C" void santa_pages_destroy(santa_pages* p) { delete p; }
 
 extern "C" int santa_pages_add(santa_pages* p, const int* lengths, int n, int* seqs) {
-  if (!p || n < 0 || (n > 0 && (!lengths || !seqs))) return set_error(SANTA_ERR_INVALID, "bad santa_pages_add arguments");
+  if (!p || n < 0 || (n > 0 && (!lengths || !seqs)))
+    return set_error(SANTA_ERR_INVALID, "bad santa_pages_add arguments");
   return guarded([&] {
     p->begin();
     int rc = new_rows(p, n, seqs);

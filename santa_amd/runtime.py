@@ -670,7 +670,7 @@ class RandomLlama:
                     for c in range(0, len(h), mlp_chunk):
                         o[c:c + mlp_chunk] = lin(lin(x[c:c + mlp_chunk], L["wgu"], swiglu=True), L["wd"])
                 nxt = self.layers[li + 1]["ln1"] if li + 1 < len(self.layers) else self.norm
-                x = _FusedOps.add_rms_norm(h, o, nxt, s.rms_eps)  # h += the MLP's, then the next layer's (or final) norm
+                x = _FusedOps.add_rms_norm(h, o, nxt, s.rms_eps)  # h += o; the next layer's norm, or the final one
         else:
             for li, L in enumerate(self.layers):
                 h = h + F.linear(attend(li, F.linear(_rms_norm(h, L["ln1"], s.rms_eps), L["wqkv"])), L["wo"])
