@@ -396,7 +396,8 @@ int santa_pages_apply(const santa_pages* p, const void* const* pools, int n_pool
  * other lengths with the same new_tokens and groups give a plan of the same
  * info (for captured graphs whose plan changes between replays).  info is
  * always written; plan (info->ints ints, 16-byte aligned, to be copied to the
- * device as it is) where it is not NULL. */
+ * device as it is) where it is not NULL.  Workgroups are planned for the current
+ * device. */
 typedef struct santa_paged_plan_info {
   int tokens;       /* queries: the sum of new_tokens */
   int groups;       /* workgroups per KV head, and the items they work through */

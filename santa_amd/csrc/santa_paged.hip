@@ -212,7 +212,7 @@ __global__ __launch_bounds__(256) void rope_append_kernel(const uint16_t* __rest
 //
 // What bounds it, at D 128 in bf16.  Few rows: HBM, 5.6 TB/s over 16-token pages
 // (16 sequences of 1000 to 40 000 tokens, 32 query and 8 KV heads, 1.55 GB:
-// 277 us; a ring of half or twice the depth, or two workgroups per compute unit,
+// 277 us; half the ring, or two workgroups of half the waves per compute unit,
 // change nothing).  256 rows: the matrix products and the softmax, each half of a
 // SIMD's cycles, and the clock, which is at 2.0 GHz then: 985 TFLOP/s behind
 // shared prompts (six sequences of 4000 shared, 100 to 1300 own and 1300 new
