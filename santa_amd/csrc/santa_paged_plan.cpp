@@ -5,7 +5,7 @@
 #include <cstddef>
 #include <cstdint>
 #include <cstring>
-#include <new>
+#include <exception>
 #include <vector>
 
 #include "santa_amd.h"
@@ -15,6 +15,9 @@
 namespace santa {
 namespace paged {
 namespace {
+
+// The kernel's 32-bit positions run past a sequence's end by up to 64 tiles.
+constexpr int kMaxLen = 1 << 30;
 
 // Rows (token, query head of one KV head) that pass over the same tokens
 // together: those of the tokens tok0 .. tok0 + ntok - 1 of the batch, or of
@@ -66,9 +69,12 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
     const int n = in.lens[b], t = in.new_tokens[b], row = in.rows ? in.rows[b] : b;
     if (n < 0 || t < 0) return set_error(SANTA_ERR_INVALID, "a sequence has 0 or more tokens and new tokens");
     if (row < 0) return set_error(SANTA_ERR_INVALID, "bad block table row %d", row);
+    if (n > kMaxLen || t > kMaxLen)
+      return set_error(SANTA_ERR_UNSUPPORTED, "the paged attention takes up to %d tokens per sequence. Got %d", kMaxLen,
+                       std::max(n, t));
     first[b] = static_cast<int>(tokens);
     tokens += t;
-    if (tokens > (1 << 30) / GH) return set_error(SANTA_ERR_INVALID, "too many new tokens");
+    if (tokens > (1 << 26) / GH) return set_error(SANTA_ERR_INVALID, "too many new tokens");
     info->max_len = std::max(info->max_len, n);
     info->max_row = std::max(info->max_row, row);
     const int g = in.group ? in.group[b] : -1;
@@ -104,7 +110,7 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
       }
     const int n = static_cast<int>(list.size()) - group_list[g];
     for (int i = 0; i < n; i += block_tokens)
-      blocks.push_back({kFromList, lead[g], 0, common, group_list[g] + i, std::min(block_tokens, n - i), INT_MAX / 2});
+      blocks.push_back({kFromList, lead[g], 0, common, group_list[g] + i, std::min(block_tokens, n - i), kMaxLen});
   }
   for (int b = 0; b < in.B; ++b) {
     const int n = in.lens[b], t = in.new_tokens[b], row = in.rows ? in.rows[b] : b;
@@ -261,7 +267,7 @@ extern "C" int santa_paged_plan(const int* lens, const int* new_tokens, const in
     return paged::build({lens, new_tokens, rows, B, n_groups > 0 ? group : nullptr, shared, n_groups, heads, kv_heads,
                          fixed},
                         info, plan, plan_ints);
-  } catch (const std::bad_alloc&) {
+  } catch (const std::exception&) {  // vectors that do not fit
     return set_error(SANTA_ERR_INVALID, "out of host memory");
   }
 }

@@ -10,6 +10,7 @@
 #include <algorithm>
 #include <cstdint>
 #include <cstring>
+#include <exception>
 #include <new>
 #include <vector>
 
@@ -90,7 +91,7 @@ template <class F>
 int guarded(F f) {
   try {
     return f();
-  } catch (const std::bad_alloc&) {
+  } catch (const std::exception&) {
     return set_error(SANTA_ERR_INVALID, "out of host memory");
   }
 }

@@ -146,9 +146,10 @@ class PagedKVCache:
         self.layers, self.num_pages, self.page_size = layers, num_pages, page_size
         self.kv_heads, self.head_dim, self.max_seqs = kv_heads, head_dim, max_seqs
         shape = (num_pages, page_size, kv_heads, head_dim)
-        self.k = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(layers)]
-        self.v = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(layers)]
-        self.block_table = torch.zeros(max_seqs, row_pages, dtype=torch.int32, device=device)
+        with torch.inference_mode(False):  # they are written to in any mode
+            self.k = tuple(torch.zeros(shape, dtype=dtype, device=device) for _ in range(layers))
+            self.v = tuple(torch.zeros(shape, dtype=dtype, device=device) for _ in range(layers))
+            self.block_table = torch.zeros(max_seqs, row_pages, dtype=torch.int32, device=device)
         self._page_bytes = page_size * kv_heads * head_dim * self.block_table.new_empty(0, dtype=dtype).element_size()
         if device.type == "cuda" and self._page_bytes % 16:
             raise ValueError("pages must be whole 16-byte pieces")
@@ -177,7 +178,7 @@ class PagedKVCache:
     def pages(self, seq: int) -> List[int]:
         """The pages that a sequence holds, first tokens first."""
         row = _IP()
-        n = _lib().santa_pages_row(self._pages, seq, ctypes.byref(row))
+        n = _lib().santa_pages_row(self._pages, *_ints([seq]), ctypes.byref(row))
         if n < 0:
             raise RuntimeError(f"no sequence {seq} in the cache")
         return row[:n]
@@ -208,8 +209,8 @@ class PagedKVCache:
     def fork(self, seq: int, n: int = 1) -> List[int]:
         """n new sequences with the same tokens, which hold the same pages."""
         self._may_change()
-        if n < 0:
-            raise ValueError(f"n must be >= 0; got {n}")
+        if not 0 <= n <= self.max_seqs:
+            raise ValueError(f"n must be in [0, {self.max_seqs}]; got {n}")
         out = (ctypes.c_int * n)()
         _check(_lib().santa_pages_fork(self._pages, *_ints([seq, n]), out))
         self._apply()
@@ -236,6 +237,9 @@ class PagedKVCache:
         self.lengths(seqs)
         if seqs == list(range(seqs[0], seqs[0] + len(seqs))) if seqs else True:
             return self.block_table[seqs[0]:seqs[0] + len(seqs)] if seqs else self.block_table[:0]
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("the rows of these sequences do not follow one another: they cannot be gathered while a "
+                               "graph is captured")
         at = torch.tensor(seqs, dtype=torch.int64, pin_memory=self.device.type == "cuda")
         return self.block_table.index_select(0, at.to(self.device, non_blocking=True))
 
@@ -314,6 +318,8 @@ def copy_pages(pools: Union[torch.Tensor, Iterable[torch.Tensor]], src: Sequence
         groups.setdefault((size, stride), []).append(t)
     if device.type == "cuda":
         pairs = _ints([p for pair in zip(src, dst) for p in pair])
+        if any(size % 16 or stride % 16 for size, stride in groups) or any(t.data_ptr() % 16 for t in pools):
+            raise RuntimeError("pages must be whole 16-byte pieces, 16-byte aligned")
         for (size, stride), ts in groups.items():
             if size == 0 and all(0 <= p < num_pages for p in pairs):
                 continue
@@ -357,7 +363,8 @@ class PagedPlan:
                  device="cuda", fixed: bool = False):
         lens = _int_list(seq_lens, "seq_lens")
         B = len(lens)
-        self.heads, self.kv_heads, self.fixed = int(heads), int(kv_heads), bool(fixed)
+        self.heads, self.kv_heads = _ints([int(heads), int(kv_heads)])
+        self.fixed = bool(fixed)
         self.device = _device(device)
         self.new_tokens = [new_tokens] * B if isinstance(new_tokens, int) else _int_list(new_tokens, "new_tokens")
         self.rows = list(range(B)) if rows is None else _int_list(rows, "rows")
@@ -399,12 +406,13 @@ class PagedPlan:
                                            int(self.fixed), ctypes.byref(info), buffer, n)
 
         _check(build(None, 0))
-        host = torch.empty(max(1, info.ints), dtype=torch.int32, pin_memory=cuda)
-        _check(build(host.data_ptr(), info.ints))
-        if self._data is not None and self._data.shape == host.shape:
-            self._data.copy_(host, non_blocking=True)
-        else:
-            self._data = host.to(self.device, non_blocking=True)
+        with torch.inference_mode(False):  # updated in any mode
+            host = torch.empty(max(1, info.ints), dtype=torch.int32, pin_memory=cuda)
+            _check(build(host.data_ptr(), info.ints))
+            if self._data is not None and self._data.shape == host.shape:
+                self._data.copy_(host, non_blocking=True)
+            else:
+                self._data = host.to(self.device, non_blocking=True)
         self._info, self.seq_lens = info, lens
 
     @property

@@ -638,8 +638,11 @@ class RandomLlama:
             raise ValueError(f"{tokens.numel()} tokens do not give {B} sequences {new} new ones, at least 1 each")
         if (cache.layers, cache.kv_heads, cache.head_dim) != (s.layers, s.kv_heads, D) or cache.dtype != self.dtype:
             raise ValueError("the cache does not have the model's layers, KV heads, head_dim and dtype")
+        if cache.device != self.embed.device:
+            raise ValueError(f"the cache is on {cache.device}, the model on {self.embed.device}")
         if backend is not None and max(new) > 1:
             raise ValueError("a backend decodes one new token per sequence")
+        h = self.embed[tokens.reshape(-1)]  # [N, hidden]
         cache.extend(seqs, new)
         plan = cache.plan(seqs, s.heads, new)
         cos, sin = _rope_cos_sin(plan.positions, D, s.rope_theta, self.dtype)  # [N, D]
@@ -655,7 +658,6 @@ class RandomLlama:
                 a = paged_attention(q, cache.k[li], cache.v[li], table, plan)
             return a.reshape(len(q), s.heads * D)
 
-        h = self.embed[tokens.reshape(-1)]  # [N, hidden]
         fused = self.device.type == "cuda" and self.dtype == torch.bfloat16
         if fused:
             lin = _FusedOps.linear

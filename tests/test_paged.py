@@ -532,6 +532,39 @@ def test_call_refusals():
             call()
 
 
+def test_sizes_that_are_refused():
+    """Lengths past the kernel's 32-bit positions, counts that do not fit, and
+    numbers that would wrap: refused, with nothing changed."""
+    for lens, kw in (([(1 << 30) + 1], {}), ([(1 << 31) - 1], {}), ([5], {"new_tokens": 1 << 30}),
+                     ([5], {"new_tokens": (1 << 26) + 1}), ([5] * 70, {"new_tokens": 1 << 20})):
+        with pytest.raises(RuntimeError):
+            PagedPlan(lens, heads=1, kv_heads=1, device="cpu", **kw)
+    assert PagedPlan([1 << 30], heads=1, kv_heads=1, device="cpu").tokens == 1
+    for heads in ((1 << 32) + 4, 1 << 40):
+        with pytest.raises(ValueError):
+            PagedPlan([5], heads=heads, kv_heads=1, device="cpu")
+    cache = _cache()
+    a, = cache.add([5])
+    for call in (lambda: cache.fork(a, 1 << 40), lambda: cache.fork(a, cache.max_seqs + 1), lambda: cache.fork(a, -1),
+                 lambda: cache.pages((1 << 32) + a)):
+        with pytest.raises(ValueError):
+            call()
+    assert cache.used_pages == 1 and cache.lengths([a]) == [5]
+
+
+def test_inference_mode():
+    """A cache and a plan made in inference mode are used outside of it."""
+    with torch.inference_mode():
+        cache = _cache()
+        a, = cache.add([9])
+        plan = cache.plan([a], 2)
+    b, = cache.fork(a)
+    cache.extend([b], 3)
+    plan.update([8])
+    q = torch.zeros(1, 2, 16)
+    assert paged_attention(q, cache.k[0], cache.v[0], cache.block_table, plan).shape == q.shape
+
+
 def test_library_refusals():
     """The C entries check what they are given before anything is launched."""
     lib = paged._lib()
@@ -620,6 +653,16 @@ def test_model_extends():
     with pytest.raises(RuntimeError, match="would hold"):
         model.extend(toks[:1, :99], cache, [a])
     assert cache.used_pages == used
+
+
+def test_model_refuses_before_the_cache_changes():
+    """Tokens that the model has no embedding for leave the cache as it was."""
+    model = RandomLlama(TINY, device="cpu", dtype=torch.float32, seed=1)
+    cache = _model_cache(TINY)
+    a, = cache.add([0])
+    with pytest.raises(IndexError):
+        model.extend(torch.full((1, 3), TINY.vocab), cache, [a])
+    assert cache.lengths([a]) == [0] and cache.used_pages == 0
 
 
 def test_backend_decodes_pages():

@@ -454,6 +454,51 @@ def test_copy_pages():
 SMALL = LlamaShape(hidden=512, intermediate=1024, heads=4, kv_heads=1, layers=2, vocab=1000)
 
 
+def test_copies_are_checked_before_any():
+    """Pools of pages that are no whole 16-byte pieces are refused before the
+    others' pages move."""
+    print("\n[case] copies refused", flush=True)
+    good = torch.arange(64, device="cuda").view(4, 16).float()
+    before = good.clone()
+    with pytest.raises(RuntimeError, match="16-byte"):
+        copy_pages([good, torch.zeros(4, 3, device="cuda")], [0], [1])
+    with pytest.raises(RuntimeError, match="16-byte"):
+        copy_pages([good, torch.zeros(4 * 16 + 1, device="cuda")[1:].view(4, 16)], [0], [1])
+    assert torch.equal(good, before)
+
+
+@pytest.mark.parametrize("D, KVH, new", [(128, 8, [1, 1]), (64, 16, [5, 40])])
+def test_offsets_past_32_bits(D, KVH, new):
+    """Pages that lie more than 4 GiB, and 2^31 elements, from the pools' start:
+    appended to, copied and attended to as in a small pool."""
+    print(f"\n[case] large pools D={D}", flush=True)
+    page, lens, H = 256, [900, 700], 4 * KVH
+    few = sum(-(-n // page) for n in lens)
+    num = (1 << 32) // (2 * page * KVH * D) + 2 * few  # K and V side by side: 8 GiB and some
+    both = torch.empty(num, 2, page, KVH, D, dtype=BF, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(1)
+    both[num - 2 * few:] = torch.randn(2 * few, 2, page, KVH, D, generator=g, device="cuda").bfloat16()
+    small = both[num - 2 * few:].clone()
+    q, qkv = (torch.randn(sum(new), n, D, generator=g, device="cuda").bfloat16() for n in (H, H + 2 * KVH))
+    cs = torch.randn(2, sum(new), D, generator=g, device="cuda").bfloat16()
+    order = torch.randperm(few, generator=torch.Generator().manual_seed(2))
+    rows = torch.zeros(2, 4, dtype=torch.int32)
+    rows[0, :4], rows[1, :3] = order[:4], order[4:7]
+    got = []
+    for pool, first in ((both, num - 2 * few), (small, 0)):
+        table = (rows + first).cuda()
+        plan = PagedPlan(lens, heads=H, kv_heads=KVH, new_tokens=new)
+        turned = rope_append(qkv, cs[0], cs[1], pool[:, 0], pool[:, 1], table, plan)
+        copy_pages([pool.view(pool.shape[0], -1)], list(range(first, first + few)),
+                   list(range(first + few, first + 2 * few)))
+        got.append((turned, paged_attention(q, pool[:, 0], pool[:, 1], table, plan),
+                    paged_attention(q, pool[:, 0], pool[:, 1], table + few, plan), pool[first:].clone()))
+    for a, b in zip(*got):
+        assert torch.equal(a, b)
+    assert torch.equal(got[0][1], got[0][2])
+    _check(got[0][1], _reference(q, small[:, 0], small[:, 1], rows.cuda(), lens, new), BF)
+
+
 @pytest.mark.parametrize("dtype", [BF, F16])
 def test_model_extends(dtype):
     """A prompt, samples of it with prompts of their own, decode steps and a
