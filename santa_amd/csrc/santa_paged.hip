@@ -5,7 +5,6 @@
 // counterpart in the reference, whose caches are contiguous and one per sequence
 // (tutorial_code/runtime_common.py:340-397).
 #include <algorithm>
-#include <climits>
 #include <cmath>
 #include <new>
 #include <vector>
@@ -594,8 +593,8 @@ __device__ __forceinline__ void barrier() {
 // LDS beside the stages, for what the waves of the same rows and dims hold of
 // different tokens.
 struct Shares {
-  float4 o[6][4][64];
-  float m[6][64], l[6][64];
+  float4 o[24][64];
+  float m[kWaves][64], l[kWaves][64];
 };
 
 // One item.  Its rows are RG groups of 32, each held by 8 / RG waves.  RG 8: one
@@ -713,74 +712,86 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv
         o[mb][e] += fabsf(low) < __builtin_inff() ? low : 0.0f;
       }
   }
-  if constexpr (TG > 1) {  // the parts of the tokens
-    const int first = (wave % DH + DH * rg) * (TG - 1);
-    if (tg > 0) {
-      x->m[first + tg - 1][lane] = m;
-      x->l[first + tg - 1][lane] = l;
-    }
-    float own = 0.0f, weight[TG - 1];
-#pragma unroll
-    for (int mb = 0; mb < MB; ++mb) {
-      if (tg > 0) {
-#pragma unroll
-        for (int e = 0; e < 16; e += 4)
-          x->o[first + tg - 1][e / 4][lane] = make_float4(o[mb][e], o[mb][e + 1], o[mb][e + 2], o[mb][e + 3]);
-      }
-      __syncthreads();
-      if (tg == 0) {
-        if (mb == 0) {
-          float top = m;
-#pragma unroll
-          for (int i = 0; i < TG - 1; ++i) top = fmaxf(top, x->m[first + i][lane]);
-          own = __builtin_amdgcn_exp2f((m - top) * a.scale_log2);
-          l *= own;
-          m = top;
-#pragma unroll
-          for (int i = 0; i < TG - 1; ++i) {
-            weight[i] = __builtin_amdgcn_exp2f((x->m[first + i][lane] - top) * a.scale_log2);
-            l = fmaf(x->l[first + i][lane], weight[i], l);
-          }
-        }
-#pragma unroll
-        for (int e = 0; e < 16; ++e) o[mb][e] *= own;
-#pragma unroll
-        for (int i = 0; i < TG - 1; ++i)
-#pragma unroll
-          for (int e = 0; e < 16; e += 4) {
-            const float4 v = x->o[first + i][e / 4][lane];
-            o[mb][e] = fmaf(v.x, weight[i], o[mb][e]);
-            o[mb][e + 1] = fmaf(v.y, weight[i], o[mb][e + 1]);
-            o[mb][e + 2] = fmaf(v.z, weight[i], o[mb][e + 2]);
-            o[mb][e + 3] = fmaf(v.w, weight[i], o[mb][e + 3]);
-          }
-      }
-      __syncthreads();
-    }
-    if (tg > 0 || (dup && (ql & 16))) return;
-  }
-  if (!any || r >= it.rows) return;
-  if (it.flags & kDirect) {
-    const float inv = pos < 0 ? 0.0f : 1.0f / l;
-    uint16_t* orow = a.out + (static_cast<size_t>(tok) * (a.KVH * a.GH) + h) * D + 32 * MB * dh;
+  // The parts of the tokens, each wave joining a share of the dims: EP of the
+  // four pieces that it has of every 32 of them.
+  constexpr int EP = 4 / TG;
+  float4 res[MB][EP];
+  if constexpr (TG == 1) {
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-      for (int e = 0; e < 16; e += 4) {
-        *reinterpret_cast<uint2*>(orow + 32 * mb + 2 * e + 4 * half) =
-            pack4<BF16>(o[mb][e] * inv, o[mb][e + 1] * inv, o[mb][e + 2] * inv, o[mb][e + 3] * inv);
+      for (int k = 0; k < EP; ++k)
+        res[mb][k] = make_float4(o[mb][4 * k], o[mb][4 * k + 1], o[mb][4 * k + 2], o[mb][4 * k + 3]);
+  } else {
+    const int team = TG * (wave % DH + DH * rg);  // its waves' number: team + tg
+    auto place = [&](int to, int from, int k) {
+      return x->o[((team + to) * (TG - 1) + (from < to ? from : from - 1)) * EP + k] + lane;
+    };
+    x->m[team + tg][lane] = m;
+    x->l[team + tg][lane] = l;
+    float own = 0.0f, weight[TG - 1];
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+#pragma unroll
+      for (int to = 0; to < TG; ++to)
+#pragma unroll
+        for (int k = 0; k < EP; ++k) {
+          const int e = 4 * (to * EP + k);
+          const float4 v = make_float4(o[mb][e], o[mb][e + 1], o[mb][e + 2], o[mb][e + 3]);
+          if (to == tg) res[mb][k] = v;
+          else *place(to, tg, k) = v;
+        }
+      __syncthreads();
+      if (mb == 0) {
+        float top = m;
+#pragma unroll
+        for (int i = 0; i < TG; ++i) top = fmaxf(top, x->m[team + i][lane]);
+        own = __builtin_amdgcn_exp2f((m - top) * a.scale_log2);
+        l *= own;
+        m = top;
+#pragma unroll
+        for (int i = 0; i < TG - 1; ++i) {
+          const int from = team + (i < tg ? i : i + 1);
+          weight[i] = __builtin_amdgcn_exp2f((x->m[from][lane] - top) * a.scale_log2);
+          l = fmaf(x->l[from][lane], weight[i], l);
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < EP; ++k) {
+        float4& c = res[mb][k];
+        c.x *= own, c.y *= own, c.z *= own, c.w *= own;
+#pragma unroll
+        for (int i = 0; i < TG - 1; ++i) {
+          const float4 v = *place(tg, i < tg ? i : i + 1, k);
+          c.x = fmaf(v.x, weight[i], c.x), c.y = fmaf(v.y, weight[i], c.y);
+          c.z = fmaf(v.z, weight[i], c.z), c.w = fmaf(v.w, weight[i], c.w);
+        }
+      }
+      __syncthreads();
+    }
+    if (dup && (ql & 16)) return;
+  }
+  if (!any || r >= it.rows) return;
+  const int d0 = 32 * MB * dh + (TG == 1 ? 0 : 8 * EP * tg) + 4 * half;  // of the first piece
+  if (it.flags & kDirect) {
+    const float inv = pos < 0 ? 0.0f : 1.0f / l;
+    uint16_t* orow = a.out + (static_cast<size_t>(tok) * (a.KVH * a.GH) + h) * D + d0;
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb)
+#pragma unroll
+      for (int k = 0; k < EP; ++k) {
+        const float4& c = res[mb][k];
+        *reinterpret_cast<uint2*>(orow + 32 * mb + 8 * k) = pack4<BF16>(c.x * inv, c.y * inv, c.z * inv, c.w * inv);
       }
     return;
   }
   const size_t rec = static_cast<size_t>(it.base) + static_cast<size_t>(kv) * it.rows + r;
-  float* prow = a.part + rec * D + 32 * MB * dh;
+  float* prow = a.part + rec * D + d0;
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
-    for (int e = 0; e < 16; e += 4)
-      *reinterpret_cast<float4*>(prow + 32 * mb + 2 * e + 4 * half) =
-          make_float4(o[mb][e], o[mb][e + 1], o[mb][e + 2], o[mb][e + 3]);
-  if (dh == 0 && half == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * rec) = make_float2(m, l);
+    for (int k = 0; k < EP; ++k) *reinterpret_cast<float4*>(prow + 32 * mb + 8 * k) = res[mb][k];
+  if (dh == 0 && tg == 0 && half == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * rec) = make_float2(m, l);
 }
 
 __device__ __forceinline__ Item read_item(const Loader& w, int i) {
