@@ -212,15 +212,17 @@ __global__ __launch_bounds__(256) void rope_append_kernel(const uint16_t* __rest
 // What bounds it, at D 128 in bf16.  Few rows: HBM, 5.6 TB/s over 16-token pages
 // (16 sequences of 1000 to 40 000 tokens, 32 query and 8 KV heads, 1.55 GB:
 // 277 us; half the ring, or two workgroups of half the waves per compute unit,
-// change nothing).  256 rows: the matrix products and the softmax, each half of a
-// SIMD's cycles, and the clock, which is at 2.0 GHz then: 985 TFLOP/s behind
-// shared prompts (six sequences of 4000 shared, 100 to 1300 own and 1300 new
-// tokens, 318 us), where a plain product of 8192^3 reaches 1202; running the two
+// change nothing).  256 rows: issue, of the products (0.42 of a SIMD's cycles), of
+// the softmax's vector work (about as many) and of the steps between them, which
+// hardly overlap: 985 TFLOP/s behind shared prompts (six sequences of 4000 shared,
+// 100 to 1300 own and 1300 new tokens, 314 us), where a plain product of 8192^3
+// reaches 1202.  Counted cycles of that kernel, 664 thousand as it is: the two
 // waves of a SIMD half a tile apart, products of one beside the softmax of the
-// other, or leaner steps, give back in clock what they save in cycles.  A batch
-// behind a long prompt has both: 64 sequences behind 32k tokens 110 us, 32 of 64
-// query heads behind 128k 216 us.  Little work: latency, about 10 us for the
-// first loads, one tile, the join of the waves and the output.
+// other, 685; loads issued between the products 711; steps without bookkeeping
+// 667; first products as soon as their first operand is there 661.  A batch behind
+// a long prompt has both: 64 sequences behind 32k tokens 104 us, 32 with 64 query and
+// 8 KV heads behind 128k 216 us.  Little work: latency, about 10 us for the first
+// loads, one tile, the join of the waves and the output.
 constexpr int kWaves = 8;
 // Above this a row's reference in log2 units is subtracted from the scores before
 // they are scaled: fma(score, scale, -round(m * scale)) is off by half an ulp of
