@@ -269,6 +269,13 @@ __device__ __forceinline__ void wait_loads() {
 // tiles (a quarter more vector work); probabilities up to 2^8 round as well as
 // those up to 1.
 constexpr float kHeadroom = 8.0f;
+// Probabilities are held 2^kLift times as large, a factor common to a row's sum and
+// mass in every wave and part.  bf16 has float32's exponents.  f16 ends at 2^-24:
+// held as they are, probabilities below 2^-25 of the reference would be lost, 0.4 %
+// of a row with 131 thousand of them.  Lifted to the type's upper end (2^7 and the
+// headroom: 2^15), the limit is 2^-32, and n tokens lose at most n of it.
+template <bool BF16>
+constexpr float kLift = BF16 ? 0.0f : 7.0f;
 
 template <bool BF16>
 __device__ __forceinline__ uint2 pack4(float a, float b, float c, float d) {
@@ -478,13 +485,13 @@ __device__ __forceinline__ void softmax(f32x16 (&s)[KB], u32x4 (&p)[2 * KB], int
     if (up) st.grows = m + kHeadroom / scale_log2;
     st.exact = __any(fabsf(st.mc) > kExactMax);
   }
-  float mc = st.mc;
+  float mc = st.mc - kLift<BF16>;
   if (st.exact) {
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[kb][e] -= st.m;
-    mc = 0.0f;
+    mc = -kLift<BF16>;
   }
 #pragma unroll
   for (int kc = 0; kc < 2 * KB; ++kc) {
