@@ -407,6 +407,7 @@ typedef struct santa_paged_plan_info {
   int heads, kv_heads;
   long long records; /* parts: rows of the workspace */
   long long ints, pos_at, merge_at, parts_at, list_at; /* ints of the plan, and where its sections start */
+  int rounded; /* how probabilities enter the second product; the caller's to change (santa_paged_attention) */
 } santa_paged_plan_info;
 int santa_paged_plan(const int* lens, const int* new_tokens, const int* rows, int B, const int* group,
                      const int* shared, int n_groups, int heads, int kv_heads, int fixed, santa_paged_plan_info* info,
@@ -420,9 +421,12 @@ int santa_paged_plan(const int* lens, const int* new_tokens, const int* rows, in
  * of 8, the last dimension contiguous, the tensors 16-byte aligned).  plan: the
  * device copy of a plan with this info.  scale: positive and finite.  Page
  * numbers are clamped to the pool.
- * Scores, softmax and sums in float32; the probabilities enter the second
- * product rounded to the 16-bit type or, where at most 16 rows share a pass
- * over a KV head's tokens, as the sum of two such values.  workspace:
+ * Scores, softmax and sums in float32.  The probabilities enter the second
+ * product as the sum of two values of the 16-bit type, with a product each, or,
+ * where info->rounded is set and more than 16 rows share a pass over a KV head's
+ * tokens, rounded to one.  A plan sets rounded where a sequence has several new
+ * tokens and more than 32 rows (tokens x query heads per KV head); a copy of info
+ * with another value may be given to any call.  workspace:
  * santa_paged_workspace_size(info, D) bytes, 16-byte aligned, no initialization
  * needed. */
 size_t santa_paged_workspace_size(const santa_paged_plan_info* info, int D);

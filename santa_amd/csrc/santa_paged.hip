@@ -209,6 +209,13 @@ __global__ __launch_bounds__(256) void rope_append_kernel(const uint16_t* __rest
 // 8 of them an XCD's L2 holds one head (16 unshared sequences: 280 us, against
 // 294 with whole sequences side by side).
 //
+// The probabilities are rounded to the 16-bit type for the second product in
+// batches with several new tokens and more than 32 rows per sequence (a prefill),
+// as the prefill over contiguous caches does.  Elsewhere they enter it as two
+// values of that type, with a product each, so that a decode step has the values of
+// float32 probabilities, however many sequences read the same pages: free up to
+// 32 rows, up to a third more time above (both sides in santa_paged_plan.cpp).
+//
 // What bounds it, at D 128 in bf16.  Few rows: HBM, 5.6 TB/s over 16-token pages
 // (16 sequences of 1000 to 40 000 tokens, 32 query and 8 KV heads, 1.55 GB:
 // 277 us; half the ring, or two workgroups of half the waves per compute unit,
@@ -220,8 +227,8 @@ __global__ __launch_bounds__(256) void rope_append_kernel(const uint16_t* __rest
 // waves of a SIMD half a tile apart, products of one beside the softmax of the
 // other, 685; loads issued between the products 711; steps without bookkeeping
 // 667; first products as soon as their first operand is there 661.  A batch behind
-// a long prompt has both: 64 sequences behind 32k tokens 104 us, 32 with 64 query and
-// 8 KV heads behind 128k 216 us.  Little work: latency, about 10 us for the first
+// a long prompt has both: 64 sequences behind 32k tokens 115 us, 32 with 64 query and
+// 8 KV heads behind 128k 267 us (106 and 215 with rounded probabilities).  Little work: latency, about 10 us for the first
 // loads, one tile, the join of the waves and the output.
 constexpr int kWaves = 8;
 // Above this a row's reference in log2 units is subtracted from the scores before
@@ -411,6 +418,44 @@ __device__ __forceinline__ void load_tile(const Loader& w, Cursor& c, uint32_t s
   else if ((c.t & 63) == 0) look_up(w, c);
 }
 
+// How probabilities enter the second product.
+enum class Parts {
+  kOne,    // rounded to the 16-bit type
+  kTwo,    // as the sum of two 16-bit values, each with a product of its own
+  kLanes,  // likewise, the second values in lanes that up to 16 rows leave free
+  kLanesOfTwo,  // likewise, in a kernel whose other items are kTwo
+};
+
+// Probabilities of kTwo are 1 + kMore times as large (cut8); those of kLanesOfTwo,
+// whose sums are joined with theirs, have the factor in their exponent.
+template <bool BF16>
+constexpr float kMore = BF16 ? 0x1p-20f : 0x1p-10f;
+template <bool BF16>
+constexpr float kMoreLog2 = BF16 ? 1.3758605e-6f : 1.4081944e-3f;  // log2(1 + kMore)
+
+// e cut off to the 16-bit type, and in low what that leaves of e (1 + kMore), as
+// 16-bit values.  low has the sign of e and is not 0 where e is not (in f16, where
+// e is a normal number): an infinite value of a token keeps its sign in both
+// products, where the remainder of a rounding, of either sign or 0, would make it
+// NaN.  The factor is common to sum and mass.
+template <bool BF16>
+__device__ __forceinline__ u32x4 cut8(const float (&e)[8], u32x4& low) {
+  u32x4 p;
+  float rest[8];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (BF16) {
+      p[j] = __builtin_amdgcn_perm(__float_as_uint(e[2 * j + 1]), __float_as_uint(e[2 * j]), 0x07060302);
+    } else {
+      p[j] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(e[2 * j], e[2 * j + 1]));
+    }
+    rest[2 * j] = fmaf(e[2 * j], 1.0f + kMore<BF16>, -lo16_to_f32<BF16>(p[j]));
+    rest[2 * j + 1] = fmaf(e[2 * j + 1], 1.0f + kMore<BF16>, -hi16_to_f32<BF16>(p[j]));
+  }
+  low = pack8<BF16>(rest);
+  return p;
+}
+
 // Running softmax of a wave's rows (one per lane of each half): the sum of MB x
 // 32 dims and the mass of this half's tokens, relative to m, a score that the
 // row's largest exceeds by less than kHeadroom (log2 units).  mc: m in log2
@@ -452,10 +497,10 @@ __device__ __forceinline__ void scores(const char* buf, const u32x4 (&qf)[D / 16
 }
 
 // Their softmax: P^T in the 16-bit type, the running state moved on.  kMasked:
-// the lane's row attends to the first lim + 1 of the tokens.  dup: up to 16 rows.
-template <bool BF16, int KB, int MB, bool kMasked>
-__device__ __forceinline__ void softmax(f32x16 (&s)[KB], u32x4 (&p)[2 * KB], int lim, bool dup, float scale_log2,
-                                        State<MB>& st) {
+// the lane's row attends to the first lim + 1 of the tokens.
+template <bool BF16, int KB, int MB, bool kMasked, Parts kParts>
+__device__ __forceinline__ void softmax(f32x16 (&s)[KB], u32x4 (&p)[2 * KB], u32x4 (&low)[2 * KB], int lim,
+                                        float scale_log2, State<MB>& st) {
   const int lane = threadIdx.x & 63;
   if constexpr (kMasked) {
     const int left = lim - 4 * (lane >> 5);
@@ -485,30 +530,37 @@ __device__ __forceinline__ void softmax(f32x16 (&s)[KB], u32x4 (&p)[2 * KB], int
     if (up) st.grows = m + kHeadroom / scale_log2;
     st.exact = __any(fabsf(st.mc) > kExactMax);
   }
-  float mc = st.mc - kLift<BF16>;
+  constexpr bool kLanes = kParts == Parts::kLanes || kParts == Parts::kLanesOfTwo;
+  constexpr float kUp = kLift<BF16> + (kParts == Parts::kLanesOfTwo ? kMoreLog2<BF16> : 0.0f);
+  float mc = st.mc - kUp;
   if (st.exact) {
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
       for (int e = 0; e < 16; ++e) s[kb][e] -= st.m;
-    mc = -kLift<BF16>;
+    mc = -kUp;
   }
 #pragma unroll
   for (int kc = 0; kc < 2 * KB; ++kc) {
     float e[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) e[j] = __builtin_amdgcn_exp2f(fmaf(s[kc >> 1][8 * (kc & 1) + j], scale_log2, -mc));
-    p[kc] = pack8<BF16>(e);
+    if constexpr (kParts == Parts::kTwo) {
+      p[kc] = cut8<BF16>(e, low[kc]);
+      st.l = sum8<BF16>(low[kc], st.l);
+    } else {
+      p[kc] = pack8<BF16>(e);
+    }
     // up to 16 rows leave lanes 16 .. 31 of the wave free: they hold the same
     // rows again, and carry what rounding took from their probabilities
-    if (dup) {
+    if constexpr (kLanes) {
 #pragma unroll
       for (int j = 0; j < 8; j += 2) {
         e[j] -= lo16_to_f32<BF16>(p[kc][j >> 1]);
         e[j + 1] -= hi16_to_f32<BF16>(p[kc][j >> 1]);
       }
-      const u32x4 low = pack8<BF16>(e);
-      if (lane & 16) p[kc] = low;
+      const u32x4 rest = pack8<BF16>(e);
+      if (lane & 16) p[kc] = rest;
     }
     // the mass of the probabilities as rounded: a row's weights sum to 1, and one
     // that attends to one token gives its value
@@ -518,27 +570,33 @@ __device__ __forceinline__ void softmax(f32x16 (&s)[KB], u32x4 (&p)[2 * KB], int
 
 // O^T += V^T P^T over MB x 32 dims; the reads of V run ahead of the products as
 // those of K do.
-template <bool BF16, int D, int KB, int MB>
-__device__ __forceinline__ void sums(const char* buf, uint32_t vo, const u32x4 (&p)[2 * KB], State<MB>& st) {
+template <bool BF16, int D, int KB, int MB, Parts kParts>
+__device__ __forceinline__ void sums(const char* buf, uint32_t vo, const u32x4 (&p)[2 * KB],
+                                     const u32x4 (&low)[2 * KB], State<MB>& st) {
   asm volatile("" : "+v"(vo));
   using G = Geometry<D>;
-  constexpr int N = 2 * KB * MB, kAhead = N < 4 ? N : 4;
+  constexpr int N = 2 * KB * MB, kAhead = N < 4 ? N : 4, kProducts = kParts == Parts::kTwo ? 2 : 1;
   u32x4 v[2 * KB][MB];
 #pragma unroll
   for (int kc = 0; kc < 2 * KB; ++kc)
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) v[kc][mb] = read_tr8<G::kRow>(buf + (vo ^ (64 * mb)) + 16 * G::kRow * kc);
 #pragma unroll
-  for (int kc = 0; kc < 2 * KB; ++kc)
+  for (int kc = 0; kc < 2 * KB; ++kc) {
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) st.o[mb] = mfma32<BF16>(v[kc][mb], p[kc], st.o[mb]);
+    if constexpr (kParts == Parts::kTwo) {
+#pragma unroll
+      for (int mb = 0; mb < MB; ++mb) st.o[mb] = mfma32<BF16>(v[kc][mb], low[kc], st.o[mb]);
+    }
+  }
   __builtin_amdgcn_sched_group_barrier(0x100, 2 * kAhead, 0);  // LDS reads
 #pragma unroll
   for (int i = 0; i < N - kAhead; ++i) {
-    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // matrix products
+    __builtin_amdgcn_sched_group_barrier(0x008, kProducts, 0);  // matrix products
     __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);
   }
-  __builtin_amdgcn_sched_group_barrier(0x008, kAhead, 0);
+  __builtin_amdgcn_sched_group_barrier(0x008, kProducts * kAhead, 0);
 }
 
 // Whether 32 KB rows of a V tile hold an infinity or a NaN.
@@ -559,9 +617,10 @@ __device__ __forceinline__ bool not_finite(const char* rows) {
 // value there is not finite (apart), and would not vanish with a probability of
 // 0: for one last token after the other, the values behind it left out, and the
 // result kept by the rows that end there.
-template <bool BF16, int D, int KB, int MB>
-__device__ __forceinline__ void sums_masked(const char* buf, uint32_t vo, const u32x4 (&p)[2 * KB], int n0,
-                                            int last, int lim, int lim_lo, int lim_hi, bool apart, State<MB>& st) {
+template <bool BF16, int D, int KB, int MB, Parts kParts>
+__device__ __forceinline__ void sums_masked(const char* buf, uint32_t vo, const u32x4 (&p)[2 * KB],
+                                            const u32x4 (&low)[2 * KB], int n0, int last, int lim, int lim_lo,
+                                            int lim_hi, bool apart, State<MB>& st) {
   using G = Geometry<D>;
   const int most = apart ? min(lim_hi, last) : last;
   for (int end = apart ? max(lim_lo, n0) : last; end <= most; ++end) {
@@ -573,7 +632,10 @@ __device__ __forceinline__ void sums_masked(const char* buf, uint32_t vo, const 
       for (int kc = 0; kc < 2 * KB; ++kc) v[kc] = read_tr8<G::kRow>(buf + (vo ^ (64 * mb)) + 16 * G::kRow * kc);
       if (!apart) {
 #pragma unroll
-        for (int kc = 0; kc < 2 * KB; ++kc) st.o[mb] = mfma32<BF16>(v[kc], p[kc], st.o[mb]);
+        for (int kc = 0; kc < 2 * KB; ++kc) {
+          st.o[mb] = mfma32<BF16>(v[kc], p[kc], st.o[mb]);
+          if constexpr (kParts == Parts::kTwo) st.o[mb] = mfma32<BF16>(v[kc], low[kc], st.o[mb]);
+        }
       } else {
         f32x16 o = st.o[mb];
 #pragma unroll
@@ -584,6 +646,7 @@ __device__ __forceinline__ void sums_masked(const char* buf, uint32_t vo, const 
             v[kc][j] = n < left ? v[kc][j] : n == left ? v[kc][j] & 0xffff : 0;
           }
           o = mfma32<BF16>(v[kc], p[kc], o);
+          if constexpr (kParts == Parts::kTwo) o = mfma32<BF16>(v[kc], low[kc], o);
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e) st.o[mb][e] = min(lim, last) == end ? o[e] : st.o[mb][e];
@@ -613,7 +676,7 @@ struct Shares {
 // tile, its latency, not HBM, would bound the pass).  tile: the number of the
 // item's first tile, loaded: that of the next one to be loaded, counted over the
 // workgroup's items.
-template <bool BF16, int D, int RG>
+template <bool BF16, int D, int RG, Parts kParts>
 __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv, const Loader& w, Cursor& cur,
                                        const uint32_t (&lk)[2], const uint32_t (&lv)[2], uint32_t& tile,
                                        uint32_t& loaded, u32x4* stages, Shares* x) {
@@ -630,7 +693,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv
   const int wave = w.wave;
   const int dh = DH == 1 ? 0 : wave & 1, tg = wave / DH % TG, rg = wave / (DH * TG);
   const int kh = TG == 1 ? 0 : tg & 1;                      // half of a tile
-  const bool dup = RG == 1 && it.rows <= 16;
+  constexpr bool dup = kParts == Parts::kLanes || kParts == Parts::kLanesOfTwo;
 
   // this lane's row
   const int r = dup ? ql & 15 : 32 * rg + ql;
@@ -693,25 +756,25 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv
   for (; t + mine < whole; t += kStep) {
     const char* stage = enter(t);
     f32x16 s[KB];
-    u32x4 p[2 * KB];
+    u32x4 p[2 * KB], low[2 * KB];
     scores<BF16, D, KB>(stage, qf, ko, s);
-    softmax<BF16, KB, MB, false>(s, p, 0, dup, a.scale_log2, st);
-    sums<BF16, D, KB, MB>(stage, vo, p, st);
+    softmax<BF16, KB, MB, false, kParts>(s, p, low, 0, a.scale_log2, st);
+    sums<BF16, D, KB, MB, kParts>(stage, vo, p, low, st);
   }
   for (; t < nt; t += kStep) {  // a loop of its own, or both would run short of registers
     const char* stage = enter(t);
     if (t + mine >= busy) continue;
     f32x16 s[KB];
-    u32x4 p[2 * KB];
+    u32x4 p[2 * KB], low[2 * KB];
     const int n0 = first + (t + mine) * kTile, last = min(it.end, n0 + 32 * KB) - 1;
     scores<BF16, D, KB>(stage, qf, ko, s);
-    softmax<BF16, KB, MB, true>(s, p, lim - n0, dup, a.scale_log2, st);
+    softmax<BF16, KB, MB, true, kParts>(s, p, low, lim - n0, a.scale_log2, st);
     const bool apart = last > lim_lo && not_finite<BF16, D, KB>(stage + 16 * G::kVecs + 32 * kh * G::kRow);
-    sums_masked<BF16, D, KB, MB>(stage, vo, p, n0, last, lim, lim_lo, lim_hi, apart, st);
+    sums_masked<BF16, D, KB, MB, kParts>(stage, vo, p, low, n0, last, lim, lim_lo, lim_hi, apart, st);
   }
   float m = st.m, l = st.l + other_half(st.l);
   f32x16(&o)[MB] = st.o;
-  if (dup) {  // an infinite value is whole in the first part, and times 0 or less in the second
+  if constexpr (dup) {  // an infinite value is whole in the first part, and times 0 or less in the second
     l += fxor<16>(l, lane);
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
@@ -811,11 +874,12 @@ __device__ __forceinline__ Item read_item(const Loader& w, int i) {
   return it;
 }
 
-template <bool BF16, int D>
+template <bool BF16, int D, Parts kParts>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_attention_kernel(AttnArgs a) {
   using G = Geometry<D>;
   __shared__ u32x4 stages[G::kStages * G::kStage];
   __shared__ Shares shares;
+  constexpr Parts kLanes = kParts == Parts::kTwo ? Parts::kLanesOfTwo : Parts::kLanes;
   const int kv = blockIdx.x % a.KVH, group = blockIdx.x / a.KVH;
   const int lane = threadIdx.x & 63;
   Loader w;
@@ -853,10 +917,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_attention_kernel(AttnArg
     const Item now = it;
     last = now.next < 0;
     if (!last) it = read_item(w, now.next);  // while this one is worked on
-    if (now.rows <= 32) attend<BF16, D, 1>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares);
-    else if (now.rows <= 64) attend<BF16, D, 2>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares);
-    else if (now.rows <= 128) attend<BF16, D, 4>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares);
-    else attend<BF16, D, 8>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares);
+    if (now.rows <= 16) attend<BF16, D, 1, kLanes>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares);
+    else if (now.rows <= 32) attend<BF16, D, 1, kParts>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares);
+    else if (now.rows <= 64) attend<BF16, D, 2, kParts>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares);
+    else if (now.rows <= 128) attend<BF16, D, 4, kParts>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares);
+    else attend<BF16, D, 8, kParts>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares);
   }
 }
 
@@ -1117,9 +1182,13 @@ extern "C" int santa_paged_attention(const void* q, const void* k_pages, const v
   auto run = [&](auto bf, auto dim) {
     constexpr bool BF16 = decltype(bf)::value;
     constexpr int kD = decltype(dim)::value;
-    if (info->groups > 0)  // one resident round
-      hipLaunchKernelGGL((paged_attention_kernel<BF16, kD>), dim3(static_cast<unsigned>(info->groups) * KVH),
-                         dim3(64 * kWaves), 0, stream, a);
+    auto attend = [&](auto kernel) {  // one resident round
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(info->groups) * KVH), dim3(64 * kWaves), 0, stream, a);
+    };
+    if (info->groups > 0) {
+      if (info->rounded) attend(paged_attention_kernel<BF16, kD, Parts::kOne>);
+      else attend(paged_attention_kernel<BF16, kD, Parts::kTwo>);
+    }
     const long long rows = static_cast<long long>(info->merge_tokens) * H;
     // a workgroup per row up to one resident round of them (2048 rows of 14 parts
     // 6.6 us, against 7.6 with a team each, and of 24 parts 8.9 against 11.4); above

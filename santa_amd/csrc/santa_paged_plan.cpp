@@ -30,10 +30,20 @@ struct Block {
 // What a tile costs a workgroup, by the rows of its block, and what a piece does
 // besides (its first loads, its output), in units of about 0.25 us.  With 64 or
 // fewer rows a tile takes as long as its 32 KiB do from HBM, with 256 as long as
-// its products.  All tiles alike and a piece like one: 122 us for 64 sequences
-// behind 32k tokens and 232 for 32 behind 128k (113 and 219 with these).
+// its products, a third more with probabilities in two parts.  All tiles alike and
+// a piece like one: 122 us for 64 sequences behind 32k tokens and 232 for 32 behind
+// 128k (113 and 219 with these, both rounded); in two parts 115 and 267, and with
+// the costs of rounded ones 121 and 272.
 constexpr int kPieceCost = 20;
-int tile_cost(int rows) { return rows > 128 ? 10 : rows > 64 ? 7 : 6; }
+int tile_cost(int rows, bool rounded) { return rows > 128 ? (rounded ? 10 : 13) : rows > 64 ? 7 : 6; }
+// Whether a sequence's new tokens have the batch's probabilities rounded for the
+// second product (santa_paged_plan_info.rounded, the default): several tokens, as
+// in a prefill, whose second products would cost more than they do behind HBM.
+// 8 sequences of 3000 to 16000 tokens, GH 4, D 128, rounded and in two parts: 8
+// tokens (32 rows) 76.8 and 77.5 us, 9 77.6 and 84.2, 32 90.9 and 102.9; a prefill
+// of 1300 tokens 313 and 410.  A single token is never rounded: what it attends to
+// must not depend on how many others read the same pages.
+bool rounds(int new_tokens, int GH) { return new_tokens > 1 && static_cast<long long>(new_tokens) * GH > 32; }
 // The fewest tiles that a block is cut off after.
 constexpr int kLeastCut = 2;
 
@@ -77,6 +87,7 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
     if (tokens > (1 << 26) / GH) return set_error(SANTA_ERR_INVALID, "too many new tokens");
     info->max_len = std::max(info->max_len, n);
     info->max_row = std::max(info->max_row, row);
+    if (rounds(t, GH)) info->rounded = 1;
     const int g = in.group ? in.group[b] : -1;
     if (g < 0) continue;
     if (g >= in.n_groups) return set_error(SANTA_ERR_INVALID, "sequence %d names group %d of %d", b, g, in.n_groups);
@@ -136,7 +147,7 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
     int slot = 0;
     long long left = budget;
     for (size_t i = 0; i < blocks.size(); ++i) {
-      const int tiles = blocks[i].tiles(), cost = tile_cost(blocks[i].ntok * GH);
+      const int tiles = blocks[i].tiles(), cost = tile_cost(blocks[i].ntok * GH, info->rounded);
       for (int t = 0; t < tiles || t == 0;) {
         long long k = std::min<long long>(tiles - t, (left - kPieceCost) / cost);
         if (left < budget && (k < 1 ? tiles > 0 || left < kPieceCost : k < tiles - t && k < kLeastCut)) {
@@ -153,8 +164,8 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
     return true;
   };
   long long total = 0;
-  for (const Block& k : blocks) total += kPieceCost + static_cast<long long>(tile_cost(k.ntok * GH)) * k.tiles();
-  long long lo = std::max<long long>(total / slots, kPieceCost + tile_cost(1) * kLeastCut), hi = lo;
+  for (const Block& k : blocks) total += kPieceCost + static_cast<long long>(tile_cost(k.ntok * GH, info->rounded)) * k.tiles();
+  long long lo = std::max<long long>(total / slots, kPieceCost + tile_cost(1, true) * kLeastCut), hi = lo;
   while (!pack(hi, false)) lo = hi + 1, hi += std::max(1LL, hi / 4);
   while (lo < hi) {
     const long long mid = lo + (hi - lo) / 2;

@@ -45,7 +45,8 @@ _IP = ctypes.POINTER(ctypes.c_int)
 class _PlanInfo(ctypes.Structure):
     _fields_ = ([(n, _I) for n in ("tokens", "groups", "items", "merge_tokens", "max_len", "max_row", "heads",
                                    "kv_heads")]
-                + [(n, _L) for n in ("records", "ints", "pos_at", "merge_at", "parts_at", "list_at")])
+                + [(n, _L) for n in ("records", "ints", "pos_at", "merge_at", "parts_at", "list_at")]
+                + [("rounded", _I)])
 
 
 _lib_ready = None
@@ -599,7 +600,8 @@ def _attention_expressions(q, k_pages, v_pages, block_table, plan: PagedPlan, sc
 
 
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
-                    plan: Union[PagedPlan, Sequence[int]], *, scale: Optional[float] = None) -> torch.Tensor:
+                    plan: Union[PagedPlan, Sequence[int]], *, scale: Optional[float] = None,
+                    rounded: Optional[bool] = None) -> torch.Tensor:
     """Exact attention of a batch's tokens over paged caches: q [tokens, H, D]
     (the tokens of the plan, sequence after sequence), k_pages and v_pages
     [num_pages, page_size, KVH, D] which hold the tokens themselves already,
@@ -610,10 +612,15 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 
     bf16 and f16 of head_dim 64 and 128 on a GPU run as one kernel over all
     sequences (and one that joins parts, where the tokens of a sequence are
-    split): float32 scores, softmax and sums; the probabilities are rounded to
-    the 16-bit type for the second product or, where at most 16 query rows pass
-    over a KV head's tokens together, split into two such values.  Prefixes of
-    the plan are read once for all their members."""
+    split).  Prefixes of the plan are read once for all their members.  Scores,
+    softmax and sums are float32.  rounded: whether the probabilities are
+    rounded to the 16-bit type for the second product (as in a prefill), or
+    enter it as the sum of two such values, which gives the values of float32
+    probabilities and takes up to a third longer where many rows read the same
+    tokens.  By default they are rounded where a sequence has several new
+    tokens, and more than 32 rows of them (tokens x query heads per KV head);
+    up to 16 rows that pass over a KV head's tokens together are not rounded
+    either way.  The expressions for other calls never round them."""
     if q.dim() != 3:
         raise ValueError(f"q must be [tokens, H, D]; got {tuple(q.shape)}")
     N, H, D = q.shape
@@ -641,7 +648,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         sq = _strides(q, "q")
     strides = (_L * 8)(*sq, *_strides(k_pages, "k_pages"), *_strides(v_pages, "v_pages"))
     table, row = _table_rows(block_table)
-    info = ctypes.byref(plan._info)
+    info = plan._info
+    if rounded is not None and bool(info.rounded) != rounded:
+        info = _PlanInfo.from_buffer_copy(info)
+        info.rounded = int(rounded)
+    info = ctypes.byref(info)
     lib = _lib()
     workspace = torch.empty(lib.santa_paged_workspace_size(info, D), dtype=torch.uint8, device=device)
     _launch(device, lib.santa_paged_attention, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(),
