@@ -356,7 +356,7 @@ int santa_rt_exact_decode(const void* q, const void* k, const void* v, void* out
  * _length: tokens of a sequence (-1: no such sequence); _used: pages in use;
  * _row: a sequence's pages, returns how many.
  * _shared: groups of the sequences seqs whose first tokens lie in the same pages,
- * the last own[i] tokens of each apart: group[i] is a group or -1, shared[g] the
+ * the last own[i] >= 0 tokens of each apart: group[i] is a group or -1, shared[g] the
  * tokens that group g has in common (shared: room for n / 2). */
 typedef struct santa_pages santa_pages;
 int santa_pages_create(int num_pages, int page_size, int max_seqs, int row_pages, santa_pages** out);

@@ -368,8 +368,10 @@ extern "C" int santa_pages_shared(const santa_pages* p, const int* seqs, const i
   if (!p || n < 0 || (n > 0 && (!seqs || !own || !group || !shared)) || !n_groups)
     return set_error(SANTA_ERR_INVALID, "bad santa_pages_shared arguments");
   return guarded([&] {
-    for (int i = 0; i < n; ++i)
+    for (int i = 0; i < n; ++i) {
       if (!p->alive(seqs[i])) return set_error(SANTA_ERR_INVALID, "no sequence %d in the cache", seqs[i]);
+      if (own[i] < 0) return set_error(SANTA_ERR_INVALID, "a sequence has 0 or more new tokens; got %d", own[i]);
+    }
     *n_groups = 0;
     // whole pages before the sequence's own tokens
     std::vector<int> limit(static_cast<size_t>(n)), common(static_cast<size_t>(n));

@@ -423,6 +423,17 @@ def test_shared_prefixes_found():
     assert cache.plan(e, heads=2, new_tokens=0).prefixes == []
 
 
+def test_plan_refuses_negative_new_tokens():
+    """Refused before a page is looked up behind a sequence's end."""
+    cache = _cache()
+    empty, (a,) = cache.add([0, 0]), cache.add([40])
+    forks = [a, *cache.fork(a, 3)]
+    for seqs, new in ((empty, -16), (forks, -1), (forks, [1, 1, 1, -1000000000]), (forks, -(1 << 31))):
+        with pytest.raises(RuntimeError, match="0 or more new tokens"):
+            cache.plan(seqs, 1, new_tokens=new)
+    assert cache.plan(forks, 1, new_tokens=1000).prefixes == []
+
+
 # ------------------------------------------------------------ expressions
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float64])
 def test_expressions(dtype):
