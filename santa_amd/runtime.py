@@ -387,6 +387,7 @@ class ExactDecodeBackend:
     name = "exact_fp32"
     exact_attention = True
     supports_true_batch_decode = True
+    decodes_plans = True  # decode_paged takes a PagedPlan
 
     def decode(self, q_bhd: torch.Tensor, k_nhd: torch.Tensor, v_nhd: torch.Tensor, valid_len: int) -> torch.Tensor:
         B, H, D = q_bhd.shape
@@ -408,12 +409,21 @@ class ExactDecodeBackend:
         """Exact decode over a paged cache, with the arguments of the sampled
         backends' decode_paged: k_pages / v_pages [num_pages, page_size, KVH, D],
         block_table int32 [B, pages per sequence], seq_lens an int or one length
-        per sequence (santa_amd.paged.paged_attention, which also reads shared
-        prefixes once)."""
-        from .paged import paged_attention
+        per sequence (a list or a tensor; one on a GPU is waited for).  These are
+        planned anew in every call, each sequence by itself.  A
+        santa_amd.paged.PagedPlan for seq_lens, whose rows are those of
+        block_table, serves all layers of a step, reads shared prefixes once and
+        can be captured."""
+        from .paged import PagedPlan, paged_attention
 
-        lens = [seq_lens] * q_bhd.shape[0] if isinstance(seq_lens, int) else seq_lens
-        return paged_attention(q_bhd, k_pages, v_pages, block_table, lens)
+        plan = seq_lens
+        if isinstance(plan, int):
+            plan = [plan] * q_bhd.shape[0]
+        elif isinstance(plan, torch.Tensor):
+            plan = plan.cpu()
+        if not isinstance(plan, PagedPlan):
+            plan = PagedPlan(plan, heads=q_bhd.shape[1], kv_heads=k_pages.shape[2], device=q_bhd.device)
+        return paged_attention(q_bhd, k_pages, v_pages, block_table, plan, rounded=False)
 
     def info(self) -> Dict[str, object]:
         return {"backend": self.name, "exact_attention": True, "supports_true_batch_decode": True}
@@ -624,7 +634,8 @@ class RandomLlama:
         the tokens' K and V into their pages and returns the logits of each
         sequence's last token [len(seqs), V] (float32, as prefill's).  Attention
         is exact, tokens that sequences hold in the same pages being read once;
-        or, for one new token each, that of a backend with decode_paged."""
+        or, for one new token each, that of a backend with decode_paged (given the
+        step's plan where its decodes_plans is set)."""
         from .paged import paged_attention, rope_append
 
         s, D = self.shape, self.shape.head_dim
@@ -646,13 +657,16 @@ class RandomLlama:
         cache.extend(seqs, new)
         plan = cache.plan(seqs, s.heads, new)
         cos, sin = _rope_cos_sin(plan.positions, D, s.rope_theta, self.dtype)  # [N, D]
-        table, tables = cache.block_table, None
-        if backend is not None:
+        table = cache.block_table
+        planned = getattr(backend, "decodes_plans", False)
+        if backend is not None and not planned:
             tables = cache.tables(seqs).contiguous()
 
         def attend(li, qkv):
             q = rope_append(qkv.view(len(qkv), -1, D), cos, sin, cache.k[li], cache.v[li], table, plan)
-            if backend is not None:
+            if planned:
+                a = backend.decode_paged(q, cache.k[li], cache.v[li], table, plan)
+            elif backend is not None:
                 a = backend.decode_paged(q, cache.k[li], cache.v[li], tables, plan.seq_lens)
             else:
                 a = paged_attention(q, cache.k[li], cache.v[li], table, plan)

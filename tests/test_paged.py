@@ -685,3 +685,27 @@ def test_backend_decodes_pages():
         assert torch.equal(ExactDecodeBackend().decode_paged(q, k, v, table, x), want)
     same = ExactDecodeBackend().decode_paged(q, k, v, table, 9)
     assert torch.equal(same, paged_attention(q, k, v, table, [9, 9, 9]))
+
+
+def test_backend_decodes_a_plan(monkeypatch):
+    """One plan for all layers, with prefixes and rows of a whole block table;
+    RandomLlama.extend hands its own over."""
+    lens, shared = [70, 66, 90], [([0, 2], 64)]
+    k, v, table = _shared_pools(lens, shared, 8, 2, 32, 3, dtype=torch.float32)
+    q = torch.randn(3, 4, 32, generator=torch.Generator().manual_seed(1))
+    wide = torch.full((6, table.shape[1]), 1 << 30, dtype=torch.int32)
+    wide[[4, 1, 5]] = table
+    plan = PagedPlan(lens, heads=4, kv_heads=2, prefixes=shared, rows=[4, 1, 5], device="cpu")
+    want = ExactDecodeBackend().decode_paged(q, k, v, table, lens)
+    assert torch.equal(ExactDecodeBackend().decode_paged(q, k, v, wide, plan), want)
+    with pytest.raises(ValueError, match="the plan is for 3 tokens"):
+        ExactDecodeBackend().decode_paged(q[:2], k, v, wide, plan)
+    model, cache = RandomLlama(TINY, seed=3, std=0.05, dtype=torch.float32, device="cpu"), _model_cache(TINY)
+    a, = cache.add([0])
+    model.extend(torch.arange(40)[None], cache, [a])
+    made, given = [], []
+    build, decode = PagedPlan.update, ExactDecodeBackend.decode_paged
+    monkeypatch.setattr(PagedPlan, "update", lambda self, *args: made.append(self) or build(self, *args))
+    monkeypatch.setattr(ExactDecodeBackend, "decode_paged", lambda self, *args: given.append(args[4]) or decode(self, *args))
+    model.extend(torch.tensor([5, 6]), cache, [a, *cache.fork(a)], 1, backend=ExactDecodeBackend())
+    assert len(made) == 1 and given == made * TINY.layers and made[0].prefixes == [([0, 1], 40)]

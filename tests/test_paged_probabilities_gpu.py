@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from santa_amd.paged import PagedPlan, paged_attention
+from santa_amd.runtime import ExactDecodeBackend
 from test_shared_pages_gpu import _case, _check, _reference
 
 pytestmark = pytest.mark.gpu
@@ -128,3 +129,28 @@ def test_infinite_values_in_two_parts(H, D, dtype):
     want[:2, :, 1], want[:2, :, 2], want[1, :, 3] = math.inf, -math.inf, math.inf
     want[2, :, 4], want[2, :, 5] = -math.inf, math.inf
     assert torch.equal(paged_attention(q, k, v, table, plan, rounded=False), want)
+
+
+def test_exact_backend():
+    """ExactDecodeBackend.decode_paged: lengths on the GPU, a plan for all layers,
+    the values of float32 probabilities for any number of query heads, and a
+    captured step."""
+    print("\n[case] the exact backend over pages", flush=True)
+    lens, shared = [700, 300, 650], [([0, 2], 640)]
+    q, k, v, table, plan = _case(lens, [1] * 3, shared, 40, 1, 128, 16, BF, 2)
+    backend = ExactDecodeBackend()
+    alone = backend.decode_paged(q, k, v, table, lens)
+    assert _tight(alone, q, k, v, table, lens, [1] * 3) <= 1
+    for x in (torch.tensor(lens), torch.tensor(lens, device="cuda"), torch.tensor(lens, device="cuda").int()):
+        assert torch.equal(backend.decode_paged(q, k, v, table, x), alone)
+    together = backend.decode_paged(q, k, v, table, plan)
+    assert _tight(together, q, k, v, table, lens, [1] * 3) <= 1
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = [backend.decode_paged(q, k, v, table, plan) for _ in range(2)]
+    for _ in range(3):
+        q.normal_()
+        graph.replay()
+        want = backend.decode_paged(q, k, v, table, plan)
+        assert torch.equal(out[0], want) and torch.equal(out[1], want)
