@@ -542,11 +542,18 @@ class RandomLlama:
         s = self.shape
         B, P = h.shape[:2]
         shape = (B, cache.storage, s.kv_heads, s.head_dim)
-        return (h.is_cuda and h.dtype == torch.bfloat16 and P <= cache.storage and B * P > 0 and s.head_dim % 16 == 0
-                and s.intermediate % 8 == 0 and s.hidden % 8 == 0
-                and B * P * (s.heads + 2 * s.kv_heads) * s.head_dim < 1 << 34
+        return (P <= cache.storage and self._fused_layers_take(h)
                 and all(t.shape == shape and t.dtype == h.dtype and t.device == h.device and t.is_contiguous()
-                        and t.data_ptr() % 16 == 0 for t in (*cache.k, *cache.v))
+                        and t.data_ptr() % 16 == 0 for t in (*cache.k, *cache.v)))
+
+    def _fused_layers_take(self, h: torch.Tensor) -> bool:
+        """Whether the elementwise work on h [.., hidden] can run as the
+        library's kernels: a bf16 model on one GPU, laid out as the kernels
+        address it (16-byte rows)."""
+        s = self.shape
+        return (h.is_cuda and h.dtype == torch.bfloat16 and h.numel() > 0 and s.head_dim % 16 == 0
+                and s.intermediate % 8 == 0 and s.hidden % 8 == 0
+                and h.numel() // s.hidden * (s.heads + 2 * s.kv_heads) * s.head_dim < 1 << 34
                 and all(w.dtype == h.dtype and w.is_contiguous() for L in self.layers for w in (L["ln1"], L["ln2"]))
                 and self.norm.dtype == h.dtype and self.norm.is_contiguous() and _plain(h))
 
@@ -653,6 +660,8 @@ class RandomLlama:
             raise ValueError(f"the cache is on {cache.device}, the model on {self.embed.device}")
         if backend is not None and max(new) > 1:
             raise ValueError("a backend decodes one new token per sequence")
+        if mlp_chunk < 1:
+            raise ValueError(f"mlp_chunk must be at least 1; got {mlp_chunk}")
         h = self.embed[tokens.reshape(-1)]  # [N, hidden]
         cache.extend(seqs, new)
         plan = cache.plan(seqs, s.heads, new)
@@ -663,6 +672,7 @@ class RandomLlama:
             tables = cache.tables(seqs).contiguous()
 
         def attend(li, qkv):
+            qkv = qkv.to(self.dtype)  # autocast gives another
             q = rope_append(qkv.view(len(qkv), -1, D), cos, sin, cache.k[li], cache.v[li], table, plan)
             if planned:
                 a = backend.decode_paged(q, cache.k[li], cache.v[li], table, plan)
@@ -672,7 +682,7 @@ class RandomLlama:
                 a = paged_attention(q, cache.k[li], cache.v[li], table, plan)
             return a.reshape(len(q), s.heads * D)
 
-        fused = self.device.type == "cuda" and self.dtype == torch.bfloat16
+        fused = self._fused_layers_take(h)
         if fused:
             lin = _FusedOps.linear
             h = h.contiguous()

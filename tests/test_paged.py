@@ -709,3 +709,13 @@ def test_backend_decodes_a_plan(monkeypatch):
     monkeypatch.setattr(ExactDecodeBackend, "decode_paged", lambda self, *args: given.append(args[4]) or decode(self, *args))
     model.extend(torch.tensor([5, 6]), cache, [a, *cache.fork(a)], 1, backend=ExactDecodeBackend())
     assert len(made) == 1 and given == made * TINY.layers and made[0].prefixes == [([0, 1], 40)]
+
+
+def test_model_refuses_chunks_without_tokens():
+    """A negative chunk would leave the layers' MLPs out."""
+    model, cache = RandomLlama(TINY, device="cpu", dtype=torch.float32, seed=1), _model_cache(TINY)
+    a, = cache.add([0])
+    for chunk in (0, -5):
+        with pytest.raises(ValueError, match="mlp_chunk"):
+            model.extend(torch.zeros(1, 3, dtype=torch.long), cache, [a], mlp_chunk=chunk)
+    assert cache.lengths([a]) == [0]
