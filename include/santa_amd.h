@@ -344,6 +344,8 @@ int santa_rt_exact_decode(const void* q, const void* k, const void* v, void* out
  *   _extend: tokens[i] more tokens for seqs[i] (each named once).  A last page
  *     that is partly filled and held by other sequences too is replaced by a
  *     copy.
+ *   _shrink: the last tokens[i] tokens of seqs[i] (each named once) leave it, and
+ *     it gives up the pages that hold none of those left.
  *   _fork: n new sequences that hold every page of seq.
  *   _free: the sequences end; a page that none holds is free.
  *   _compact: with n pages in use, those numbered n and above move to the
@@ -363,6 +365,7 @@ int santa_pages_create(int num_pages, int page_size, int max_seqs, int row_pages
 void santa_pages_destroy(santa_pages* p);
 int santa_pages_add(santa_pages* p, const int* lengths, int n, int* seqs);
 int santa_pages_extend(santa_pages* p, const int* seqs, const int* tokens, int n);
+int santa_pages_shrink(santa_pages* p, const int* seqs, const int* tokens, int n);
 int santa_pages_fork(santa_pages* p, int seq, int n, int* seqs);
 int santa_pages_free(santa_pages* p, const int* seqs, int n);
 int santa_pages_compact(santa_pages* p);

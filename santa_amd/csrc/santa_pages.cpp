@@ -252,6 +252,24 @@ extern "C" int santa_pages_extend(santa_pages* p, const int* seqs, const int* to
   });
 }
 
+extern "C" int santa_pages_shrink(santa_pages* p, const int* seqs, const int* tokens, int n) {
+  if (!p || (n > 0 && !tokens)) return set_error(SANTA_ERR_INVALID, "bad santa_pages_shrink arguments");
+  p->begin();
+  const int rc = check_seqs(p, seqs, n);
+  if (rc != SANTA_OK) return rc;
+  for (int i = 0; i < n; ++i)
+    if (tokens[i] < 0 || tokens[i] > p->seqs[seqs[i]].len)
+      return set_error(SANTA_ERR_INVALID, "%d tokens cannot leave sequence %d, which holds %d", tokens[i], seqs[i],
+                       p->seqs[seqs[i]].len);
+  for (int i = 0; i < n; ++i) {
+    santa_pages::Seq& s = p->seqs[seqs[i]];
+    s.len -= tokens[i];
+    for (const size_t pages = static_cast<size_t>(p->pages_for(s.len)); s.pages.size() > pages; s.pages.pop_back())
+      p->drop(s.pages.back());
+  }
+  return clear_error();
+}
+
 extern "C" int santa_pages_fork(santa_pages* p, int seq, int n, int* seqs) {
   if (!p || n < 0 || (n > 0 && !seqs)) return set_error(SANTA_ERR_INVALID, "bad santa_pages_fork arguments");
   return guarded([&] {

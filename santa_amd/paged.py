@@ -62,6 +62,7 @@ def _lib():
         L.santa_pages_destroy.restype = None
         L.santa_pages_add.argtypes = [_P, _IP, _I, _IP]
         L.santa_pages_extend.argtypes = [_P, _IP, _IP, _I]
+        L.santa_pages_shrink.argtypes = [_P, _IP, _IP, _I]
         L.santa_pages_fork.argtypes = [_P, _I, _I, _IP]
         L.santa_pages_free.argtypes = [_P, _IP, _I]
         L.santa_pages_compact.argtypes = [_P]
@@ -206,6 +207,11 @@ class PagedKVCache:
         self._may_change()
         _check(_lib().santa_pages_extend(self._pages, _ints(seqs), _ints(tokens), len(seqs)))
         self._apply()
+
+    def _take_back(self, seqs: Sequence[int], tokens: Sequence[int]) -> None:
+        """Those many last tokens, whose K and V were never written, leave the
+        sequences again (a last page that extend() copied stays theirs)."""
+        _check(_lib().santa_pages_shrink(self._pages, _ints(seqs), _ints(tokens), len(seqs)))
 
     def fork(self, seq: int, n: int = 1) -> List[int]:
         """n new sequences with the same tokens, which hold the same pages."""

@@ -642,10 +642,12 @@ class RandomLlama:
         sequence's last token [len(seqs), V] (float32, as prefill's).  Attention
         is exact, tokens that sequences hold in the same pages being read once;
         or, for one new token each, that of a backend with decode_paged (given the
-        step's plan where its decodes_plans is set)."""
-        from .paged import paged_attention, rope_append
+        step's plan where its decodes_plans is set).  A call that fails leaves
+        the sequences with the tokens that they had."""
+        from .paged import _int_list
 
         s, D = self.shape, self.shape.head_dim
+        seqs = _int_list(seqs, "seqs")
         B = len(seqs)
         if new_tokens is None:
             if tokens.dim() != 2 or tokens.shape[0] != B:
@@ -664,6 +666,18 @@ class RandomLlama:
             raise ValueError(f"mlp_chunk must be at least 1; got {mlp_chunk}")
         h = self.embed[tokens.reshape(-1)]  # [N, hidden]
         cache.extend(seqs, new)
+        try:
+            return self._extend(h, cache, seqs, new, backend, mlp_chunk)
+        except BaseException:  # a backend that does not take the model, a GPU without room
+            cache._take_back(seqs, new)
+            raise
+
+    def _extend(self, h: torch.Tensor, cache, seqs: List[int], new: List[int], backend, mlp_chunk: int) -> torch.Tensor:
+        """extend() of embedded tokens h [N, hidden] that the sequences have
+        pages for."""
+        from .paged import paged_attention, rope_append
+
+        s, D = self.shape, self.shape.head_dim
         plan = cache.plan(seqs, s.heads, new)
         cos, sin = _rope_cos_sin(plan.positions, D, s.rope_theta, self.dtype)  # [N, D]
         table = cache.block_table

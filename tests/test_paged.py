@@ -719,3 +719,54 @@ def test_model_refuses_chunks_without_tokens():
         with pytest.raises(ValueError, match="mlp_chunk"):
             model.extend(torch.zeros(1, 3, dtype=torch.long), cache, [a], mlp_chunk=chunk)
     assert cache.lengths([a]) == [0]
+
+
+def test_shrink():
+    """Tokens leave from the end; pages that are left without any are given up,
+    shared ones by one holder; refused for more than there are."""
+    cache = _cache()
+    a, b = cache.add([20, 9])
+    lib, ints = paged._lib(), lambda *x: (ctypes.c_int * len(x))(*x)
+    c, = cache.fork(a)
+    cache.extend([c], 10)  # copies the last page
+    pages, used = cache.pages(c), cache.used_pages
+    cache._take_back([c, b], [10, 0])
+    assert cache.lengths([a, b, c]) == [20, 9, 20] and cache.pages(c) == pages[:3] and cache.used_pages == used - 1
+    cache._take_back([c], [13])
+    assert cache.pages(c) == pages[:1] == cache.pages(a)[:1] and cache.used_pages == used - 2
+    for seqs, tokens, text in (([c], [8], "8 tokens cannot leave"), ([a, b], [1, -1], "-1 tokens cannot leave"),
+                               ([a, a], [1, 1], "named twice"), ([5], [1], "no sequence 5")):
+        with pytest.raises(RuntimeError, match=text):
+            cache._take_back(seqs, tokens)
+    assert lib.santa_pages_shrink(None, ints(0), ints(0), 1) != 0
+    assert lib.santa_pages_shrink(cache._pages, ints(0), None, 1) != 0
+    cache._take_back([a, b, c], [20, 9, 7])
+    assert cache.lengths([a, b, c]) == [0, 0, 0] and cache.used_pages == 0 and cache.compact() == 0
+
+
+def test_model_takes_tokens_back():
+    """A call that fails behind the lengthening leaves every sequence with the
+    tokens that it had, and the next one goes on from there."""
+    model, cache = RandomLlama(TINY, device="cpu", dtype=torch.float32, seed=1), _model_cache(TINY)
+    a, = cache.add([0])
+    first = torch.arange(19)[None]
+    model.extend(first, cache, [a])
+    seqs = [a, *cache.fork(a)]
+
+    class Refuses:
+        def decode_paged(self, *args):
+            raise RuntimeError("This build supports only D=128")
+
+    for backend in (Refuses(), object()):
+        with pytest.raises((RuntimeError, AttributeError)):
+            model.extend(torch.tensor([3, 4]), cache, seqs, 1, backend=backend)
+        assert cache.lengths(seqs) == [19, 19]
+    two = RandomLlama(TINY, device="cpu", dtype=torch.float32, seed=1)
+    two.layers[1]["wo"] = two.layers[1]["wo"][:, :-1]
+    with pytest.raises(RuntimeError):
+        two.extend(torch.arange(40)[None], cache, seqs, [30, 10])
+    assert cache.lengths(seqs) == [19, 19] and cache.used_pages == 4  # the copied last page stays one
+    logits = model.extend(torch.tensor([3, 4]), cache, seqs, 1)
+    for t, x in zip((3, 4), logits):
+        want = model.prefill(torch.cat([first, torch.tensor([[t]])], 1), NHDCache(TINY, 1, 20, torch.float32, "cpu"))[0]
+        assert (x - want).abs().max() < 1e-5
