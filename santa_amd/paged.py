@@ -389,7 +389,7 @@ class PagedPlan:
         self._args = (_ints(self.new_tokens), _ints(self.rows), B, _ints(group),
                       _ints([n for _, n in self.prefixes]), len(self.prefixes))
         self._info = _PlanInfo()
-        self._data = None
+        self._data = self._stream = None
         self.update(lens)
 
     def update(self, seq_lens: Sequence[int]) -> None:
@@ -417,10 +417,19 @@ class PagedPlan:
             host = torch.empty(max(1, info.ints), dtype=torch.int32, pin_memory=cuda)
             _check(build(host.data_ptr(), info.ints))
             if self._data is not None and self._data.shape == host.shape:
+                self._used()
                 self._data.copy_(host, non_blocking=True)
             else:
                 self._data = host.to(self.device, non_blocking=True)
+                if cuda:
+                    self._stream = torch._C._cuda_getCurrentRawStream(self.device.index)
         self._info, self.seq_lens = info, lens
+
+    def _used(self) -> None:
+        """Before a call on the current stream: the plan's memory, where it comes
+        from another stream, is not given out again before the call has ended."""
+        if self._stream is not None and torch._C._cuda_getCurrentRawStream(self.device.index) != self._stream:
+            self._data.record_stream(torch.cuda.current_stream(self.device))
 
     @property
     def tokens(self) -> int:
@@ -548,6 +557,7 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages
         q = qkv.new_empty((plan.tokens, H, D))
         table, row = _table_rows(block_table)
         if plan.tokens:
+            plan._used()
             _launch(device, _lib().santa_paged_rope_append, qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(),
                     q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), int(dtype == torch.float16), D,
                     k_pages.shape[0], k_pages.shape[1], (_L * 6)(*strides), table.data_ptr(), row, table.shape[0],
@@ -661,6 +671,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     info = ctypes.byref(info)
     lib = _lib()
     workspace = torch.empty(lib.santa_paged_workspace_size(info, D), dtype=torch.uint8, device=device)
+    plan._used()
     _launch(device, lib.santa_paged_attention, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(),
             int(q.dtype == torch.float16), D, k_pages.shape[0], k_pages.shape[1], strides, table.data_ptr(), row,
             table.shape[0], info, plan._data.data_ptr(), scale, workspace.data_ptr(), workspace.numel())
