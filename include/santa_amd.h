@@ -397,7 +397,8 @@ int santa_pages_apply(const santa_pages* p, const void* const* pools, int n_pool
  * precede every member's queries; the pages of one of the members are
  * read for all.  fixed != 0: items and the workspace are sized so that any
  * other lengths with the same new_tokens and groups give a plan of the same
- * info (for captured graphs whose plan changes between replays).  info is
+ * info but for max_len (for captured graphs whose plan changes between replays,
+ * up to the lengths that the captured calls' block tables have room for).  info is
  * always written; plan (info->ints ints, 16-byte aligned, to be copied to the
  * device as it is) where it is not NULL.  Workgroups are planned for the current
  * device. */

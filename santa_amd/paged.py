@@ -362,8 +362,11 @@ class PagedPlan:
     The plan is built on the host and copied to the device on the current
     stream.  `update(seq_lens)` makes it that of other lengths of the same
     sequences.  With fixed=True an update keeps the launches and workspaces of
-    every other call the same, so that a captured graph can be replayed after
-    it (at the cost of workgroups without work)."""
+    the kernels' calls the same, so that a captured graph can be replayed after
+    it (at the cost of workgroups without work), up to the lengths that the
+    captured calls' block tables have room for.  A plan that a graph holds in
+    another way is not updated, and one that a graph holds is kept as long as
+    the graph."""
 
     def __init__(self, seq_lens: Sequence[int], *, heads: int, kv_heads: int, new_tokens: Union[int, Sequence[int]] = 1,
                  prefixes: Sequence[Tuple[Sequence[int], int]] = (), rows: Optional[Sequence[int]] = None,
@@ -390,6 +393,7 @@ class PagedPlan:
                       _ints([n for _, n in self.prefixes]), len(self.prefixes))
         self._info = _PlanInfo()
         self._data = self._stream = None
+        self._room = None  # what captured calls have room for
         self.update(lens)
 
     def update(self, seq_lens: Sequence[int]) -> None:
@@ -402,6 +406,12 @@ class PagedPlan:
         cuda = self.device.type == "cuda"
         if cuda and torch.cuda.is_current_stream_capturing():
             raise RuntimeError("a plan cannot be made while a graph is captured: a replay would not make it again")
+        if self._room is not None and max(lens, default=0) > self._room:
+            if self._room < 0:
+                raise RuntimeError("a captured call holds this plan's lengths: only the kernels' calls of a plan with "
+                                   "fixed=True follow an update")
+            raise RuntimeError(f"seq_lens exceeds the block table's capacity in a captured call: {max(lens)} > "
+                               f"{self._room}")
         info = _PlanInfo()
 
         def build(buffer, n):
@@ -424,6 +434,11 @@ class PagedPlan:
                 if cuda:
                     self._stream = torch._C._cuda_getCurrentRawStream(self.device.index)
         self._info, self.seq_lens = info, lens
+
+    def _captured(self, room: int, follows: bool) -> None:
+        """Notes a captured call with a block table for `room` tokens, whose
+        replays follow an update (a kernel's, which reads the plan) or do not."""
+        self._room = min(room if follows and self.fixed else -1, room if self._room is None else self._room)
 
     def _used(self) -> None:
         """Before a call on the current stream: the plan's memory, where it comes
@@ -550,6 +565,8 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages
         raise ValueError("cos and sin must have the device and dtype of qkv")
     if (device.type == "cuda" and dtype in (torch.bfloat16, torch.float16) and D % 16 == 0
             and _plain(qkv, cos, sin, k_pages, v_pages)):
+        if torch.cuda.is_current_stream_capturing():
+            plan._captured(block_table.shape[1] * k_pages.shape[1], True)
         strides = (*_strides(k_pages, "k_pages"), *_strides(v_pages, "v_pages"))
         if _overlaps(k_pages) or _overlaps(v_pages):
             raise ValueError("rows of pages that are written must not overlap")
@@ -563,6 +580,8 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages
                     k_pages.shape[0], k_pages.shape[1], (_L * 6)(*strides), table.data_ptr(), row, table.shape[0],
                     ctypes.byref(plan._info), plan._data.data_ptr())
         return q
+    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        plan._captured(0, False)
     wide = torch.float64 if qkv.dtype == torch.float64 else torch.float32
     x, c, s = qkv[:, :H + KVH].to(wide), cos.to(wide)[:, None], sin.to(wide)[:, None]
     turned = (x * c + torch.cat([-x[..., D // 2:], x[..., :D // 2]], dim=-1) * s).to(qkv.dtype)
@@ -651,8 +670,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if not 1e-37 < scale < 1e37:  # normal in float32, times log2(e) too
         raise ValueError(f"scale must be positive and finite; got {scale}")
     device = q.device
-    if not (device.type == "cuda" and q.dtype in (torch.bfloat16, torch.float16) and D in (64, 128)
-            and _plain(q, k_pages, v_pages)):
+    kernel = (device.type == "cuda" and q.dtype in (torch.bfloat16, torch.float16) and D in (64, 128)
+              and _plain(q, k_pages, v_pages))
+    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        plan._captured(block_table.shape[1] * k_pages.shape[1], kernel)
+    if not kernel:
         return _attention_expressions(q, k_pages, v_pages, block_table, plan, scale)
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if N == 0:

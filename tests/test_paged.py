@@ -770,3 +770,22 @@ def test_model_takes_tokens_back():
     for t, x in zip((3, 4), logits):
         want = model.prefill(torch.cat([first, torch.tensor([[t]])], 1), NHDCache(TINY, 1, 20, torch.float32, "cpu"))[0]
         assert (x - want).abs().max() < 1e-5
+
+
+def test_captured_plans_are_held():
+    """What a captured call has room for bounds later updates; where a replay
+    would not follow an update, there is none."""
+    args = dict(heads=2, kv_heads=1, device="cpu")
+    plan = PagedPlan([20, 30], fixed=True, **args)
+    plan._captured(100, True)
+    plan._captured(80, True)
+    plan.update([80, 1])
+    with pytest.raises(RuntimeError, match="81 > 80"):
+        plan.update([5, 81])
+    assert plan.seq_lens == [80, 1]
+    plan._captured(1000, False)
+    loose = PagedPlan([20, 30], **args)
+    loose._captured(1000, True)
+    for p in (plan, loose):
+        with pytest.raises(RuntimeError, match="a captured call holds"):
+            p.update([5, 5])
