@@ -74,7 +74,6 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
   std::vector<int> first(static_cast<size_t>(in.B));       // first token of each sequence
   std::vector<int> prefix(static_cast<size_t>(in.B), 0);   // tokens read with the group
   std::vector<int> lead(static_cast<size_t>(in.n_groups), -1), members(static_cast<size_t>(in.n_groups), 0);
-  std::vector<long long> group_tokens(static_cast<size_t>(in.n_groups), 0);
   for (int b = 0; b < in.B; ++b) {
     const int n = in.lens[b], t = in.new_tokens[b], row = in.rows ? in.rows[b] : b;
     if (n < 0 || t < 0) return set_error(SANTA_ERR_INVALID, "a sequence has 0 or more tokens and new tokens");
@@ -97,7 +96,6 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
     if (t == 0 || static_cast<long long>(t) * GH >= kBlockRows) continue;  // fills workgroups by itself
     if (lead[g] < 0) lead[g] = row;
     ++members[g];
-    group_tokens[g] += t;
   }
   info->tokens = static_cast<int>(tokens);
 

@@ -392,6 +392,11 @@ class PagedPlan:
         self._args = (_ints(self.new_tokens), _ints(self.rows), B, _ints(group),
                       _ints([n for _, n in self.prefixes]), len(self.prefixes))
         self._info = _PlanInfo()
+        # room for a plan: its items, in whole pieces of 256 rows and a cut for every workgroup, and what it says of
+        # each token; one that is larger is built again
+        tokens, rows = sum(max(0, t) for t in self.new_tokens), max(1, 256 * self.kv_heads // max(1, self.heads))
+        self._size = min(1 << 22, 16 * (B + 2 * (tokens // rows) + len(self.prefixes) + 256 // max(1, self.kv_heads) + 1)
+                         + 12 * tokens + 2)
         self._data = self._stream = None
         self._room = None  # what captured calls have room for
         self.update(lens)
@@ -422,10 +427,14 @@ class PagedPlan:
             return _lib().santa_paged_plan(_ints(lens), new, rows, B, group, shared, groups, self.heads, self.kv_heads,
                                            int(self.fixed), ctypes.byref(info), buffer, n)
 
-        _check(build(None, 0))
         with torch.inference_mode(False):  # updated in any mode
-            host = torch.empty(max(1, info.ints), dtype=torch.int32, pin_memory=cuda)
-            _check(build(host.data_ptr(), info.ints))
+            host = torch.empty(self._size, dtype=torch.int32, pin_memory=cuda)
+            rc = build(host.data_ptr(), self._size)
+            if rc != 0 and info.ints > self._size:
+                host = torch.empty(info.ints, dtype=torch.int32, pin_memory=cuda)
+                rc = build(host.data_ptr(), info.ints)
+            _check(rc)
+            host = host[:max(1, info.ints)]
             if self._data is not None and self._data.shape == host.shape:
                 self._used()
                 self._data.copy_(host, non_blocking=True)

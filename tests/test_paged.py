@@ -789,3 +789,37 @@ def test_captured_plans_are_held():
     for p in (plan, loose):
         with pytest.raises(RuntimeError, match="a captured call holds"):
             p.update([5, 5])
+
+
+def test_plans_are_built_once(monkeypatch):
+    """The buffer is large enough at first, of whatever shape the batch is; one
+    that is not is made again."""
+    lib, calls = paged._lib(), []
+
+    class Counted:
+        def __getattr__(self, name):
+            if name == "santa_paged_plan":
+                return lambda *args: calls.append(args[-1]) or lib.santa_paged_plan(*args)
+            return getattr(lib, name)
+
+    monkeypatch.setattr(paged, "_lib_ready", Counted())
+    r = random.Random(1)
+    for _ in range(60):
+        KVH, GH, B = r.choice((1, 2, 8, 32)), r.choice((1, 4, 7, 16, 40, 128, 255)), r.randint(0, 40)
+        new = [r.choice((0, 1, 1, 5, 300)) for _ in range(B)]
+        lens = [r.choice((0, 1, 100, 5000, 70000)) + 400 for _ in range(B)]
+        order = r.sample(range(B), B)
+        cut = r.randint(0, B)
+        calls.clear()
+        plan = PagedPlan(lens, heads=KVH * GH, kv_heads=KVH, new_tokens=new, device="cpu", fixed=r.random() < 0.5,
+                         prefixes=[(order[:cut], 70), (order[cut:], 64)])
+        plan.update(lens)
+        assert len(calls) == 2 and len(plan._data) == max(1, plan._info.ints)
+    calls.clear()
+    plan = PagedPlan([5, 70], heads=2, kv_heads=2, device="cpu")
+    want = plan._data.clone()
+    plan._size = 3
+    plan.update([5, 70])
+    assert calls[1:] == [3, len(want)] and torch.equal(plan._data, want)
+    with pytest.raises(RuntimeError, match="0 or more"):
+        plan.update([5, -1])
