@@ -144,8 +144,12 @@ int extend(santa_pages* p, const int* seqs, const int* tokens, int n) {
     try {
       p->edits.reserve(static_cast<size_t>(need));
       p->copies.reserve(dropped.size());
-      for (int j = 0; j < n; ++j)
-        p->seqs[seqs[j]].pages.reserve(static_cast<size_t>(p->pages_for(p->seqs[seqs[j]].len + tokens[j])));
+      for (int j = 0; j < n; ++j) {
+        std::vector<int>& pages = p->seqs[seqs[j]].pages;
+        const size_t want = static_cast<size_t>(p->pages_for(p->seqs[seqs[j]].len + tokens[j]));
+        // twice as many as there were, or a sequence that grows by single pages copies its list each time
+        if (want > pages.capacity()) pages.reserve(std::max(want, 2 * pages.capacity()));
+      }
     } catch (const std::bad_alloc&) {
       rc = set_error(SANTA_ERR_INVALID, "out of host memory");
     }

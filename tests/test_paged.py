@@ -823,3 +823,15 @@ def test_plans_are_built_once(monkeypatch):
     assert calls[1:] == [3, len(want)] and torch.equal(plan._data, want)
     with pytest.raises(RuntimeError, match="0 or more"):
         plan.update([5, -1])
+
+
+def test_page_lists_grow_in_steps():
+    """A sequence that gains its pages one by one does not move its list each time."""
+    cache = _cache(pages=1000, page=8, seqs=1, max_len=8000, layers=0)
+    a, = cache.add([0])
+    row, seen = ctypes.POINTER(ctypes.c_int)(), []
+    for i in range(1000):
+        cache.extend([a], 8)
+        assert paged._lib().santa_pages_row(cache._pages, a, ctypes.byref(row)) == i + 1
+        seen.append(ctypes.addressof(row.contents))
+    assert sum(x != y for x, y in zip(seen, seen[1:])) <= 10 and cache.pages(a) == list(range(1000))
