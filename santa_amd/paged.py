@@ -111,7 +111,11 @@ def _int_list(values, what: str) -> List[int]:
         values = values.tolist()
     if isinstance(values, int):
         raise ValueError(f"{what} must be a list")
-    return [int(v) for v in values]
+    values = list(values)
+    ints = [int(v) for v in values]
+    if ints != values:
+        raise ValueError(f"{what} must be whole numbers")
+    return ints
 
 
 def _ints(values: Sequence[int]):
@@ -172,9 +176,10 @@ class PagedKVCache:
         return self.num_pages - self.used_pages
 
     def lengths(self, seqs: Sequence[int]) -> List[int]:
-        out = [_lib().santa_pages_length(self._pages, s) for s in _ints(_int_list(seqs, "seqs"))]
+        seqs = _int_list(seqs, "seqs")
+        out = [_lib().santa_pages_length(self._pages, s) for s in _ints(seqs)]
         if min(out, default=0) < 0:
-            raise RuntimeError(f"no sequence {list(seqs)[out.index(-1)]} in the cache")
+            raise RuntimeError(f"no sequence {seqs[out.index(-1)]} in the cache")
         return out
 
     def pages(self, seq: int) -> List[int]:

@@ -835,3 +835,19 @@ def test_page_lists_grow_in_steps():
         assert paged._lib().santa_pages_row(cache._pages, a, ctypes.byref(row)) == i + 1
         seen.append(ctypes.addressof(row.contents))
     assert sum(x != y for x, y in zip(seen, seen[1:])) <= 10 and cache.pages(a) == list(range(1000))
+
+
+def test_numbers_that_are_not_whole():
+    """2.5 tokens are none: refused, where they were cut off; any kind of whole
+    numbers is taken, iterators among them."""
+    cache = _cache()
+    a, b = cache.add(x for x in (3.0, 5))
+    for call in (lambda: cache.add([2.5]), lambda: cache.extend([a], [0.5]), lambda: cache.free([a + 0.5]),
+                 lambda: cache.plan([a], 1, [0.5]), lambda: PagedPlan([4.5], heads=1, kv_heads=1, device="cpu"),
+                 lambda: PagedPlan(torch.tensor([4.5]), heads=1, kv_heads=1, device="cpu"),
+                 lambda: copy_pages(cache.k, [0.5], [1]), lambda: cache.lengths([float("nan")])):
+        with pytest.raises(ValueError):
+            call()
+    assert cache.lengths(iter([b, a])) == [5, 3] and cache.lengths(torch.tensor([a, b]).numpy()) == [3, 5]
+    with pytest.raises(RuntimeError, match="no sequence 7"):
+        cache.lengths(x for x in (a, 7))
