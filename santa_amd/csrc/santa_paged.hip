@@ -221,14 +221,14 @@ __global__ __launch_bounds__(256) void rope_append_kernel(const uint16_t* __rest
 // 277 us; half the ring, or two workgroups of half the waves per compute unit,
 // change nothing).  256 rows: issue, of the products (0.42 of a SIMD's cycles), of
 // the softmax's vector work (about as many) and of the steps between them, which
-// hardly overlap: 985 TFLOP/s behind shared prompts (six sequences of 4000 shared,
-// 100 to 1300 own and 1300 new tokens, 314 us), where a plain product of 8192^3
-// reaches 1202.  Counted cycles of that kernel, 664 thousand as it is: the two
+// hardly overlap: 984 TFLOP/s behind shared prompts (six sequences of 4000 shared,
+// 100 to 1300 own and 1300 new tokens, 295 us, and 314 with the join), where a plain
+// product of 8192^3 reaches 1202.  Counted cycles of that kernel, 664 thousand as it is: the two
 // waves of a SIMD half a tile apart, products of one beside the softmax of the
 // other, 685; loads issued between the products 711; steps without bookkeeping
 // 667; first products as soon as their first operand is there 661.  A batch behind
-// a long prompt has both: 64 sequences behind 32k tokens 115 us, 32 with 64 query and
-// 8 KV heads behind 128k 267 us (106 and 215 with rounded probabilities).  Little work: latency, about 10 us for the first
+// a long prompt has both: 64 sequences behind 32k tokens 114 us, 32 with 64 query and
+// 8 KV heads behind 128k 262 us (106 and 215 with rounded probabilities).  Little work: latency, about 10 us for the first
 // loads, one tile, the join of the waves and the output.
 constexpr int kWaves = 8;
 // Above this a row's reference in log2 units is subtracted from the scores before
