@@ -450,9 +450,14 @@ class PagedPlan:
         self._info, self.seq_lens = info, lens
 
     def _captured(self, room: int, follows: bool) -> None:
-        """Notes a captured call with a block table for `room` tokens, whose
-        replays follow an update (a kernel's, which reads the plan) or do not."""
-        self._room = min(room if follows and self.fixed else -1, room if self._room is None else self._room)
+        """Where a graph is captured, notes that it holds a call with a block
+        table for `room` tokens, whose replays follow an update (a kernel's,
+        which reads the plan) or do not."""
+        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+            self._hold(room if follows and self.fixed else -1)
+
+    def _hold(self, room: int) -> None:
+        self._room = room if self._room is None else min(room, self._room)
 
     def _used(self) -> None:
         """Before a call on the current stream: the plan's memory, where it comes
@@ -579,8 +584,6 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages
         raise ValueError("cos and sin must have the device and dtype of qkv")
     if (device.type == "cuda" and dtype in (torch.bfloat16, torch.float16) and D % 16 == 0
             and _plain(qkv, cos, sin, k_pages, v_pages)):
-        if torch.cuda.is_current_stream_capturing():
-            plan._captured(block_table.shape[1] * k_pages.shape[1], True)
         strides = (*_strides(k_pages, "k_pages"), *_strides(v_pages, "v_pages"))
         if _overlaps(k_pages) or _overlaps(v_pages):
             raise ValueError("rows of pages that are written must not overlap")
@@ -593,9 +596,8 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages
                     q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), int(dtype == torch.float16), D,
                     k_pages.shape[0], k_pages.shape[1], (_L * 6)(*strides), table.data_ptr(), row, table.shape[0],
                     ctypes.byref(plan._info), plan._data.data_ptr())
+            plan._captured(block_table.shape[1] * k_pages.shape[1], True)
         return q
-    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-        plan._captured(0, False)
     wide = torch.float64 if qkv.dtype == torch.float64 else torch.float32
     x, c, s = qkv[:, :H + KVH].to(wide), cos.to(wide)[:, None], sin.to(wide)[:, None]
     turned = (x * c + torch.cat([-x[..., D // 2:], x[..., :D // 2]], dim=-1) * s).to(qkv.dtype)
@@ -603,6 +605,7 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages
     page, row = slot // k_pages.shape[1], slot % k_pages.shape[1]
     k_pages[page, row] = turned[token, H:]
     v_pages[page, row] = qkv[token, H + KVH:]
+    plan._captured(0, False)
     return turned[:, :H]
 
 
@@ -684,12 +687,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     if not 1e-37 < scale < 1e37:  # normal in float32, times log2(e) too
         raise ValueError(f"scale must be positive and finite; got {scale}")
     device = q.device
-    kernel = (device.type == "cuda" and q.dtype in (torch.bfloat16, torch.float16) and D in (64, 128)
-              and _plain(q, k_pages, v_pages))
-    if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
-        plan._captured(block_table.shape[1] * k_pages.shape[1], kernel)
-    if not kernel:
-        return _attention_expressions(q, k_pages, v_pages, block_table, plan, scale)
+    if not (device.type == "cuda" and q.dtype in (torch.bfloat16, torch.float16) and D in (64, 128)
+            and _plain(q, k_pages, v_pages)):
+        out = _attention_expressions(q, k_pages, v_pages, block_table, plan, scale)
+        plan._captured(0, False)
+        return out
     out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if N == 0:
         return out
@@ -711,4 +713,5 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     _launch(device, lib.santa_paged_attention, q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(),
             int(q.dtype == torch.float16), D, k_pages.shape[0], k_pages.shape[1], strides, table.data_ptr(), row,
             table.shape[0], info, plan._data.data_ptr(), scale, workspace.data_ptr(), workspace.numel())
+    plan._captured(block_table.shape[1] * k_pages.shape[1], True)
     return out

@@ -777,15 +777,16 @@ def test_captured_plans_are_held():
     would not follow an update, there is none."""
     args = dict(heads=2, kv_heads=1, device="cpu")
     plan = PagedPlan([20, 30], fixed=True, **args)
-    plan._captured(100, True)
-    plan._captured(80, True)
+    plan._captured(10, True)  # nothing is captured here
+    plan._hold(100)
+    plan._hold(80)
     plan.update([80, 1])
     with pytest.raises(RuntimeError, match="81 > 80"):
         plan.update([5, 81])
     assert plan.seq_lens == [80, 1]
-    plan._captured(1000, False)
+    plan._hold(-1)
     loose = PagedPlan([20, 30], **args)
-    loose._captured(1000, True)
+    loose._hold(-1)
     for p in (plan, loose):
         with pytest.raises(RuntimeError, match="a captured call holds"):
             p.update([5, 5])
@@ -851,3 +852,11 @@ def test_numbers_that_are_not_whole():
     assert cache.lengths(iter([b, a])) == [5, 3] and cache.lengths(torch.tensor([a, b]).numpy()) == [3, 5]
     with pytest.raises(RuntimeError, match="no sequence 7"):
         cache.lengths(x for x in (a, 7))
+
+
+def test_which_plans_round():
+    """Several new tokens with more than 32 rows in a sequence; never single ones."""
+    for new, GH, want in (([1, 1], 256, 0), ([1, 0], 33, 0), ([8, 1], 4, 0), ([1, 9], 4, 1), ([2], 16, 0), ([2], 17, 1),
+                          ([0], 4, 0), ([300], 1, 1)):
+        plan = PagedPlan([400] * len(new), heads=2 * GH, kv_heads=2, new_tokens=new, device="cpu")
+        assert plan._info.rounded == want, (new, GH)
