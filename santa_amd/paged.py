@@ -453,7 +453,7 @@ class PagedPlan:
         """Where a graph is captured, notes that it holds a call with a block
         table for `room` tokens, whose replays follow an update (a kernel's,
         which reads the plan) or do not."""
-        if self.device.type == "cuda" and torch.cuda.is_current_stream_capturing():
+        if self._stream is not None and torch._C._cuda_isCurrentStreamCapturing():
             self._hold(room if follows and self.fixed else -1)
 
     def _hold(self, room: int) -> None:
