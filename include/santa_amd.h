@@ -412,10 +412,28 @@ typedef struct santa_paged_plan_info {
   long long records; /* parts: rows of the workspace */
   long long ints, pos_at, merge_at, parts_at, list_at; /* ints of the plan, and where its sections start */
   int rounded; /* how probabilities enter the second product; the caller's to change (santa_paged_attention) */
+  int tree_ints;     /* of a token's record in a plan with trees, 0 in others */
+  long long tree_at; /* where the records start */
 } santa_paged_plan_info;
 int santa_paged_plan(const int* lens, const int* new_tokens, const int* rows, int B, const int* group,
                      const int* shared, int n_groups, int heads, int kv_heads, int fixed, santa_paged_plan_info* info,
                      int* plan, long long plan_ints);
+/* The same where the new tokens of sequences b with trees[b] != 0 are drafts that
+ * follow one another as trees, up to 1024 each: parents (one int per new token of
+ * the batch, those of other sequences not read) names the earlier new token of the
+ * sequence that a token follows, -1: the context (the tokens before the new ones),
+ * -2: not in use, and followed by none.  A token attends to the context, the
+ * tokens that it follows up to there, and itself; one that is not in use is not
+ * written, attends to nothing and gives zeros, as all do of a sequence shorter
+ * than its tree.  Tokens lie in the cache one after the other; a token's position
+ * is the context's length and one for every drafted token that it follows.
+ * A token's record is tree_ints ints from plan[tree_at + token * tree_ints] on: the context
+ * tokens it attends to, its position (-1: not in use), and a bit for each place
+ * from the last multiple of 64 up to the context's end on (bit n % 32 of int
+ * n / 32 behind): whether it attends to that token. */
+int santa_paged_tree_plan(const int* lens, const int* new_tokens, const int* rows, int B, const int* group,
+                          const int* shared, int n_groups, int heads, int kv_heads, int fixed, const int* trees,
+                          const int* parents, santa_paged_plan_info* info, int* plan, long long plan_ints);
 
 /* Exact attention over pages, D = 64 or 128: query i of sequence b (row
  * sum of the earlier new_tokens + i of q [tokens, H, D]) attends to the tokens

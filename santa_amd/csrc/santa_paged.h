@@ -10,8 +10,16 @@ constexpr int kBlockRows = 256;  // rows per workgroup: 32 for each of its 8 wav
 
 enum ItemFlags {
   kFromList = 1,  // tok0 indexes the plan's list of tokens; no row is before the item's end
-  kDirect = 2     // the item is all its rows attend to: it writes the output
+  kDirect = 2,    // the item is all its rows attend to: it writes the output
+  kTree = 4       // what token i attends to from position tree0 on is in its record
 };
+
+// A token's record in a plan with trees: the context tokens that it attends to,
+// its position (-1: not in use), and one bit for each position from the last
+// multiple of 64 up to the context's end on: whether it attends to that token.
+// Records of the plan's other tokens say the same (no bits beyond the context).
+constexpr int kTreeWords = 2;  // where the bits begin
+constexpr int kMostDrafts = 1024;
 
 // What one workgroup per KV head does: rows r < rows, row r being query head
 // r % GH of token tok0 + r / GH, over the tokens begin .. end - 1 (begin a
@@ -21,7 +29,8 @@ struct Item {
   int flags, row, begin, end, tok0, rows, pos0;
   int base;  // record of row 0 at KV head 0; KV head h's are h * rows further
   int next;  // the workgroup's next item, or -1
-  int unused[7];
+  int tree0;
+  int unused[6];
 };
 constexpr int kItemInts = 16;
 static_assert(sizeof(Item) == kItemInts * sizeof(int), "packed");

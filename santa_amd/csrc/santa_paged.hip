@@ -326,6 +326,8 @@ struct AttnArgs {
   uint32_t sk_p, sk_r, sv_p, sv_r;
   int KVH, GH;
   float scale_log2;
+  const int* tree;  // the tokens' records, of tree_ints ints each
+  int tree_ints;
 };
 
 // Where a workgroup's loads are: tile t of an item (in scalar registers), and
@@ -496,13 +498,28 @@ __device__ __forceinline__ void scores(const char* buf, const u32x4 (&qf)[D / 16
   __builtin_amdgcn_sched_group_barrier(0x008, D / 16, 0);
 }
 
-// Their softmax: P^T in the 16-bit type, the running state moved on.  kMasked:
-// the lane's row attends to the first lim + 1 of the tokens.
-template <bool BF16, int KB, int MB, bool kMasked, Parts kParts>
+// Which tokens of a tile rows attend to.
+enum class Mask {
+  kNone,   // all
+  kFirst,  // the first lim + 1
+  kBits    // those whose bit is set
+};
+
+// Their softmax: P^T in the 16-bit type, the running state moved on; lim and bits:
+// what the lane's row attends to.
+template <bool BF16, int KB, int MB, Mask kMask, Parts kParts>
 __device__ __forceinline__ void softmax(f32x16 (&s)[KB], u32x4 (&p)[2 * KB], u32x4 (&low)[2 * KB], int lim,
-                                        float scale_log2, State<MB>& st) {
+                                        const uint32_t (&bits)[KB], float scale_log2, State<MB>& st) {
   const int lane = threadIdx.x & 63;
-  if constexpr (kMasked) {
+  if constexpr (kMask == Mask::kBits) {
+#pragma unroll
+    for (int kb = 0; kb < KB; ++kb) {
+      const uint32_t b = bits[kb] >> (4 * (lane >> 5));
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (!(b & 1u << (8 * (e >> 2) + (e & 3)))) s[kb][e] = -__builtin_inff();
+    }
+  } else if constexpr (kMask == Mask::kFirst) {
     const int left = lim - 4 * (lane >> 5);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb)
@@ -655,6 +672,56 @@ __device__ __forceinline__ void sums_masked(const char* buf, uint32_t vo, const 
   }
 }
 
+// The same for rows of trees, which attend to the tokens of their bits: where a
+// value is not finite, for one drafted token after the other (token: this lane's),
+// the values that it does not attend to left out, and the result kept by its rows.
+template <bool BF16, int D, int KB, int MB, Parts kParts>
+__device__ __forceinline__ void sums_of_bits(const char* buf, uint32_t vo, const u32x4 (&p)[2 * KB],
+                                             const u32x4 (&low)[2 * KB], const uint32_t (&bits)[KB], int token,
+                                             bool apart, State<MB>& st) {
+  using G = Geometry<D>;
+  const int first = apart ? __builtin_amdgcn_readlane(token, 0) : 0;
+  const int last = apart ? __builtin_amdgcn_readlane(token, 31) : 0;
+  for (int at = first; at <= last; ++at) {
+    uint32_t seen[KB];
+    if (apart) {
+      const int from = __ffsll(static_cast<unsigned long long>(__ballot(token == at))) - 1;  // -1: no row here
+      if (from < 0) continue;
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb)
+        seen[kb] = static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(bits[kb]), from)) >>
+                   (4 * (static_cast<int>(threadIdx.x & 63) >> 5));
+    }
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      u32x4 v[2 * KB];
+#pragma unroll
+      for (int kc = 0; kc < 2 * KB; ++kc) v[kc] = read_tr8<G::kRow>(buf + (vo ^ (64 * mb)) + 16 * G::kRow * kc);
+      if (!apart) {
+#pragma unroll
+        for (int kc = 0; kc < 2 * KB; ++kc) {
+          st.o[mb] = mfma32<BF16>(v[kc], p[kc], st.o[mb]);
+          if constexpr (kParts == Parts::kTwo) st.o[mb] = mfma32<BF16>(v[kc], low[kc], st.o[mb]);
+        }
+      } else {
+        f32x16 o = st.o[mb];
+#pragma unroll
+        for (int kc = 0; kc < 2 * KB; ++kc) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const uint32_t two = seen[kc >> 1] >> (16 * (kc & 1) + 8 * (j >> 1) + 2 * (j & 1));  // of the dword's values
+            v[kc][j] &= (two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
+          }
+          o = mfma32<BF16>(v[kc], p[kc], o);
+          if constexpr (kParts == Parts::kTwo) o = mfma32<BF16>(v[kc], low[kc], o);
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) st.o[mb][e] = token == at ? o[e] : st.o[mb][e];
+      }
+    }
+  }
+}
+
 // The workgroup's barrier alone: no wave waits for its loads here.
 __device__ __forceinline__ void barrier() {
   asm volatile("" ::: "memory");
@@ -675,11 +742,13 @@ struct Shares {
 // of the dims and a quarter of the tokens of two tiles (with four waves to a
 // tile, its latency, not HBM, would bound the pass).  tile: the number of the
 // item's first tile, loaded: that of the next one to be loaded, counted over the
-// workgroup's items.
-template <bool BF16, int D, int RG, Parts kParts>
+// workgroup's items.  kTrees: the plan has trees.  A tree's rows differ in the
+// tiles from the context's end on, one or two for trees of up to 64 tokens, whose
+// bits are read with Q; all other tiles are as without trees.
+template <bool BF16, int D, int RG, Parts kParts, bool kTrees>
 __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv, const Loader& w, Cursor& cur,
                                        const uint32_t (&lk)[2], const uint32_t (&lv)[2], uint32_t& tile,
-                                       uint32_t& loaded, u32x4* stages, Shares* x) {
+                                       uint32_t& loaded, u32x4* stages, Shares* x, uint32_t* first_bits) {
   using G = Geometry<D>;
   constexpr int KB = RG == 8 ? 2 : 1;                       // 32s of a tile's tokens that a wave takes
   constexpr int DH = RG >= 4 ? 1 : 2, MB = D / 32 / DH;     // parts of the dims, 32s of them in each
@@ -700,10 +769,27 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv
   const int rc = min(r, it.rows - 1);
   const int i = rc / a.GH, h = kv * a.GH + (rc - i * a.GH);
   const int tok = it.flags & kFromList ? a.list[it.tok0 + i] : it.tok0 + i;
-  const int pos = it.pos0 + i;
-  const int lim = min(it.end - 1, pos);  // last position this row attends to here
-  const int lim_lo = __builtin_amdgcn_readlane(lim, 0), lim_hi = __builtin_amdgcn_readlane(lim, 31);
+  const bool tree = kTrees && (it.flags & kTree);
+  int pos = it.pos0 + i;
+  const int lim = tree ? it.end - 1 : min(it.end - 1, pos);  // last position this row attends to here
+  const int lim_lo = tree ? min(lim, it.tree0 - 1) : __builtin_amdgcn_readlane(lim, 0);
+  const int lim_hi = __builtin_amdgcn_readlane(lim, 31);
   const bool any = 32 * rg < it.rows;
+  // of a tree's tiles, this lane's bits of the first two, in LDS: read by itself
+  // alone, and in registers they would not fit beside the sums
+  uint32_t* const held = kTrees ? first_bits + 4 * (32 * wave + ql) : nullptr;
+  if constexpr (kTrees) {
+    if (tree) {
+      const int* record = a.tree + static_cast<long long>(tok) * a.tree_ints;
+      const int second = a.tree_ints > kTreeWords + 2 ? 2 : 0;
+      pos = record[1];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        held[kb] = record[kTreeWords + kh + kb];
+        held[2 + kb] = record[kTreeWords + kh + second + kb];
+      }
+    }
+  }
 
   // Q fragments: dims 16c + 8 half .. + 7 of this lane's row
   u32x4 qf[D / 16];
@@ -758,7 +844,7 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv
     f32x16 s[KB];
     u32x4 p[2 * KB], low[2 * KB];
     scores<BF16, D, KB>(stage, qf, ko, s);
-    softmax<BF16, KB, MB, false, kParts>(s, p, low, 0, a.scale_log2, st);
+    softmax<BF16, KB, MB, Mask::kNone, kParts>(s, p, low, 0, {}, a.scale_log2, st);
     sums<BF16, D, KB, MB, kParts>(stage, vo, p, low, st);
   }
   for (; t < nt; t += kStep) {  // a loop of its own, or both would run short of registers
@@ -768,9 +854,29 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv
     u32x4 p[2 * KB], low[2 * KB];
     const int n0 = first + (t + mine) * kTile, last = min(it.end, n0 + 32 * KB) - 1;
     scores<BF16, D, KB>(stage, qf, ko, s);
-    softmax<BF16, KB, MB, true, kParts>(s, p, low, lim - n0, a.scale_log2, st);
-    const bool apart = last > lim_lo && not_finite<BF16, D, KB>(stage + 16 * G::kVecs + 32 * kh * G::kRow);
-    sums_masked<BF16, D, KB, MB, kParts>(stage, vo, p, low, n0, last, lim, lim_lo, lim_hi, apart, st);
+    if constexpr (kTrees) {
+      // a row of no tree, as bits: its first lim - n0 + 1 tokens
+      uint32_t now[KB];
+#pragma unroll
+      for (int kb = 0; kb < KB; ++kb) {
+        const int n = lim - n0 - 32 * kb;
+        now[kb] = n >= 31 ? 0xffffffffu : n < 0 ? 0u : (2u << n) - 1u;
+      }
+      if (tree) {
+        const int nth = ((n0 - 32 * kh) >> 6) - (it.tree0 >> 6);  // of the tree's tiles
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+          now[kb] = nth < 2 ? held[2 * nth + kb]
+                            : a.tree[static_cast<long long>(tok) * a.tree_ints + kTreeWords + kh + 2 * nth + kb];
+      }
+      softmax<BF16, KB, MB, Mask::kBits, kParts>(s, p, low, 0, now, a.scale_log2, st);
+      const bool apart = last > lim_lo && not_finite<BF16, D, KB>(stage + 16 * G::kVecs + 32 * kh * G::kRow);
+      sums_of_bits<BF16, D, KB, MB, kParts>(stage, vo, p, low, now, i, apart, st);
+    } else {
+      softmax<BF16, KB, MB, Mask::kFirst, kParts>(s, p, low, lim - n0, {}, a.scale_log2, st);
+      const bool apart = last > lim_lo && not_finite<BF16, D, KB>(stage + 16 * G::kVecs + 32 * kh * G::kRow);
+      sums_masked<BF16, D, KB, MB, kParts>(stage, vo, p, low, n0, last, lim, lim_lo, lim_hi, apart, st);
+    }
   }
   float m = st.m, l = st.l + other_half(st.l);
   f32x16(&o)[MB] = st.o;
@@ -846,13 +952,15 @@ __device__ __forceinline__ void attend(const AttnArgs& a, const Item& it, int kv
   if (!any || r >= it.rows) return;
   const int d0 = 32 * MB * dh + (TG == 1 ? 0 : 8 * EP * tg) + 4 * half;  // of the first piece
   if (it.flags & kDirect) {
-    const float inv = pos < 0 ? 0.0f : 1.0f / l;
+    const bool blind = pos < 0;
+    const float inv = blind ? 0.0f : 1.0f / l;
     uint16_t* orow = a.out + (static_cast<size_t>(tok) * (a.KVH * a.GH) + h) * D + d0;
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb)
 #pragma unroll
       for (int k = 0; k < EP; ++k) {
-        const float4& c = res[mb][k];
+        float4 c = res[mb][k];
+        if (kTrees && blind) c = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // the context's infinities and NaNs
         *reinterpret_cast<uint2*>(orow + 32 * mb + 8 * k) = pack4<BF16>(c.x * inv, c.y * inv, c.z * inv, c.w * inv);
       }
     return;
@@ -870,15 +978,16 @@ __device__ __forceinline__ Item read_item(const Loader& w, int i) {
   Const<Item>* p = w.items + i;
   Item it;
   it.flags = p->flags, it.row = p->row, it.begin = p->begin, it.end = p->end, it.tok0 = p->tok0, it.rows = p->rows;
-  it.pos0 = p->pos0, it.base = p->base, it.next = p->next;
+  it.pos0 = p->pos0, it.base = p->base, it.next = p->next, it.tree0 = p->tree0;
   return it;
 }
 
-template <bool BF16, int D, Parts kParts>
+template <bool BF16, int D, Parts kParts, bool kTrees>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_attention_kernel(AttnArgs a) {
   using G = Geometry<D>;
   __shared__ u32x4 stages[G::kStages * G::kStage];
   __shared__ Shares shares;
+  __shared__ uint32_t first_bits[kTrees ? 4 * kBlockRows : 1];
   constexpr Parts kLanes = kParts == Parts::kTwo ? Parts::kLanesOfTwo : Parts::kLanes;
   const int kv = blockIdx.x % a.KVH, group = blockIdx.x / a.KVH;
   const int lane = threadIdx.x & 63;
@@ -917,11 +1026,11 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_attention_kernel(AttnArg
     const Item now = it;
     last = now.next < 0;
     if (!last) it = read_item(w, now.next);  // while this one is worked on
-    if (now.rows <= 16) attend<BF16, D, 1, kLanes>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares);
-    else if (now.rows <= 32) attend<BF16, D, 1, kParts>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares);
-    else if (now.rows <= 64) attend<BF16, D, 2, kParts>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares);
-    else if (now.rows <= 128) attend<BF16, D, 4, kParts>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares);
-    else attend<BF16, D, 8, kParts>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares);
+    if (now.rows <= 16) attend<BF16, D, 1, kLanes, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares, first_bits);
+    else if (now.rows <= 32) attend<BF16, D, 1, kParts, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares, first_bits);
+    else if (now.rows <= 64) attend<BF16, D, 2, kParts, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares, first_bits);
+    else if (now.rows <= 128) attend<BF16, D, 4, kParts, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares, first_bits);
+    else attend<BF16, D, 8, kParts, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares, first_bits);
   }
 }
 
@@ -992,6 +1101,7 @@ __global__ __launch_bounds__(256) void merge_kernel(const float* __restrict__ pa
 #pragma unroll
     for (int t = 0; t < kTeams; ++t) add(s_m[t], s_z[t], s_o[t][d4]);
   }
+  if (blind) acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);  // a token not in use has parts where others share a prefix
   const float inv = blind ? 0.0f : 1.0f / z;
   *reinterpret_cast<uint2*>(out + (static_cast<size_t>(tok) * H + h) * D + 4 * d4) =
       pack4<BF16>(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
@@ -1161,6 +1271,8 @@ extern "C" int santa_paged_attention(const void* q, const void* k_pages, const v
   a.part_ml = a.part + static_cast<size_t>(info->records) * D;
   a.items = reinterpret_cast<const Item*>(plan);
   a.list = plan + info->list_at;
+  a.tree = plan + info->tree_at;
+  a.tree_ints = info->tree_ints;
   a.pg = pg;
   a.sq_t = strides[0], a.sq_h = strides[1];
   if (strides[2] >= 1LL << 31 || strides[5] >= 1LL << 31)
@@ -1186,8 +1298,13 @@ extern "C" int santa_paged_attention(const void* q, const void* k_pages, const v
       hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(info->groups) * KVH), dim3(64 * kWaves), 0, stream, a);
     };
     if (info->groups > 0) {
-      if (info->rounded) attend(paged_attention_kernel<BF16, kD, Parts::kOne>);
-      else attend(paged_attention_kernel<BF16, kD, Parts::kTwo>);
+      if (info->tree_ints > 0) {
+        if (info->rounded) attend(paged_attention_kernel<BF16, kD, Parts::kOne, true>);
+        else attend(paged_attention_kernel<BF16, kD, Parts::kTwo, true>);
+      } else {
+        if (info->rounded) attend(paged_attention_kernel<BF16, kD, Parts::kOne, false>);
+        else attend(paged_attention_kernel<BF16, kD, Parts::kTwo, false>);
+      }
     }
     const long long rows = static_cast<long long>(info->merge_tokens) * H;
     // a workgroup per row up to one resident round of them (2048 rows of 14 parts

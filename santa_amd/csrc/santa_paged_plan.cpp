@@ -24,6 +24,7 @@ constexpr int kMaxLen = 1 << 30;
 // the list.
 struct Block {
   int flags, row, begin, end, tok0, ntok, pos0;
+  int tree0 = 0;
   int tiles() const { return (end - begin + kTile - 1) / kTile; }
 };
 
@@ -61,7 +62,31 @@ struct Input {
   int B;
   const int *group, *shared;
   int n_groups, heads, kv_heads, fixed;
+  const int *parents, *trees;  // NULL: no trees
+  bool tree(int b) const { return trees && trees[b]; }
 };
+
+// The most drafted tokens that a sequence has in a tree, or an error.
+int check_trees(const Input& in, int* most) {
+  *most = 0;
+  const int* parent = in.parents;
+  for (int b = 0; b < in.B; parent += in.new_tokens[b++]) {
+    if (!in.tree(b)) continue;
+    const int t = in.new_tokens[b];
+    if (t > kMostDrafts)
+      return set_error(SANTA_ERR_UNSUPPORTED, "a tree has up to %d tokens. Got %d", kMostDrafts, t);
+    *most = std::max(*most, t);
+    for (int i = 0; i < t; ++i) {
+      if (parent[i] < -2 || parent[i] >= i)
+        return set_error(SANTA_ERR_INVALID, "sequence %d: the parent of new token %d is an earlier one, -1 or -2; got %d",
+                         b, i, parent[i]);
+      if (parent[i] >= 0 && parent[parent[i]] == -2)
+        return set_error(SANTA_ERR_INVALID, "sequence %d: new token %d follows token %d, which is not in use", b, i,
+                         parent[i]);
+    }
+  }
+  return SANTA_OK;
+}
 
 int build(const Input& in, santa_paged_plan_info* info, int* plan, long long plan_ints) {
   const int GH = in.heads / in.kv_heads;
@@ -98,6 +123,14 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
     ++members[g];
   }
   info->tokens = static_cast<int>(tokens);
+  int most = 0;
+  if (in.trees) {
+    const int rc = check_trees(in, &most);
+    if (rc != SANTA_OK) return rc;
+    // the context's last tile and those that the new tokens begin
+    info->tree_ints = kTreeWords + 2 * ((std::max(1, most) + 126) / 64);
+    if (tokens * info->tree_ints > 1 << 26) return set_error(SANTA_ERR_INVALID, "too many new tokens beside trees");
+  }
 
   // the passes: whole tiles of each group's common tokens for all its rows, and
   // the rest of each sequence for its own
@@ -119,18 +152,19 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
       }
     const int n = static_cast<int>(list.size()) - group_list[g];
     for (int i = 0; i < n; i += block_tokens)
-      blocks.push_back({kFromList, lead[g], 0, common, group_list[g] + i, std::min(block_tokens, n - i), kMaxLen});
+      blocks.push_back({kFromList, lead[g], 0, common, group_list[g] + i, std::min(block_tokens, n - i), kMaxLen, 0});
   }
   for (int b = 0; b < in.B; ++b) {
     const int n = in.lens[b], t = in.new_tokens[b], row = in.rows ? in.rows[b] : b;
+    const bool tree = in.tree(b), vacant = tree && n < t;  // a tree that its sequence does not hold: no token in use
     for (int i = 0; i < t; ++i) {
-      token_pos[first[b] + i] = n - t + i;
+      token_pos[first[b] + i] = tree && (vacant || in.parents[first[b] + i] == -2) ? -1 : n - t + i;
       token_row[first[b] + i] = row;
     }
     for (int i = 0; i < t; i += block_tokens) {
       const int k = std::min(block_tokens, t - i);
-      const int end = std::max(prefix[b], std::min(n, n - t + i + k));
-      blocks.push_back({0, row, prefix[b], end, first[b] + i, k, n - t + i});
+      const int end = vacant ? 0 : std::max(prefix[b], std::min(n, n - t + i + k));
+      blocks.push_back({tree ? kTree : 0, row, prefix[b], end, first[b] + i, k, n - t + i, tree ? std::max(0, n - t) : 0});
     }
   }
 
@@ -214,6 +248,10 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
   info->merge_at = info->parts_at + 8 * tokens;
   info->list_at = info->merge_at + info->merge_tokens;
   info->ints = info->list_at + static_cast<long long>(list.size());
+  if (in.trees) {
+    info->tree_at = (info->ints + 3) & ~3LL;
+    info->ints = info->tree_at + tokens * info->tree_ints;
+  }
   if (!plan) return clear_error();
   if (plan_ints < info->ints) return set_error(SANTA_ERR_INVALID, "the plan does not fit its buffer");
 
@@ -235,6 +273,7 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
     it.pos0 = k.pos0;
     it.base = base[i];
     it.next = -1;
+    it.tree0 = k.tree0;
     const bool first = i == 0 || pieces[i - 1].slot != p.slot;
     const int at = first ? p.slot : more++;
     if (!first) plan[static_cast<size_t>(last) * kItemInts + offsetof(Item, next) / sizeof(int)] = at;
@@ -253,6 +292,29 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
   for (int t = 0; t < info->merge_tokens; ++t)
     plan[info->merge_at + t] = t < static_cast<int>(joined.size()) ? joined[t] : -1;
   std::copy(list.begin(), list.end(), plan + info->list_at);
+  for (int b = 0; in.trees && b < in.B; ++b) {
+    const int n = in.lens[b], t = in.new_tokens[b], p0 = n - t, from = p0 & ~63;
+    const int* parent = in.parents + first[b];
+    int* record = plan + info->tree_at + static_cast<long long>(first[b]) * info->tree_ints;
+    for (int i = 0; i < t; ++i, record += info->tree_ints) {
+      uint32_t* bits = reinterpret_cast<uint32_t*>(record + kTreeWords);
+      record[0] = std::max(0, p0 + i + 1);
+      record[1] = p0 + i;
+      if (!in.tree(b)) continue;
+      record[0] = 0;
+      record[1] = -1;
+      if (p0 < 0 || parent[i] == -2) continue;
+      record[0] = p0;
+      const int* before = record - static_cast<long long>(i - parent[i]) * info->tree_ints;
+      if (parent[i] >= 0) {
+        std::memcpy(bits, before + kTreeWords, static_cast<size_t>(info->tree_ints - kTreeWords) * sizeof(int));
+      } else {
+        for (int p = from; p < p0; ++p) bits[(p - from) >> 5] |= 1u << (p & 31);
+      }
+      record[1] = parent[i] >= 0 ? before[1] + 1 : p0;
+      bits[(p0 + i - from) >> 5] |= 1u << ((p0 + i) & 31);
+    }
+  }
   return clear_error();
 }
 
@@ -260,12 +322,13 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
 }  // namespace paged
 }  // namespace santa
 
-extern "C" int santa_paged_plan(const int* lens, const int* new_tokens, const int* rows, int B, const int* group,
-                                const int* shared, int n_groups, int heads, int kv_heads, int fixed,
-                                santa_paged_plan_info* info, int* plan, long long plan_ints) {
+namespace {
+int make_plan(const santa::paged::Input& in, santa_paged_plan_info* info, int* plan, long long plan_ints) {
   using namespace santa;
-  if (!info || B < 0 || (B > 0 && (!lens || !new_tokens)) || n_groups < 0 || (n_groups > 0 && (!group || !shared)))
+  if (!info || in.B < 0 || (in.B > 0 && (!in.lens || !in.new_tokens)) || in.n_groups < 0 ||
+      (in.n_groups > 0 && (!in.group || !in.shared)))
     return set_error(SANTA_ERR_INVALID, "bad santa_paged_plan arguments");
+  const int heads = in.heads, kv_heads = in.kv_heads;
   if (kv_heads <= 0 || heads <= 0 || heads % kv_heads != 0)
     return set_error(SANTA_ERR_INVALID, "H must be divisible by KVH. Got H=%d KVH=%d", heads, kv_heads);
   if (heads > 1 << 16) return set_error(SANTA_ERR_UNSUPPORTED, "too many heads");
@@ -273,10 +336,27 @@ extern "C" int santa_paged_plan(const int* lens, const int* new_tokens, const in
     return set_error(SANTA_ERR_UNSUPPORTED, "the paged attention takes up to %d query heads per KV head. Got %d",
                      paged::kBlockRows, heads / kv_heads);
   try {
-    return paged::build({lens, new_tokens, rows, B, n_groups > 0 ? group : nullptr, shared, n_groups, heads, kv_heads,
-                         fixed},
-                        info, plan, plan_ints);
+    return paged::build(in, info, plan, plan_ints);
   } catch (const std::exception&) {  // vectors that do not fit
     return set_error(SANTA_ERR_INVALID, "out of host memory");
   }
+}
+}  // namespace
+
+extern "C" int santa_paged_plan(const int* lens, const int* new_tokens, const int* rows, int B, const int* group,
+                                const int* shared, int n_groups, int heads, int kv_heads, int fixed,
+                                santa_paged_plan_info* info, int* plan, long long plan_ints) {
+  return make_plan({lens, new_tokens, rows, B, n_groups > 0 ? group : nullptr, shared, n_groups, heads, kv_heads, fixed,
+                    nullptr, nullptr},
+                   info, plan, plan_ints);
+}
+
+extern "C" int santa_paged_tree_plan(const int* lens, const int* new_tokens, const int* rows, int B, const int* group,
+                                     const int* shared, int n_groups, int heads, int kv_heads, int fixed,
+                                     const int* trees, const int* parents, santa_paged_plan_info* info, int* plan,
+                                     long long plan_ints) {
+  if (B > 0 && (!trees || !parents)) return santa::set_error(SANTA_ERR_INVALID, "bad santa_paged_tree_plan arguments");
+  return make_plan({lens, new_tokens, rows, B, n_groups > 0 ? group : nullptr, shared, n_groups, heads, kv_heads, fixed,
+                    parents, trees},
+                   info, plan, plan_ints);
 }

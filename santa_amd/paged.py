@@ -46,7 +46,7 @@ class _PlanInfo(ctypes.Structure):
     _fields_ = ([(n, _I) for n in ("tokens", "groups", "items", "merge_tokens", "max_len", "max_row", "heads",
                                    "kv_heads")]
                 + [(n, _L) for n in ("records", "ints", "pos_at", "merge_at", "parts_at", "list_at")]
-                + [("rounded", _I)])
+                + [("rounded", _I), ("tree_ints", _I), ("tree_at", _L)])
 
 
 _lib_ready = None
@@ -74,6 +74,7 @@ def _lib():
         L.santa_pages_apply.argtypes = [_P, ctypes.POINTER(_P), _I, _L, _L, _P, _L, _I, _P]
         L.santa_paged_copy.argtypes = [ctypes.POINTER(_P), _I, _L, _L, _I, _IP, _I, _P]
         L.santa_paged_plan.argtypes = [_IP, _IP, _IP, _I, _IP, _IP, _I, _I, _I, _I, info, _P, _L]
+        L.santa_paged_tree_plan.argtypes = [_IP, _IP, _IP, _I, _IP, _IP, _I, _I, _I, _I, _IP, _IP, info, _P, _L]
         L.santa_paged_workspace_size.argtypes = [info, _I]
         L.santa_paged_workspace_size.restype = ctypes.c_size_t
         L.santa_paged_attention.argtypes = [_P] * 4 + [_I] * 4 + [ctypes.POINTER(_L), _P, _L, _I, info, _P,
@@ -256,10 +257,10 @@ class PagedKVCache:
         return self.block_table.index_select(0, at.to(self.device, non_blocking=True))
 
     def plan(self, seqs: Sequence[int], heads: int, new_tokens: Union[int, Sequence[int]] = 1, *,
-             fixed: bool = False) -> "PagedPlan":
+             fixed: bool = False, parents: Optional[Sequence[Optional[Sequence[int]]]] = None) -> "PagedPlan":
         """The plan of these sequences' attention, the last new_tokens of each
-        being its queries; tokens that sequences hold in the same pages are read
-        once."""
+        being its queries (parents: as trees); tokens that sequences hold in the
+        same pages are read once."""
         seqs = _int_list(seqs, "seqs")
         lens = self.lengths(seqs)
         own = [new_tokens] * len(seqs) if isinstance(new_tokens, int) else _int_list(new_tokens, "new_tokens")
@@ -273,7 +274,7 @@ class PagedKVCache:
             if g >= 0:
                 members[g].append(i)
         return PagedPlan(lens, heads=heads, kv_heads=self.kv_heads, new_tokens=own, rows=seqs, fixed=fixed,
-                         prefixes=[(m, shared[g]) for g, m in enumerate(members)], device=self.device)
+                         parents=parents, prefixes=[(m, shared[g]) for g, m in enumerate(members)], device=self.device)
 
     # -------------------------------------------------------------- changes
     def _may_change(self) -> None:
@@ -364,9 +365,19 @@ class PagedPlan:
     tokens in common, which lie before the new tokens of each; they are read
     once for all, through the row of one of them.
 
+    parents: for new tokens that are drafts and follow one another as trees, one
+    entry per sequence: None, or for each of its new tokens (at most 1024) the
+    earlier one of them that it follows, -1: the context (the tokens before the
+    new ones), -2: not in use.  A drafted token attends to the context, the drafted
+    tokens that it follows up to there, and itself, and its position is the one
+    behind the token that it follows; in the cache the new tokens lie one after the
+    other all the same.  A token not in use is not written and attends to nothing,
+    which gives zeros, and none follows it; a sequence shorter than its tree has
+    none in use.
+
     The plan is built on the host and copied to the device on the current
     stream.  `update(seq_lens)` makes it that of other lengths of the same
-    sequences.  With fixed=True an update keeps the launches and workspaces of
+    sequences, and of other trees of as many tokens.  With fixed=True an update keeps the launches and workspaces of
     the kernels' calls the same, so that a captured graph can be replayed after
     it (at the cost of workgroups without work), up to the lengths that the
     captured calls' block tables have room for.  A plan that a graph holds in
@@ -375,7 +386,7 @@ class PagedPlan:
 
     def __init__(self, seq_lens: Sequence[int], *, heads: int, kv_heads: int, new_tokens: Union[int, Sequence[int]] = 1,
                  prefixes: Sequence[Tuple[Sequence[int], int]] = (), rows: Optional[Sequence[int]] = None,
-                 device="cuda", fixed: bool = False):
+                 device="cuda", fixed: bool = False, parents: Optional[Sequence[Optional[Sequence[int]]]] = None):
         lens = _int_list(seq_lens, "seq_lens")
         B = len(lens)
         self.heads, self.kv_heads = _ints([int(heads), int(kv_heads)])
@@ -396,20 +407,42 @@ class PagedPlan:
                 group[b] = g
         self._args = (_ints(self.new_tokens), _ints(self.rows), B, _ints(group),
                       _ints([n for _, n in self.prefixes]), len(self.prefixes))
+        self.parents = None if parents is None else self._trees(parents)
         self._info = _PlanInfo()
         # room for a plan: its items, in whole pieces of 256 rows and a cut for every workgroup, and what it says of
         # each token; one that is larger is built again
         tokens, rows = sum(max(0, t) for t in self.new_tokens), max(1, 256 * self.kv_heads // max(1, self.heads))
         self._size = min(1 << 22, 16 * (B + 2 * (tokens // rows) + len(self.prefixes) + 256 // max(1, self.kv_heads) + 1)
                          + 12 * tokens + 2)
+        if self.parents is not None:
+            most = max((len(p) for p in self.parents if p is not None), default=0)
+            self._size = min(1 << 22, self._size + (2 + 2 * ((max(1, most) + 126) // 64)) * tokens + 4)
         self._data = self._stream = None
         self._room = None  # what captured calls have room for
         self.update(lens)
 
-    def update(self, seq_lens: Sequence[int]) -> None:
-        """The plan of other lengths.  Calls that use the plan on other streams,
-        and replays of graphs that hold them, are ordered by the caller."""
+    def _trees(self, parents) -> List[Optional[List[int]]]:
+        parents = [None if p is None else _int_list(p, "parents") for p in parents]
+        if len(parents) != len(self.new_tokens):
+            raise ValueError(f"parents must have one entry per sequence ({len(self.new_tokens)})")
+        for b, (p, t) in enumerate(zip(parents, self.new_tokens)):
+            if p is not None and len(p) != t:
+                raise ValueError(f"sequence {b} has {t} new tokens; got {len(p)} parents")
+        return parents
+
+    def update(self, seq_lens: Sequence[int], parents: Optional[Sequence[Optional[Sequence[int]]]] = None) -> None:
+        """The plan of other lengths and, with parents, of other trees for the
+        sequences that have one.  Calls that use the plan on other streams, and
+        replays of graphs that hold them, are ordered by the caller."""
         lens = _int_list(seq_lens, "seq_lens")
+        trees = self.parents
+        if parents is not None:
+            if trees is None:
+                raise ValueError("the plan was made without trees")
+            parents = self._trees(parents)
+            if any((p is None) != (old is None) for p, old in zip(parents, trees)):
+                raise ValueError("an update has trees for the sequences that had one")
+            trees = parents
         new, rows, B, group, shared, groups = self._args
         if len(lens) != B:
             raise ValueError(f"seq_lens must have one entry per sequence ({B})")
@@ -423,14 +456,19 @@ class PagedPlan:
             raise RuntimeError(f"seq_lens exceeds the block table's capacity in a captured call: {max(lens)} > "
                                f"{self._room}")
         info = _PlanInfo()
+        args = (_ints(lens), new, rows, B, group, shared, groups, self.heads, self.kv_heads, int(self.fixed))
+        if trees is None:
+            make = _lib().santa_paged_plan
+        else:
+            make = _lib().santa_paged_tree_plan
+            args += (_ints([p is not None for p in trees]),
+                     _ints([x for p, t in zip(trees, self.new_tokens) for x in ([-1] * t if p is None else p)]))
 
         def build(buffer, n):
             if cuda:  # the plan is cut to that device's compute units
                 with torch.cuda.device(self.device):
-                    return _lib().santa_paged_plan(_ints(lens), new, rows, B, group, shared, groups, self.heads,
-                                                   self.kv_heads, int(self.fixed), ctypes.byref(info), buffer, n)
-            return _lib().santa_paged_plan(_ints(lens), new, rows, B, group, shared, groups, self.heads, self.kv_heads,
-                                           int(self.fixed), ctypes.byref(info), buffer, n)
+                    return make(*args, ctypes.byref(info), buffer, n)
+            return make(*args, ctypes.byref(info), buffer, n)
 
         with torch.inference_mode(False):  # updated in any mode
             host = torch.empty(self._size, dtype=torch.int32, pin_memory=cuda)
@@ -447,7 +485,7 @@ class PagedPlan:
                 self._data = host.to(self.device, non_blocking=True)
                 if cuda:
                     self._stream = torch._C._cuda_getCurrentRawStream(self.device.index)
-        self._info, self.seq_lens = info, lens
+        self._info, self.seq_lens, self.parents = info, lens, trees
 
     def _captured(self, room: int, follows: bool) -> None:
         """Where a graph is captured, notes that it holds a call with a block
@@ -472,9 +510,28 @@ class PagedPlan:
 
     @property
     def positions(self) -> torch.Tensor:
-        """The position of every token of the batch, int32 [tokens] on the device."""
-        at = self._info.pos_at
-        return self._data[at:at + 2 * self.tokens:2]
+        """The position of every token of the batch, int32 [tokens] on the device
+        (-1: a drafted token not in use)."""
+        at, step = self._info.pos_at, 2
+        if self._info.tree_ints:
+            at, step = self._info.tree_at + 1, self._info.tree_ints
+        return self._data[at:at + step * self.tokens:step]
+
+    def _in_use(self, b: int) -> List[int]:
+        """Which of sequence b's new tokens have a place in it."""
+        n, t, parents = self.seq_lens[b], self.new_tokens[b], self.parents and self.parents[b]
+        if parents is None:
+            return list(range(max(0, t - n), t))
+        return [] if n < t else [i for i, p in enumerate(parents) if p != -2]
+
+    def _sees(self, b: int) -> torch.Tensor:
+        """[t, t]: which of sequence b's drafted tokens its drafted tokens attend to."""
+        parents = self.parents[b]
+        sees = torch.eye(len(parents), dtype=torch.bool)
+        for i, p in enumerate(parents):
+            if p >= 0:
+                sees[i] |= sees[p]
+        return sees
 
 
 def _check_pools(k_pages, v_pages, block_table, plan: PagedPlan, like: torch.Tensor) -> None:
@@ -552,8 +609,8 @@ def _table_rows(table: torch.Tensor) -> Tuple[torch.Tensor, int]:
 def _token_slots(block_table, plan: PagedPlan, page_size: int):
     """(token of the batch, pool row) of the tokens that have a position."""
     token, seq, pos, t0 = [], [], [], 0
-    for row, n, t in zip(plan.rows, plan.seq_lens, plan.new_tokens):
-        for i in range(max(0, t - n), t):
+    for b, (row, n, t) in enumerate(zip(plan.rows, plan.seq_lens, plan.new_tokens)):
+        for i in plan._in_use(b):
             token.append(t0 + i)
             seq.append(row)
             pos.append(n - t + i)
@@ -630,7 +687,11 @@ def _attention_expressions(q, k_pages, v_pages, block_table, plan: PagedPlan, sc
     page_size, KVH = k_pages.shape[1:3]
     wide = torch.float64 if q.dtype == torch.float64 else torch.float32
     out, t0 = [], 0
-    for row, n, t in zip(plan.rows, plan.seq_lens, plan.new_tokens):
+    for b, (row, n, t) in enumerate(zip(plan.rows, plan.seq_lens, plan.new_tokens)):
+        if plan.parents is not None and plan.parents[b] is not None:
+            out.append(_tree_expressions(q[t0:t0 + t], k_pages, v_pages, block_table[row], plan, b, scale))
+            t0 += t
+            continue
         blind = min(t, max(0, t - n))  # tokens of a negative position
         if blind:
             out.append(torch.zeros_like(q[t0:t0 + blind]))
@@ -651,6 +712,28 @@ def _attention_expressions(q, k_pages, v_pages, block_table, plan: PagedPlan, sc
     return torch.cat(out) if out else torch.empty_like(q)
 
 
+def _tree_expressions(q, k_pages, v_pages, table, plan: PagedPlan, b: int, scale: float) -> torch.Tensor:
+    """The same for the drafted tokens q [t, H, D] of sequence b."""
+    t, H, D = q.shape
+    page_size, KVH = k_pages.shape[1:3]
+    n, used = plan.seq_lens[b], torch.tensor(plan._in_use(b), dtype=torch.int64, device=q.device)
+    if not len(used):
+        return torch.zeros_like(q)
+    wide = torch.float64 if q.dtype == torch.float64 else torch.float32
+    at = torch.arange(n, device=q.device)
+    page, r = table[at // page_size].long(), at % page_size
+    k = k_pages[page, r].to(wide).permute(1, 2, 0).contiguous()
+    v = v_pages[page, r].to(wide).permute(1, 0, 2).contiguous()
+    seen = torch.ones(len(used), n, dtype=torch.bool, device=q.device)
+    seen[:, n - t:] = plan._sees(b).to(q.device)[used]
+    seen = seen.repeat_interleave(H // KVH, 0)                                               # [tokens * GH, n]
+    x = q[used].to(wide).reshape(-1, KVH, H // KVH, D).permute(1, 0, 2, 3).reshape(KVH, -1, D).contiguous()
+    s = (torch.bmm(x, k) * scale).masked_fill(~seen, float("-inf"))
+    o = _weighted(torch.softmax(s, dim=-1), v, seen)
+    o = o.view(KVH, len(used), H // KVH, D).permute(1, 0, 2, 3).reshape(len(used), H, D).to(q.dtype)
+    return torch.zeros_like(q).index_copy(0, used, o)
+
+
 def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, block_table: torch.Tensor,
                     plan: Union[PagedPlan, Sequence[int]], *, scale: Optional[float] = None,
                     rounded: Optional[bool] = None) -> torch.Tensor:
@@ -658,8 +741,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     (the tokens of the plan, sequence after sequence), k_pages and v_pages
     [num_pages, page_size, KVH, D] which hold the tokens themselves already,
     block_table int32 [sequences, pages] -> [tokens, H, D].  A token attends to
-    the tokens of its sequence up to itself; one at a negative position gives
-    zeros.  plan: a PagedPlan, or the lengths of the sequences, each with one
+    the tokens of its sequence up to itself or, where the plan has a tree of them,
+    to those that it follows in it; one at a negative position gives zeros.  plan: a PagedPlan, or the lengths of the sequences, each with one
     new token.  scale: of the scores, positive, 1 / sqrt(D) by default.
 
     bf16 and f16 of head_dim 64 and 128 on a GPU run as one kernel over all
