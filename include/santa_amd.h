@@ -346,6 +346,10 @@ int santa_rt_exact_decode(const void* q, const void* k, const void* v, void* out
  *     copy.
  *   _shrink: the last tokens[i] tokens of seqs[i] (each named once) leave it, and
  *     it gives up the pages that hold none of those left.
+ *   _keep: of the last new_tokens[i] tokens of seqs[i] (each named once) the
+ *     counts[i] of those numbers stay that kept names (one sequence's after the
+ *     other's, ascending), and move up behind the tokens before; the others leave.
+ *     What moves must not be in pages that other sequences hold.
  *   _fork: n new sequences that hold every page of seq.
  *   _free: the sequences end; a page that none holds is free.
  *   _compact: with n pages in use, those numbered n and above move to the
@@ -354,8 +358,11 @@ int santa_rt_exact_decode(const void* q, const void* k, const void* v, void* out
  * page copies [n][2] (source, destination), edits of the block table [n][4]
  * (row, first entry, count, value: entry first + i becomes value + i or, for a
  * negative value, entry first + i of row -1 - value), and whether every table
- * entry that is a copy's source becomes its destination.
- * _length: tokens of a sequence (-1: no such sequence); _used: pages in use;
+ * entry that is a copy's source becomes its destination.  _moves: the rows that
+ * _keep moves, [n][5]: page and row of the source, page and row of the destination,
+ * the sequence's number (0, 1, ...); those of a sequence are carried out in order.
+ * _length: tokens of a sequence (-1: no such sequence); _page_size: as created;
+ * _used: pages in use;
  * _row: a sequence's pages, returns how many.
  * _shared: groups of the sequences seqs whose first tokens lie in the same pages,
  * the last own[i] >= 0 tokens of each apart: group[i] is a group or -1, shared[g] the
@@ -366,6 +373,9 @@ void santa_pages_destroy(santa_pages* p);
 int santa_pages_add(santa_pages* p, const int* lengths, int n, int* seqs);
 int santa_pages_extend(santa_pages* p, const int* seqs, const int* tokens, int n);
 int santa_pages_shrink(santa_pages* p, const int* seqs, const int* tokens, int n);
+int santa_pages_keep(santa_pages* p, const int* seqs, const int* new_tokens, const int* kept, const int* counts, int n);
+int santa_pages_moves(const santa_pages* p, const int** moves, int* n);
+int santa_pages_page_size(const santa_pages* p);
 int santa_pages_fork(santa_pages* p, int seq, int n, int* seqs);
 int santa_pages_free(santa_pages* p, const int* seqs, int n);
 int santa_pages_compact(santa_pages* p);
@@ -388,6 +398,10 @@ int santa_paged_copy(const void* const* pools, int n_pools, long long page_bytes
  * table [max_seqs, table_stride], on `stream`. */
 int santa_pages_apply(const santa_pages* p, const void* const* pools, int n_pools, long long page_bytes,
                       long long page_stride, int* table, long long table_stride, int max_seqs, hipStream_t stream);
+/* The rows that the last call, santa_pages_keep, moves, in every pool (whose
+ * pages are rows of page_bytes / page_size bytes). */
+int santa_pages_apply_moves(const santa_pages* p, const void* const* pools, int n_pools, long long page_bytes,
+                            long long page_stride, hipStream_t stream);
 
 /* Attention plan: how the work of santa_paged_attention is cut up for one set
  * of lengths, built on the host once and used by every layer.  Sequence b

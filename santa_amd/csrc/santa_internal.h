@@ -62,6 +62,12 @@ struct PageCopy {
 struct TableEdit {
   int row, col, count, value;
 };
+// A token's K and V moved to another place of its sequence, in every pool; the
+// moves of a sequence (`group`: 0, 1, ...) follow one another and move it towards its
+// front, so that carried out in order none reads what an earlier one wrote.
+struct RowMove {
+  int src_page, src_row, dst_page, dst_row, group;
+};
 
 constexpr size_t kWsAlign = 256;
 inline size_t align_up(size_t x) { return (x + kWsAlign - 1) & ~(kWsAlign - 1); }

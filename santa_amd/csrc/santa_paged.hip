@@ -94,6 +94,67 @@ __global__ __launch_bounds__(256) void remap_table_kernel(RemapArgs a) {
   if (lo < a.n && a.pair[lo].src == page) a.table[i] = a.pair[lo].dst;
 }
 
+constexpr int kMovesPerLaunch = 152;
+constexpr int kMovePools = 64;
+constexpr int kMoveAhead = 8;
+
+struct MoveArgs {
+  char* pool[kMovePools];
+  RowMove move[kMovesPerLaunch];
+  short first[kMovesPerLaunch + 1];  // of each group, and the end of the last one
+  long long stride, row;             // bytes from page to page and from row to row
+  uint32_t pieces;                   // of a row
+};
+
+// Workgroup (pieces of a row, sequence, pool).  A thread moves its own piece of
+// every row of a sequence, in order, up to eight read before they are written (a
+// later row never reads what an earlier one wrote, so that a batch of reads may come
+// first), and no thread touches another's pieces: nothing to wait for.  Latency bound:
+// a launch, a read and a write.
+template <class T>
+__global__ __launch_bounds__(128) void move_rows_kernel(MoveArgs a) {
+  const uint32_t i = blockIdx.x * 128u + threadIdx.x;
+  if (i >= a.pieces) return;
+  char* const pool = a.pool[blockIdx.z] + i * sizeof(T);
+  const int end = a.first[blockIdx.y + 1];
+  for (int m = a.first[blockIdx.y]; m < end; m += kMoveAhead) {
+    T v[kMoveAhead];
+#pragma unroll
+    for (int k = 0; k < kMoveAhead; ++k)
+      if (m + k < end)
+        v[k] = *reinterpret_cast<const T*>(pool + a.move[m + k].src_page * a.stride + a.move[m + k].src_row * a.row);
+#pragma unroll
+    for (int k = 0; k < kMoveAhead; ++k)
+      if (m + k < end)
+        *reinterpret_cast<T*>(pool + a.move[m + k].dst_page * a.stride + a.move[m + k].dst_row * a.row) = v[k];
+  }
+}
+
+hipError_t launch_moves(const void* const* pools, int n_pools, long long row, long long stride, const RowMove* moves,
+                        int n, hipStream_t stream) {
+  MoveArgs a;
+  a.stride = stride;
+  a.row = row;
+  const bool wide = row % 16 == 0;
+  a.pieces = static_cast<uint32_t>(wide ? row / 16 : row);
+  for (int i = 0; i < n; i += kMovesPerLaunch) {  // a sequence may go on in the next launch, which waits for this one
+    const int k = std::min(kMovesPerLaunch, n - i);
+    std::copy(moves + i, moves + i + k, a.move);
+    int groups = 0;
+    for (int j = 0; j < k; ++j)
+      if (j == 0 || a.move[j].group != a.move[j - 1].group) a.first[groups++] = static_cast<short>(j);
+    a.first[groups] = static_cast<short>(k);
+    for (int j = 0; j < n_pools; j += kMovePools) {
+      const int m = std::min(kMovePools, n_pools - j);
+      for (int p = 0; p < m; ++p) a.pool[p] = static_cast<char*>(const_cast<void*>(pools[j + p]));
+      const dim3 grid((a.pieces + 127) / 128, static_cast<unsigned>(groups), static_cast<unsigned>(m));
+      if (wide) hipLaunchKernelGGL(move_rows_kernel<u32x4>, grid, dim3(128), 0, stream, a);
+      else hipLaunchKernelGGL(move_rows_kernel<char>, grid, dim3(128), 0, stream, a);
+    }
+  }
+  return hipGetLastError();
+}
+
 hipError_t launch_copies(const void* const* pools, int n_pools, long long bytes, long long stride,
                          const PageCopy* pairs, int n, hipStream_t stream) {
   CopyArgs a;
@@ -1204,6 +1265,23 @@ extern "C" int santa_pages_apply(const santa_pages* p, const void* const* pools,
   }
   if (e == hipSuccess) e = hipGetLastError();
   if (e != hipSuccess) return set_error(SANTA_ERR_HIP, "page update launch failed: %s", hipGetErrorString(e));
+  return clear_error();
+}
+
+extern "C" int santa_pages_apply_moves(const santa_pages* p, const void* const* pools, int n_pools,
+                                       long long page_bytes, long long page_stride, hipStream_t stream) {
+  const int* moves;
+  int n;
+  int rc = paged::check_pools(pools, n_pools, page_bytes, page_stride);
+  if (rc != SANTA_OK) return rc;
+  rc = santa_pages_moves(p, &moves, &n);
+  if (rc != SANTA_OK) return rc;
+  const int page_size = santa_pages_page_size(p);
+  if (page_bytes % page_size != 0)
+    return set_error(SANTA_ERR_INVALID, "a page of %lld bytes is not %d rows", page_bytes, page_size);
+  const hipError_t e = paged::launch_moves(pools, n_pools, page_bytes / page_size, page_stride,
+                                           reinterpret_cast<const RowMove*>(moves), n, stream);
+  if (e != hipSuccess) return set_error(SANTA_ERR_HIP, "row move launch failed: %s", hipGetErrorString(e));
   return clear_error();
 }
 

@@ -32,6 +32,7 @@ struct santa_pages {
   // what the last operation asks of the device
   std::vector<santa::PageCopy> copies;
   std::vector<santa::TableEdit> edits;
+  std::vector<santa::RowMove> moves;
   bool remap = false;
 
   int num_pages() const { return static_cast<int>(refs.size()); }
@@ -67,6 +68,7 @@ struct santa_pages {
   void begin() {
     copies.clear();
     edits.clear();
+    moves.clear();
     remap = false;
   }
   bool alive(int s) const { return s >= 0 && s < static_cast<int>(seqs.size()) && seqs[s].len >= 0; }
@@ -179,6 +181,14 @@ int extend(santa_pages* p, const int* seqs, const int* tokens, int n) {
   return SANTA_OK;
 }
 
+// A sequence's last tokens leave it.
+void shrink(santa_pages* p, int seq, int tokens) {
+  santa_pages::Seq& s = p->seqs[seq];
+  s.len -= tokens;
+  for (const size_t pages = static_cast<size_t>(p->pages_for(s.len)); s.pages.size() > pages; s.pages.pop_back())
+    p->drop(s.pages.back());
+}
+
 // The n free rows of the lowest numbers, as empty sequences.
 int new_rows(santa_pages* p, int n, int* out) {
   int got = 0;
@@ -265,14 +275,59 @@ extern "C" int santa_pages_shrink(santa_pages* p, const int* seqs, const int* to
     if (tokens[i] < 0 || tokens[i] > p->seqs[seqs[i]].len)
       return set_error(SANTA_ERR_INVALID, "%d tokens cannot leave sequence %d, which holds %d", tokens[i], seqs[i],
                        p->seqs[seqs[i]].len);
-  for (int i = 0; i < n; ++i) {
-    santa_pages::Seq& s = p->seqs[seqs[i]];
-    s.len -= tokens[i];
-    for (const size_t pages = static_cast<size_t>(p->pages_for(s.len)); s.pages.size() > pages; s.pages.pop_back())
-      p->drop(s.pages.back());
-  }
+  for (int i = 0; i < n; ++i) shrink(p, seqs[i], tokens[i]);
   return clear_error();
 }
+
+extern "C" int santa_pages_keep(santa_pages* p, const int* seqs, const int* new_tokens, const int* kept,
+                                const int* counts, int n) {
+  if (!p || (n > 0 && (!new_tokens || !counts || !kept)))
+    return set_error(SANTA_ERR_INVALID, "bad santa_pages_keep arguments");
+  return guarded([&] {
+    p->begin();
+    const int rc = check_seqs(p, seqs, n);
+    if (rc != SANTA_OK) return rc;
+    std::vector<santa::RowMove> moves;
+    const int* at = kept;
+    int groups = 0;
+    for (int i = 0; i < n; at += counts[i++]) {
+      const santa_pages::Seq& s = p->seqs[seqs[i]];
+      if (new_tokens[i] < 0 || new_tokens[i] > s.len)
+        return set_error(SANTA_ERR_INVALID, "sequence %d holds %d tokens; got %d new ones", seqs[i], s.len,
+                         new_tokens[i]);
+      if (counts[i] < 0 || counts[i] > new_tokens[i])
+        return set_error(SANTA_ERR_INVALID, "%d of %d new tokens cannot stay", counts[i], new_tokens[i]);
+      const int base = s.len - new_tokens[i];
+      const size_t before = moves.size();
+      for (int j = 0; j < counts[i]; ++j)
+        if (at[j] < 0 || at[j] >= new_tokens[i] || (j > 0 && at[j] <= at[j - 1]))
+          return set_error(SANTA_ERR_INVALID, "sequence %d: the new tokens that stay are named in ascending order, by "
+                           "numbers below %d", seqs[i], new_tokens[i]);
+      for (int j = 0; j < counts[i]; ++j) {
+        if (at[j] == j) continue;
+        const int from = base + at[j], to = base + j, page = s.pages[static_cast<size_t>(to / p->page_size)];
+        if (p->refs[page] > 1)
+          return set_error(SANTA_ERR_INVALID, "other sequences hold new tokens of sequence %d", seqs[i]);
+        moves.push_back({s.pages[static_cast<size_t>(from / p->page_size)], from % p->page_size, page,
+                         to % p->page_size, groups});
+      }
+      if (moves.size() > before) ++groups;
+    }
+    for (int i = 0; i < n; ++i) shrink(p, seqs[i], new_tokens[i] - counts[i]);
+    p->moves.swap(moves);
+    return clear_error();
+  });
+}
+
+extern "C" int santa_pages_moves(const santa_pages* p, const int** moves, int* n) {
+  static_assert(sizeof(santa::RowMove) == 5 * sizeof(int), "packed");
+  if (!p || !moves || !n) return set_error(SANTA_ERR_INVALID, "null pointer argument");
+  *moves = reinterpret_cast<const int*>(p->moves.data());
+  *n = static_cast<int>(p->moves.size());
+  return clear_error();
+}
+
+extern "C" int santa_pages_page_size(const santa_pages* p) { return p ? p->page_size : -1; }
 
 extern "C" int santa_pages_fork(santa_pages* p, int seq, int n, int* seqs) {
   if (!p || n < 0 || (n > 0 && !seqs)) return set_error(SANTA_ERR_INVALID, "bad santa_pages_fork arguments");

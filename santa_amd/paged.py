@@ -63,6 +63,9 @@ def _lib():
         L.santa_pages_add.argtypes = [_P, _IP, _I, _IP]
         L.santa_pages_extend.argtypes = [_P, _IP, _IP, _I]
         L.santa_pages_shrink.argtypes = [_P, _IP, _IP, _I]
+        L.santa_pages_keep.argtypes = [_P, _IP, _IP, _IP, _IP, _I]
+        L.santa_pages_moves.argtypes = [_P, ctypes.POINTER(_IP), _IP]
+        L.santa_pages_apply_moves.argtypes = [_P, ctypes.POINTER(_P), _I, _L, _L, _P]
         L.santa_pages_fork.argtypes = [_P, _I, _I, _IP]
         L.santa_pages_free.argtypes = [_P, _IP, _I]
         L.santa_pages_compact.argtypes = [_P]
@@ -218,6 +221,31 @@ class PagedKVCache:
         """Those many last tokens, whose K and V were never written, leave the
         sequences again (a last page that extend() copied stays theirs)."""
         _check(_lib().santa_pages_shrink(self._pages, _ints(seqs), _ints(tokens), len(seqs)))
+
+    def keep(self, seqs: Sequence[int], new_tokens: Union[int, Sequence[int]], kept: Sequence[Sequence[int]]) -> None:
+        """Of the last new_tokens tokens of each sequence (drafted ones) those stay
+        that kept names by their numbers among them, ascending, moved up behind
+        the tokens before them in every layer; the others leave the sequence,
+        which gives up the pages behind.  Tokens that move must not be held by
+        other sequences too."""
+        seqs = _int_list(seqs, "seqs")
+        new = [new_tokens] * len(seqs) if isinstance(new_tokens, int) else _int_list(new_tokens, "new_tokens")
+        kept = [_int_list(k, "kept") for k in kept]
+        if len(new) != len(seqs) or len(kept) != len(seqs):
+            raise ValueError(f"new_tokens and kept must have one entry per sequence ({len(seqs)})")
+        self._may_change()
+        _check(_lib().santa_pages_keep(self._pages, _ints(seqs), _ints(new), _ints([i for k in kept for i in k]),
+                                       _ints([len(k) for k in kept]), len(seqs)))
+        if self.device.type == "cuda":
+            _launch(self.device, _lib().santa_pages_apply_moves, self._pages, self._pools, len(self._pools),
+                    self._page_bytes, self._page_bytes)
+            return
+        moves, n = _IP(), ctypes.c_int()
+        _check(_lib().santa_pages_moves(self._pages, ctypes.byref(moves), ctypes.byref(n)))
+        if n.value:
+            page, row, to_page, to_row, _ = torch.tensor(moves[:5 * n.value]).view(-1, 5).t()
+            for t in (*self.k, *self.v):
+                t[to_page, to_row] = t[page, row]
 
     def fork(self, seq: int, n: int = 1) -> List[int]:
         """n new sequences with the same tokens, which hold the same pages."""
