@@ -62,7 +62,11 @@ extern "C" {
 
 /* Element type of q, K, V and out (the reference accepts bf16 or f16,
  * flash/santa_cuda.cpp:128-133). */
-enum santa_dtype { SANTA_BF16 = 0, SANTA_F16 = 1 };
+enum santa_dtype {
+  SANTA_BF16 = 0,
+  SANTA_F16 = 1,
+  SANTA_F32 = 2 /* where an entry says so */
+};
 
 /* Return codes.  On failure santa_last_error() holds a message whose text
  * follows the reference's TORCH_CHECK messages where one exists. */
@@ -481,6 +485,24 @@ int santa_paged_rope_append(const void* qkv, const void* cos_, const void* sin_,
                             void* v_pages, int dtype, int D, int num_pages, int page_size, const long long* strides,
                             const int* table, long long table_stride, int table_rows,
                             const santa_paged_plan_info* info, const int* plan, hipStream_t stream);
+
+/* The same for heads that are normed first, and rotated in part or in the other
+ * layout: with q_norm, k_norm (NULL: none; q_norm_heads rows of D, one or H, and
+ * k_norm_heads, one or KVH), x / sqrt(mean(x^2) + eps) * w over the D dims of every q
+ * and k head; then a rotation of its first R dims, R even, by cos_, sin_ [tokens, R]:
+ * dims d and d + R / 2 or, interleaved, 2d and 2d + 1 belong together.  float32,
+ * rounded once.  D up to 512. */
+int santa_paged_heads_append(const void* qkv, const void* cos_, const void* sin_, int R, int interleaved,
+                             const void* q_norm, int q_norm_heads, const void* k_norm, int k_norm_heads, float eps,
+                             void* q_out, void* k_pages, void* v_pages, int dtype, int D, int num_pages, int page_size,
+                             const long long* strides, const int* table, long long table_stride, int table_rows,
+                             const santa_paged_plan_info* info, const int* plan, hipStream_t stream);
+/* magnitude times cos and sin of 2 pi x positions[i * stride] x turns[p], i < n, p <
+ * pairs (up to 256; turns: host array, read before the call returns), to dims p and
+ * p + pairs of cos_, sin_ [n, 2 pairs] or, interleaved, 2p and 2p + 1.  positions: int
+ * or, wide, 64-bit.  dtype: bf16, f16 or float32.  Angles in float64. */
+int santa_rope_tables(const void* positions, int wide, long long stride, long long n, const double* turns, int pairs,
+                      float magnitude, int interleaved, int dtype, void* cos_, void* sin_, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,6 +1,8 @@
 // santa_paged.h -- what the planner (santa_paged_plan.cpp) and the kernels
-// (santa_paged.hip) of the paged attention agree on.
+// (santa_paged.hip, santa_rotary.hip) of the paged attention agree on.
 #pragma once
+
+#include "santa_amd.h"
 
 namespace santa {
 namespace paged {
@@ -34,6 +36,22 @@ struct Item {
 };
 constexpr int kItemInts = 16;
 static_assert(sizeof(Item) == kItemInts * sizeof(int), "packed");
+
+// Strides in elements of a pool: pages, rows, heads.
+struct PoolStrides {
+  long long page, row, head;
+};
+
+struct Pages {
+  const int* table;
+  long long stride;  // entries per row
+  int shift, num_pages;
+};
+
+// A block table, pools and plan that belong together.
+int check_paged(const void* q, const void* k, const void* v, const void* out, int dtype, int num_pages, int page_size,
+                const long long* strides, int n_strides, const int* table, long long table_stride, int table_rows,
+                const santa_paged_plan_info* info, const int* plan, const char* what, Pages* pg);
 
 }  // namespace paged
 }  // namespace santa

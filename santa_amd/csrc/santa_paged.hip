@@ -186,17 +186,6 @@ int check_pools(const void* const* pools, int n_pools, long long bytes, long lon
 }
 
 // -------------------------------------------------------------------- append
-// Strides in elements of a pool: pages, rows, heads.
-struct PoolStrides {
-  long long page, row, head;
-};
-
-struct Pages {
-  const int* table;
-  long long stride;  // entries per row
-  int shift, num_pages;
-};
-
 __device__ __forceinline__ int in_pool(const Pages& pg, int page) { return min(max(page, 0), pg.num_pages - 1); }
 
 // y_d = x_d cos_d - x_{d + D/2} sin_d and y_{d + D/2} = x_{d + D/2} cos_{d + D/2}
@@ -1168,7 +1157,6 @@ __global__ __launch_bounds__(256) void merge_kernel(const float* __restrict__ pa
       pack4<BF16>(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv);
 }
 
-// A block table, pools and plan that belong together.
 int check_paged(const void* q, const void* k, const void* v, const void* out, int dtype, int num_pages, int page_size,
                 const long long* strides, int n_strides, const int* table, long long table_stride, int table_rows,
                 const santa_paged_plan_info* info, const int* plan, const char* what, Pages* pg) {

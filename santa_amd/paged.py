@@ -29,14 +29,16 @@ not take (float32, head_dim other than 64 and 128, autograd).
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
+from dataclasses import dataclass
 from typing import Iterable, List, Optional, Sequence, Tuple, Union
 
 import torch
 
 from .runtime import _FusedOps, _plain
 
-__all__ = ["PagedKVCache", "PagedPlan", "paged_attention", "rope_append", "copy_pages"]
+__all__ = ["PagedKVCache", "PagedPlan", "RopeScaling", "paged_attention", "rope_append", "rope_tables", "copy_pages"]
 
 _P, _I, _L = ctypes.c_void_p, ctypes.c_int, ctypes.c_longlong
 _IP = ctypes.POINTER(ctypes.c_int)
@@ -83,6 +85,10 @@ def _lib():
         L.santa_paged_attention.argtypes = [_P] * 4 + [_I] * 4 + [ctypes.POINTER(_L), _P, _L, _I, info, _P,
                                                                   ctypes.c_float, _P, ctypes.c_size_t, _P]
         L.santa_paged_rope_append.argtypes = [_P] * 6 + [_I] * 4 + [ctypes.POINTER(_L), _P, _L, _I, info, _P, _P]
+        L.santa_paged_heads_append.argtypes = [_P] * 3 + [_I, _I, _P, _I, _P, _I, ctypes.c_float] + [_P] * 3 + [
+            _I] * 4 + [ctypes.POINTER(_L), _P, _L, _I, info, _P, _P]
+        L.santa_rope_tables.argtypes = [_P, _I, _L, _L, ctypes.POINTER(ctypes.c_double), _I, ctypes.c_float, _I, _I, _P,
+                                        _P, _P]
         _lib_ready = L
     return _lib_ready
 
@@ -647,28 +653,50 @@ def _token_slots(block_table, plan: PagedPlan, page_size: int):
     return token, block_table[seq, pos // page_size].long() * page_size + pos % page_size
 
 
+def _norm(w: Optional[torch.Tensor], heads: int, what: str, like: torch.Tensor) -> Optional[torch.Tensor]:
+    """A norm's weights as [1, D] or [heads, D]."""
+    if w is None:
+        return None
+    D = like.shape[2]
+    if w.shape not in ((D,), (heads, D)):
+        raise ValueError(f"{what} must be [{D}] or [{heads}, {D}]; got {tuple(w.shape)}")
+    if w.device != like.device or w.dtype != like.dtype:
+        raise ValueError(f"{what} must have the device and dtype of qkv")
+    return w.view(1, D) if w.dim() == 1 else w
+
+
 def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
-                block_table: torch.Tensor, plan: PagedPlan) -> torch.Tensor:
+                block_table: torch.Tensor, plan: PagedPlan, *, q_norm: Optional[torch.Tensor] = None,
+                k_norm: Optional[torch.Tensor] = None, eps: float = 1e-6, interleaved: bool = False) -> torch.Tensor:
     """RoPE of the batch's tokens with their write into pages: qkv [tokens, H +
-    2 KVH, D], cos and sin [tokens, D] (rotate-half convention).  The k heads
-    are rotated and written to k_pages, the v heads to v_pages, at the tokens'
-    positions; returns the rotated q heads [tokens, H, D].  float32 arithmetic,
-    rounded once.  Two tokens of one position and page (sequences that share a
-    page they write to) leave one of the two there: ``PagedKVCache.extend``
-    gives every sequence its own."""
+    2 KVH, D], cos and sin [tokens, R], R even and at most D: the first R dims of
+    a head are rotated, dims d and d + R / 2 together (rotate-half convention) or,
+    interleaved, 2d and 2d + 1.  The k heads are rotated and written to k_pages,
+    the v heads to v_pages, at the tokens' positions; returns the rotated q heads
+    [tokens, H, D].  q_norm, k_norm: weights [D], or [H, D] and [KVH, D], of an
+    RMS norm of each q and k head before its rotation, x / sqrt(mean(x^2) + eps) *
+    weight.  float32 arithmetic, rounded once.  Two tokens of one position and page
+    (sequences that share a page they write to) leave one of the two there:
+    ``PagedKVCache.extend`` gives every sequence its own."""
     if qkv.dim() != 3 or qkv.shape[:2] != (plan.tokens, plan.heads + 2 * plan.kv_heads):
         raise ValueError(f"qkv must be [{plan.tokens}, {plan.heads + 2 * plan.kv_heads}, D]; got {tuple(qkv.shape)}")
     D, H, KVH = qkv.shape[2], plan.heads, plan.kv_heads
     _check_pools(k_pages, v_pages, block_table, plan, qkv)
     if k_pages.shape[3] != D:
         raise ValueError(f"D mismatch: qkv {D}, pages {k_pages.shape[3]}")
-    if D % 2 or cos.shape != (plan.tokens, D) or sin.shape != cos.shape:
-        raise ValueError(f"cos and sin must be [{plan.tokens}, D], D even")
+    R = cos.shape[1] if cos.dim() == 2 else -1
+    if cos.shape != (plan.tokens, R) or sin.shape != cos.shape or R % 2 or not 0 < R <= D:
+        raise ValueError(f"cos and sin must be [{plan.tokens}, R], R even and at most {D}")
     device, dtype = qkv.device, qkv.dtype
     if cos.device != device or sin.device != device or cos.dtype != dtype or sin.dtype != dtype:
         raise ValueError("cos and sin must have the device and dtype of qkv")
-    if (device.type == "cuda" and dtype in (torch.bfloat16, torch.float16) and D % 16 == 0
-            and _plain(qkv, cos, sin, k_pages, v_pages)):
+    q_norm, k_norm, eps = _norm(q_norm, H, "q_norm", qkv), _norm(k_norm, KVH, "k_norm", qkv), float(eps)
+    if not 0.0 <= eps < math.inf:
+        raise ValueError(f"eps must be at least 0 and finite; got {eps}")
+    norms = [w for w in (q_norm, k_norm) if w is not None]
+    plain = R == D and not norms and not interleaved
+    if (device.type == "cuda" and dtype in (torch.bfloat16, torch.float16) and D % 16 == 0 and (plain or D <= 512)
+            and _plain(qkv, cos, sin, k_pages, v_pages, *norms)):
         strides = (*_strides(k_pages, "k_pages"), *_strides(v_pages, "v_pages"))
         if _overlaps(k_pages) or _overlaps(v_pages):
             raise ValueError("rows of pages that are written must not overlap")
@@ -677,21 +705,140 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages
         table, row = _table_rows(block_table)
         if plan.tokens:
             plan._used()
-            _launch(device, _lib().santa_paged_rope_append, qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(),
-                    q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), int(dtype == torch.float16), D,
-                    k_pages.shape[0], k_pages.shape[1], (_L * 6)(*strides), table.data_ptr(), row, table.shape[0],
+            rest = (k_pages.data_ptr(), v_pages.data_ptr(), int(dtype == torch.float16), D, k_pages.shape[0],
+                    k_pages.shape[1], (_L * 6)(*strides), table.data_ptr(), row, table.shape[0],
                     ctypes.byref(plan._info), plan._data.data_ptr())
+            if plain:
+                _launch(device, _lib().santa_paged_rope_append, qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+                        q.data_ptr(), *rest)
+            else:
+                q_norm, k_norm = (w if w is None else _packed(w) for w in (q_norm, k_norm))
+                weights = [x for w in (q_norm, k_norm) for x in ((None, 1) if w is None else (w.data_ptr(), len(w)))]
+                _launch(device, _lib().santa_paged_heads_append, qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), R,
+                        int(interleaved), *weights, eps, q.data_ptr(), *rest)
             plan._captured(block_table.shape[1] * k_pages.shape[1], True)
         return q
     wide = torch.float64 if qkv.dtype == torch.float64 else torch.float32
     x, c, s = qkv[:, :H + KVH].to(wide), cos.to(wide)[:, None], sin.to(wide)[:, None]
-    turned = (x * c + torch.cat([-x[..., D // 2:], x[..., :D // 2]], dim=-1) * s).to(qkv.dtype)
+    if norms:
+        normed = x * torch.rsqrt(x.square().mean(-1, keepdim=True) + eps)
+        x = torch.cat([part if w is None else n * w.to(wide)
+                       for part, n, w in ((x[:, :H], normed[:, :H], q_norm), (x[:, H:], normed[:, H:], k_norm))], 1)
+    y = x[..., :R]
+    if interleaved:
+        other = torch.stack([-y[..., 1::2], y[..., ::2]], -1).flatten(-2)
+    else:
+        other = torch.cat([-y[..., R // 2:], y[..., :R // 2]], dim=-1)
+    turned = torch.cat([y * c + other * s, x[..., R:]], -1).to(qkv.dtype)
     token, slot = _token_slots(block_table, plan, k_pages.shape[1])
     page, row = slot // k_pages.shape[1], slot % k_pages.shape[1]
     k_pages[page, row] = turned[token, H:]
     v_pages[page, row] = qkv[token, H + KVH:]
     plan._captured(0, False)
     return turned[:, :H]
+
+
+# ---------------------------------------------------------------- positions
+@dataclass(frozen=True)
+class RopeScaling:
+    """How the frequencies theta^(-2i / dim) of rotary positions are scaled for
+    contexts `factor` times as long as the original_len tokens that a model was
+    trained on:
+
+    * "linear": all by 1 / factor (position interpolation);
+    * "ntk": through the base, theta factor^(dim / (dim - 2)), so that the lowest
+      one shrinks by the factor and the highest one stays;
+    * "llama3": by 1 / factor where a pair makes fewer than `low` turns over
+      original_len, not at all above `high` turns, and by a share that is linear in
+      the turns between (Llama 3.1);
+    * "yarn": by 1 / factor from the pair of `low` turns on, not at all up to the
+      pair of `high` turns, and by a share that is linear in the pair's number between,
+      with cos and sin `magnitude` times as large, 0.1 ln(factor) + 1 by default
+      (YaRN).
+
+    low and high: 1 and 4 (llama3) or 1 and 32 (yarn) by default."""
+
+    kind: str
+    factor: float
+    original_len: int = 8192
+    low: Optional[float] = None
+    high: Optional[float] = None
+    magnitude: Optional[float] = None
+
+    def __post_init__(self):
+        if self.kind not in ("linear", "ntk", "llama3", "yarn"):
+            raise ValueError(f"kind must be linear, ntk, llama3 or yarn; got {self.kind!r}")
+        if not 0.0 < self.factor < math.inf or self.original_len <= 0:
+            raise ValueError("factor and original_len must be positive")
+        low, high = self._turns()
+        if not 0.0 < low < high < math.inf:
+            raise ValueError("low and high must be positive, low below high")
+        if self.magnitude is not None and not math.isfinite(self.magnitude):
+            raise ValueError("magnitude must be finite")
+
+    def _turns(self) -> Tuple[float, float]:
+        return (1.0 if self.low is None else self.low,
+                (32.0 if self.kind == "yarn" else 4.0) if self.high is None else self.high)
+
+    def frequencies(self, dim: int, theta: float) -> Tuple[List[float], float]:
+        """(Angle per position of each pair of dim rotated dims, magnitude)."""
+        if self.kind == "ntk":
+            if dim <= 2:
+                raise ValueError("the base scales more than two dims")
+            theta = theta * self.factor ** (dim / (dim - 2))
+        f = [theta ** (-2.0 * i / dim) for i in range(dim // 2)]
+        magnitude = 1.0 if self.magnitude is None else self.magnitude
+        if self.kind == "ntk":
+            return f, magnitude
+        low, high = self._turns()
+        if self.kind == "linear":
+            left = [0.0] * len(f)  # the share that is not scaled
+        elif self.kind == "llama3":
+            left = [(self.original_len * x / (2 * math.pi) - low) / (high - low) for x in f]
+        else:
+            at = [dim * math.log(self.original_len / (t * 2 * math.pi)) / (2 * math.log(theta)) for t in (high, low)]
+            first, last = max(math.floor(at[0]), 0), min(math.ceil(at[1]), dim - 1)
+            left = [1.0 - (i - first) / max(last - first, 0.001) for i in range(len(f))]
+            if self.magnitude is None:
+                magnitude = 0.1 * math.log(self.factor) + 1.0 if self.factor > 1.0 else 1.0
+        left = [min(max(x, 0.0), 1.0) for x in left]
+        return [x / self.factor * (1.0 - s) + x * s for x, s in zip(f, left)], magnitude
+
+
+@functools.lru_cache(maxsize=64)
+def _frequencies(dim: int, theta: float, scaling: Optional[RopeScaling]):
+    """(Angles per position, the same in turns as a C array, magnitude)."""
+    f, magnitude = ([theta ** (-2.0 * i / dim) for i in range(dim // 2)], 1.0) if scaling is None else \
+        scaling.frequencies(dim, theta)
+    return f, (ctypes.c_double * len(f))(*[x / (2 * math.pi) for x in f]), magnitude
+
+
+def rope_tables(positions: torch.Tensor, dim: int, *, theta: float = 10000.0, scaling: Optional[RopeScaling] = None,
+                interleaved: bool = False, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """cos and sin [tokens, dim] of integer positions [tokens] (``plan.positions``)
+    for ``rope_append``: the angle positions x theta^(-2i / dim), scaled as
+    `scaling` says, in dims i and i + dim / 2 or, interleaved, 2i and 2i + 1.  dim:
+    the number of rotated dims, even.  Angles are float64: far positions lose nothing."""
+    if positions.dim() != 1 or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError("positions must be [tokens] of int32 or int64")
+    if dim <= 0 or dim % 2:
+        raise ValueError(f"dim must be even and positive; got {dim}")
+    if not 1.0 < theta < math.inf:
+        raise ValueError(f"theta must be above 1 and finite; got {theta}")
+    if not dtype.is_floating_point:
+        raise ValueError("the tables have a floating point dtype")
+    f, turns, magnitude = _frequencies(int(dim), float(theta), scaling)
+    device = positions.device
+    kind = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}.get(dtype)
+    if device.type == "cuda" and kind is not None and dim <= 512 and _plain(positions):
+        cos, sin = (torch.empty(len(positions), dim, dtype=dtype, device=device) for _ in range(2))
+        _launch(device, _lib().santa_rope_tables, positions.data_ptr(), int(positions.dtype == torch.int64),
+                positions.stride(0), len(positions), turns, len(f), magnitude, int(interleaved), kind, cos.data_ptr(),
+                sin.data_ptr())
+        return cos, sin
+    angle = positions.to(torch.float64)[:, None] * torch.tensor(f, dtype=torch.float64, device=device)
+    angle = angle.repeat_interleave(2, -1) if interleaved else torch.cat([angle, angle], -1)
+    return (angle.cos() * magnitude).to(dtype), (angle.sin() * magnitude).to(dtype)
 
 
 # ---------------------------------------------------------------- attention
