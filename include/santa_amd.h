@@ -504,6 +504,51 @@ int santa_paged_heads_append(const void* qkv, const void* cos_, const void* sin_
 int santa_rope_tables(const void* positions, int wide, long long stride, long long n, const double* turns, int pairs,
                       float magnitude, int interleaved, int dtype, void* cos_, void* sin_, hipStream_t stream);
 
+/* ----------------------------------------------------------- rules on logits */
+
+/* What santa_adjust_logits applies to row r of sequence s (the block table row that
+ * a plan's token r belongs to; without a plan s = r).  NULL pointers: not applied.
+ *   tokens [tokens_rows, tokens_len] (int, or 64-bit where tokens_wide; rows
+ *     tokens_stride entries apart): the tokens of every sequence.  A row has seen
+ *     those that its token of the plan attends to.
+ *   prompts[s]: how many of a sequence's first tokens are its prompt's (NULL: 0);
+ *     the others and all drafted ones are the answer's.
+ *   repetition, frequency, presence: [s], or where NULL the values _all.
+ *   bias_ids, bias: biases entries of sequence s from entry s * bias_stride on (0:
+ *     the same for all); ids outside of the vocabulary count for nothing, and of a
+ *     token named twice the last entry counts.  Up to 2046.
+ *   allowed: bit v % 32 of int r * allowed_stride + v / 32 (0: the same for all rows):
+ *     whether token v may come. */
+typedef struct santa_logit_rules {
+  const void* tokens;
+  int tokens_wide, tokens_rows, tokens_len;
+  long long tokens_stride;
+  const int* prompts;
+  const float *repetition, *frequency, *presence;
+  float repetition_all, frequency_all, presence_all;
+  const int* bias_ids;
+  const float* bias;
+  int biases;
+  long long bias_stride;
+  const int* allowed;
+  long long allowed_stride;
+} santa_logit_rules;
+
+/* Row by row of x [N, V] (bf16, f16 or float32, rows stride elements apart), in
+ * float32: a token that the row has seen has its logit divided by the repetition
+ * penalty where it is positive and multiplied by it elsewhere; one that is in the
+ * answer c > 0 times loses c times the frequency penalty and once the presence
+ * penalty; then the bias is added; one that may not come is -inf.  Either out [N, V]
+ * (float32, contiguous) is written or token [N]: the index of the row's maximum, NaN
+ * above any number, the first one among equal values.  info, plan: those of a
+ * santa_paged_plan of N tokens, or NULL.  At most 2^20 - 1 tokens are counted.
+ * workspace (for token): santa_adjust_logits_workspace_size bytes, 8-byte aligned,
+ * no initialization needed. */
+size_t santa_adjust_logits_workspace_size(int N, int V);
+int santa_adjust_logits(const void* x, int dtype, long long stride, int N, int V, const santa_logit_rules* rules,
+                        const santa_paged_plan_info* info, const int* plan, float* out, long long* token,
+                        void* workspace, size_t workspace_bytes, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

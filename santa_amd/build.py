@@ -35,7 +35,7 @@ HIPCC = os.path.join(ROCM, "bin", "hipcc")
 ARCH = "gfx950"
 
 HIP_SOURCES = ["santa_flash.hip", "santa_prop.hip", "santa_prop_gen.hip", "santa_runtime.hip", "santa_attn.hip",
-               "santa_paged.hip", "santa_rotary.hip"]
+               "santa_paged.hip", "santa_rotary.hip", "santa_logits.hip"]
 CXX_SOURCES = ["santa_common.cpp", "santa_pages.cpp", "santa_paged_plan.cpp"]
 EXTENSIONS = {"santa_flash_batch_cuda": "ext_flash.cpp", "santa_prop_batch_cuda": "ext_prop.cpp"}
 
