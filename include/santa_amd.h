@@ -437,7 +437,7 @@ int santa_paged_plan(const int* lens, const int* new_tokens, const int* rows, in
                      const int* shared, int n_groups, int heads, int kv_heads, int fixed, santa_paged_plan_info* info,
                      int* plan, long long plan_ints);
 /* The same where the new tokens of sequences b with trees[b] != 0 are drafts that
- * follow one another as trees, up to 1024 each: parents (one int per new token of
+ * follow one another as trees, up to 8192 each: parents (one int per new token of
  * the batch, those of other sequences not read) names the earlier new token of the
  * sequence that a token follows, -1: the context (the tokens before the new ones),
  * -2: not in use, and followed by none.  A token attends to the context, the

@@ -21,7 +21,7 @@ enum ItemFlags {
 // multiple of 64 up to the context's end on: whether it attends to that token.
 // Records of the plan's other tokens say the same (no bits beyond the context).
 constexpr int kTreeWords = 2;  // where the bits begin
-constexpr int kMostDrafts = 1024;
+constexpr int kMostDrafts = 8192;
 
 // What one workgroup per KV head does: rows r < rows, row r being query head
 // r % GH of token tok0 + r / GH, over the tokens begin .. end - 1 (begin a

@@ -400,7 +400,7 @@ class PagedPlan:
     once for all, through the row of one of them.
 
     parents: for new tokens that are drafts and follow one another as trees, one
-    entry per sequence: None, or for each of its new tokens (at most 1024) the
+    entry per sequence: None, or for each of its new tokens (at most 8192) the
     earlier one of them that it follows, -1: the context (the tokens before the
     new ones), -2: not in use.  A drafted token attends to the context, the drafted
     tokens that it follows up to there, and itself, and its position is the one

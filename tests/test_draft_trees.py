@@ -202,9 +202,9 @@ def test_refusals():
     for parents in ([[-1, 0]], [[-1, 0, 0], None], [[-1, 0, 0.5]], [5], [None, None]):
         with pytest.raises((ValueError, TypeError)):
             make(parents)
-    assert make([list(range(-1, 1023))], 1024, 2000).tokens == 1024
-    with pytest.raises(RuntimeError, match="up to 1024"):
-        make([list(range(-1, 1024))], 1025, 2000)
+    assert make([list(range(-1, 8191))], 8192, 9000).tokens == 8192
+    with pytest.raises(RuntimeError, match="up to 8192"):
+        make([list(range(-1, 8192))], 8193, 9000)
     with pytest.raises(RuntimeError, match="beside trees"):
         PagedPlan([2000, 1 << 21], heads=1, kv_heads=1, new_tokens=[1024, 1 << 21], device="cpu",
                   parents=[[-1] * 1024, None])

@@ -64,7 +64,7 @@ CASES = [
     ([700, 20, 0], [16, 16, 16], (), 0.2, [], 4, 2, 128, 32, BF), ([1000], [8], (), 0.0, [], 32, 8, 128, 16, BF),
     ([500, 400], [12, 5], (1,), 0.0, [], 40, 1, 64, 16, F16), ([300, 65], [64, 64], (), 0.1, [], 4, 1, 128, 256, BF),
     ([300, 200], [65, 130], (), 0.1, [], 2, 1, 64, 8, BF), ([1500], [200], (), 0.3, [], 7, 1, 128, 64, F16),
-    ([900, 70], [64, 64], (), 0.05, [], 64, 8, 128, 16, BF), ([2100], [1024], (), 0.2, [], 1, 1, 64, 16, BF),
+    ([900, 70], [64, 64], (), 0.05, [], 64, 8, 128, 16, BF), ([2100], [1024], (), 0.2, [], 1, 1, 64, 16, BF), ([2500], [2400], (), 0.1, [], 2, 1, 64, 32, BF),
     # prefixes: a group's members with trees and without, tokens not in use in front of shared pages
     ([400, 390, 380, 100], [3, 5, 7, 2], (2,), 0.2, [([2, 0, 1], 320)], 4, 1, 64, 32, F16),
     ([300, 200, 310, 250, 99], [9, 1, 30, 4, 8], (), 0.3, [([3, 0], 200), ([1, 4, 2], 80)], 28, 4, 128, 8, BF),
