@@ -532,6 +532,7 @@ typedef struct santa_logit_rules {
   long long bias_stride;
   const int* allowed;
   long long allowed_stride;
+  int sequences; /* how many sequences the rows are of, 0: as many as rows; how the work is cut up goes by it */
 } santa_logit_rules;
 
 /* Row by row of x [N, V] (bf16, f16 or float32, rows stride elements apart), in
@@ -541,10 +542,10 @@ typedef struct santa_logit_rules {
  * penalty; then the bias is added; one that may not come is -inf.  Either out [N, V]
  * (float32, contiguous) is written or token [N]: the index of the row's maximum, NaN
  * above any number, the first one among equal values.  info, plan: those of a
- * santa_paged_plan of N tokens, or NULL.  At most 2^20 - 1 tokens are counted.
- * workspace (for token): santa_adjust_logits_workspace_size bytes, 8-byte aligned,
- * no initialization needed. */
-size_t santa_adjust_logits_workspace_size(int N, int V);
+ * santa_paged_plan of N tokens, or NULL.  At most 2^19 - 1 tokens are counted.
+ * workspace (for token): santa_adjust_logits_workspace_size bytes for these N, V and
+ * rules->sequences, 8-byte aligned, no initialization needed. */
+size_t santa_adjust_logits_workspace_size(int N, int V, int sequences);
 int santa_adjust_logits(const void* x, int dtype, long long stride, int N, int V, const santa_logit_rules* rules,
                         const santa_paged_plan_info* info, const int* plan, float* out, long long* token,
                         void* workspace, size_t workspace_bytes, hipStream_t stream);

@@ -34,7 +34,7 @@ class _Rules(ctypes.Structure):
     _fields_ = [("tokens", _P), ("tokens_wide", _I), ("tokens_rows", _I), ("tokens_len", _I), ("tokens_stride", _L),
                 ("prompts", _P), ("repetition", _P), ("frequency", _P), ("presence", _P), ("repetition_all", _F),
                 ("frequency_all", _F), ("presence_all", _F), ("bias_ids", _P), ("bias", _P), ("biases", _I),
-                ("bias_stride", _L), ("allowed", _P), ("allowed_stride", _L)]
+                ("bias_stride", _L), ("allowed", _P), ("allowed_stride", _L), ("sequences", _I)]
 
 
 _lib_ready = None
@@ -44,7 +44,7 @@ def _lib():
     global _lib_ready
     if _lib_ready is None:
         L = _FusedOps.lib()
-        L.santa_adjust_logits_workspace_size.argtypes = [_I, _I]
+        L.santa_adjust_logits_workspace_size.argtypes = [_I, _I, _I]
         L.santa_adjust_logits_workspace_size.restype = ctypes.c_size_t
         L.santa_adjust_logits.argtypes = [_P, _I, _L, _I, _I, ctypes.POINTER(_Rules), ctypes.POINTER(_PlanInfo), _P, _P, _P,
                                           _P, ctypes.c_size_t, _P]
@@ -99,7 +99,7 @@ def adjust_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
     ceil(V / 32)], has bit v % 32 of entry v // 32 set where token v may.  Penalties: a
     number, or float32 [sequences] on the device.  Tensors by sequence are read at the
     sequence's row of the block table, like tokens.  Tokens outside of the vocabulary
-    are in no row's way.  At most 2^20 - 1 tokens are counted."""
+    are in no row's way.  At most 2^19 - 1 tokens are counted."""
     if logits.dim() != 2 or not logits.dtype.is_floating_point or logits.shape[1] == 0:
         raise ValueError(f"logits must be [rows, vocabulary] of a floating point dtype; got {tuple(logits.shape)}")
     N, V = logits.shape
@@ -140,8 +140,8 @@ def adjust_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
                 allowed.shape[1] != -(-V // 32):
             raise ValueError(f"allowed must be int32 [1 or {N}, {-(-V // 32)}] on the logits' device")
         allowed, allowed_stride = _rows(allowed, N, "allowed")
-    if plan is not None and tokens is not None and plan._info.max_len >= 1 << 20:
-        raise ValueError(f"at most {(1 << 20) - 1} tokens are counted; got {plan._info.max_len}")
+    if plan is not None and tokens is not None and plan._info.max_len >= 1 << 19:
+        raise ValueError(f"at most {(1 << 19) - 1} tokens are counted; got {plan._info.max_len}")
     kind = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}.get(logits.dtype)
     given = [t for t in (tokens, prompts, *penalties, ids, values, allowed) if isinstance(t, torch.Tensor)]
     if not (device.type == "cuda" and kind is not None
@@ -173,8 +173,10 @@ def adjust_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
         rules.bias_stride = bias_stride
     if allowed is not None:
         rules.allowed, rules.allowed_stride = allowed.data_ptr(), allowed_stride
+    if plan is not None:
+        rules.sequences = len(plan.seq_lens)
     lib = _lib()
-    workspace = torch.empty(lib.santa_adjust_logits_workspace_size(N, V) if greedy else 0, dtype=torch.uint8,
+    workspace = torch.empty(lib.santa_adjust_logits_workspace_size(N, V, rules.sequences) if greedy else 0, dtype=torch.uint8,
                             device=device)
     info, data = (None, None) if plan is None else (ctypes.byref(plan._info), plan._data.data_ptr())
     if plan is not None:
@@ -183,7 +185,7 @@ def adjust_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
             ctypes.byref(rules), info, data, None if greedy else out.data_ptr(), out.data_ptr() if greedy else None,
             workspace.data_ptr(), workspace.numel())
     if plan is not None:
-        plan._captured(1 << 30 if tokens is None else min(tokens.shape[1], (1 << 20) - 1), True)
+        plan._captured(1 << 30 if tokens is None else min(tokens.shape[1], (1 << 19) - 1), True)
     return out
 
 

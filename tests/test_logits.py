@@ -185,7 +185,7 @@ def test_refusals():
         with pytest.raises(ValueError):
             adjust_logits(*args, **more)
     with pytest.raises(ValueError, match="are counted"):
-        adjust_logits(torch.zeros(1, 3), torch.zeros(1, 1).long().expand(1, 1 << 20), [1 << 20])
+        adjust_logits(torch.zeros(1, 3), torch.zeros(1, 1).long().expand(1, 1 << 19), [1 << 19])
 
 
 def test_library_refusals():
@@ -205,4 +205,4 @@ def test_library_refusals():
                      ({"biases": 3}, "bad adjust"), ({"biases": 2047, "bias_ids": 16, "bias": 16}, "up to 2046"),
                      ({"out": None, "token": one, "size": 7}, "workspace"), ({"out": None, "token": one, "ws": None}, "workspace")]:
         assert call(**kw) != 0 and text in error(), (kw, error())
-    assert lib.santa_adjust_logits_workspace_size(4, 128256) >= 32 and lib.santa_adjust_logits_workspace_size(0, 5) == 0
+    assert lib.santa_adjust_logits_workspace_size(4, 128256, 4) >= 32 and lib.santa_adjust_logits_workspace_size(0, 5, 0) == 0
