@@ -500,7 +500,8 @@ int santa_paged_heads_append(const void* qkv, const void* cos_, const void* sin_
 /* magnitude times cos and sin of 2 pi x positions[i * stride] x turns[p], i < n, p <
  * pairs (up to 256; turns: host array, read before the call returns), to dims p and
  * p + pairs of cos_, sin_ [n, 2 pairs] or, interleaved, 2p and 2p + 1.  positions: int
- * or, wide, 64-bit.  dtype: bf16, f16 or float32.  Angles in float64. */
+ * or, wide, 64-bit.  dtype: bf16, f16 or float32; tables 16-byte aligned.  Angles in
+ * float64. */
 int santa_rope_tables(const void* positions, int wide, long long stride, long long n, const double* turns, int pairs,
                       float magnitude, int interleaved, int dtype, void* cos_, void* sin_, hipStream_t stream);
 

@@ -3,6 +3,7 @@
 // and k heads with their rotation, wholly or in part, and the write into pages.
 // No counterpart in the reference, whose models rotate and norm in torch
 // (tutorial_code/runtime_common.py:501-571).
+#include <algorithm>
 #include <cmath>
 
 #include "santa_amd.h"
@@ -33,33 +34,53 @@ __device__ __forceinline__ __bf16 rounded<__bf16>(float x) { return static_cast<
 template <>
 __device__ __forceinline__ _Float16 rounded<_Float16>(float x) { return static_cast<_Float16>(x); }
 
-// cos and sin of pos x f for every (position, pair).  The angle is taken in turns,
+// cos and sin of pos x f for every (position, pair), kMore pairs to a thread (4 where
+// their number allows it: stores of up to 16 bytes).  The angle is taken in turns,
 // in float64, of which the whole ones leave nothing: what remains is rounded to
 // float32 as a part of one turn, at any position.
-template <class T>
+template <class T, int kMore, bool kInterleaved>
 __global__ __launch_bounds__(256) void rope_tables_kernel(const void* __restrict__ positions, int wide,
-                                                          long long stride, Frequencies f, int pairs, int interleaved,
-                                                          T* __restrict__ cos_, T* __restrict__ sin_, uint32_t total) {
-  const uint32_t i = blockIdx.x * 256u + threadIdx.x;
-  if (i >= total) return;
-  const uint32_t row = i / static_cast<uint32_t>(pairs);
-  const int p = static_cast<int>(i % static_cast<uint32_t>(pairs));
-  const long long at = static_cast<long long>(row) * stride;
-  const double pos = wide ? static_cast<double>(static_cast<const long long*>(positions)[at])
-                          : static_cast<double>(static_cast<const int*>(positions)[at]);
-  const double turns = pos * f.turns[p];
-  float s, c;
-  sincospif(2.0f * static_cast<float>(turns - rint(turns)), &s, &c);
-  const T ct = rounded<T>(c * f.magnitude), st = rounded<T>(s * f.magnitude);
-  const size_t base = static_cast<size_t>(row) * (2 * pairs);
-  const size_t a = base + (interleaved ? 2 * p : p), b = base + (interleaved ? 2 * p + 1 : p + pairs);
-  cos_[a] = cos_[b] = ct;
-  sin_[a] = sin_[b] = st;
+                                                          long long stride, Frequencies f, int pairs,
+                                                          T* __restrict__ cos_, T* __restrict__ sin_, uint32_t n) {
+  typedef T Vec __attribute__((ext_vector_type(kMore)));
+  const uint32_t per = static_cast<uint32_t>(pairs / kMore), rows = 256u / per;  // positions of a workgroup at once
+  if (threadIdx.x >= per * rows) return;
+  const int p = kMore * static_cast<int>(threadIdx.x % per);
+  double f_[kMore];
+#pragma unroll
+  for (int k = 0; k < kMore; ++k) f_[k] = f.turns[p + k];
+  for (uint32_t row = blockIdx.x * rows + threadIdx.x / per; row < n; row += gridDim.x * rows) {
+    const long long at = static_cast<long long>(row) * stride;
+    const double pos = wide ? static_cast<double>(static_cast<const long long*>(positions)[at])
+                            : static_cast<double>(static_cast<const int*>(positions)[at]);
+    T c[kMore], s[kMore];
+#pragma unroll
+    for (int k = 0; k < kMore; ++k) {
+      const double turns = pos * f_[k];
+      float sk, ck;
+      sincospif(2.0f * static_cast<float>(turns - rint(turns)), &sk, &ck);
+      c[k] = rounded<T>(ck * f.magnitude), s[k] = rounded<T>(sk * f.magnitude);
+    }
+    const size_t base = static_cast<size_t>(row) * (2 * pairs);
+    // the kMore values of a pair's first dims, then of the second ones; or both in turn
+    Vec c0, c1, s0, s1;
+#pragma unroll
+    for (int k = 0; k < kMore; ++k) {
+      const int a = kInterleaved ? k / 2 : k, b = kInterleaved ? (kMore + k) / 2 : k;
+      c0[k] = c[a], s0[k] = s[a], c1[k] = c[b], s1[k] = s[b];
+    }
+    const size_t first = base + (kInterleaved ? 2 * p : p), second = kInterleaved ? first + kMore : first + pairs;
+    *reinterpret_cast<Vec*>(cos_ + first) = c0;
+    *reinterpret_cast<Vec*>(cos_ + second) = c1;
+    *reinterpret_cast<Vec*>(sin_ + first) = s0;
+    *reinterpret_cast<Vec*>(sin_ + second) = s1;
+  }
 }
 
 // --------------------------------------------------------------------- heads
 enum class Layout {
   kHalf,   // dims d and d + R/2, R a multiple of 16
+  kFours,  // the same, R a multiple of 8
   kPairs,  // dims 2d and 2d + 1, R a multiple of 8
   kAny     // either, R even
 };
@@ -150,6 +171,32 @@ __global__ __launch_bounds__(256) void heads_append_kernel(HeadArgs a) {
           y1[k] = fmaf(v, half_of<BF16>(c1, k), u * half_of<BF16>(s1, k));
         }
       }
+    } else if constexpr (kLayout == Layout::kFours) {
+      // four dims lie in one half, and those that belong to them in the other: read
+      // again, 8 bytes at a time
+      auto turn = [&](float(&y)[8], int d) {
+        if (d >= a.R) return;
+        const u32x4 c = *reinterpret_cast<const u32x4*>(cp + d), s = *reinterpret_cast<const u32x4*>(sp + d);
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const bool first = d + 4 * j < a.R / 2;
+          const int o = first ? d + 4 * j + a.R / 2 : d + 4 * j - a.R / 2;
+          const uint2 x = *reinterpret_cast<const uint2*>(src + o);
+          float other[4] = {lo16_to_f32<BF16>(x.x), hi16_to_f32<BF16>(x.x), lo16_to_f32<BF16>(x.y), hi16_to_f32<BF16>(x.y)};
+          if (w) {
+            const uint2 v = *reinterpret_cast<const uint2*>(w + o);
+            other[0] *= scale * lo16_to_f32<BF16>(v.x), other[1] *= scale * hi16_to_f32<BF16>(v.x);
+            other[2] *= scale * lo16_to_f32<BF16>(v.y), other[3] *= scale * hi16_to_f32<BF16>(v.y);
+          }
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const float o = other[k] * half_of<BF16>(s, 4 * j + k);
+            y[4 * j + k] = fmaf(y[4 * j + k], half_of<BF16>(c, 4 * j + k), first ? -o : o);
+          }
+        }
+      };
+      turn(y0, d0);
+      turn(y1, d1);
     } else if constexpr (kLayout == Layout::kPairs) {
       auto turn = [&](float(&y)[8], int d) {
         if (d >= a.R) return;
@@ -219,15 +266,24 @@ extern "C" int santa_rope_tables(const void* positions, int wide, long long stri
   paged::Frequencies f;
   for (int i = 0; i < pairs; ++i) f.turns[i] = turns[i];
   f.magnitude = magnitude;
-  const uint32_t total = static_cast<uint32_t>(n * pairs);
-  auto launch = [&](auto kernel, auto* c, auto* s) {
-    hipLaunchKernelGGL(kernel, dim3((total + 255) / 256), dim3(256), 0, stream, positions, wide, stride, f, pairs,
-                       interleaved, c, s, total);
+  if ((reinterpret_cast<uintptr_t>(cos_) | reinterpret_cast<uintptr_t>(sin_)) % 16 != 0)
+    return set_error(SANTA_ERR_INVALID, "rope_tables: the tables must be 16-byte aligned");
+  auto run = [&](auto* c, auto* s) {
+    using T = std::remove_reference_t<decltype(*c)>;
+    auto launch = [&](auto kernel, int more) {
+      const long long rows = 256 / (pairs / more), wgs = (n + rows - 1) / rows;
+      // a few rounds of positions to a workgroup, for one look at the frequencies
+      hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(std::min(wgs, 1024LL))), dim3(256), 0, stream, positions,
+                         wide, stride, f, pairs, c, s, static_cast<uint32_t>(n));
+    };
+    if (pairs % 4 == 0)
+      interleaved ? launch(paged::rope_tables_kernel<T, 4, true>, 4) : launch(paged::rope_tables_kernel<T, 4, false>, 4);
+    else
+      interleaved ? launch(paged::rope_tables_kernel<T, 1, true>, 1) : launch(paged::rope_tables_kernel<T, 1, false>, 1);
   };
-  if (dtype == SANTA_F32) launch(paged::rope_tables_kernel<float>, static_cast<float*>(cos_), static_cast<float*>(sin_));
-  else if (dtype == SANTA_BF16)
-    launch(paged::rope_tables_kernel<__bf16>, static_cast<__bf16*>(cos_), static_cast<__bf16*>(sin_));
-  else launch(paged::rope_tables_kernel<_Float16>, static_cast<_Float16*>(cos_), static_cast<_Float16*>(sin_));
+  if (dtype == SANTA_F32) run(static_cast<float*>(cos_), static_cast<float*>(sin_));
+  else if (dtype == SANTA_BF16) run(static_cast<__bf16*>(cos_), static_cast<__bf16*>(sin_));
+  else run(static_cast<_Float16*>(cos_), static_cast<_Float16*>(sin_));
   const hipError_t e = hipGetLastError();
   if (e != hipSuccess) return set_error(SANTA_ERR_HIP, "rope_tables launch failed: %s", hipGetErrorString(e));
   return clear_error();
@@ -278,8 +334,9 @@ extern "C" int santa_paged_heads_append(const void* qkv, const void* cos_, const
   a.total = static_cast<uint32_t>(heads);
   auto run = [&](auto bf) {
     constexpr bool BF16 = decltype(bf)::value;
-    if (interleaved ? R % 8 != 0 : R % 16 != 0) launch_heads<BF16, Layout::kAny>(a, stream);
+    if (R % 8 != 0) launch_heads<BF16, Layout::kAny>(a, stream);
     else if (interleaved) launch_heads<BF16, Layout::kPairs>(a, stream);
+    else if (R % 16 != 0) launch_heads<BF16, Layout::kFours>(a, stream);
     else launch_heads<BF16, Layout::kHalf>(a, stream);
   };
   if (dtype == SANTA_BF16) run(std::true_type{});

@@ -22,7 +22,7 @@ from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
-from .paged import PagedPlan, _launch, _PlanInfo
+from .paged import _KINDS, PagedPlan, _launch, _PlanInfo
 from .runtime import _FusedOps, _plain
 
 __all__ = ["adjust_logits"]
@@ -142,10 +142,9 @@ def adjust_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
         allowed, allowed_stride = _rows(allowed, N, "allowed")
     if plan is not None and tokens is not None and plan._info.max_len >= 1 << 19:
         raise ValueError(f"at most {(1 << 19) - 1} tokens are counted; got {plan._info.max_len}")
-    kind = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}.get(logits.dtype)
-    given = [t for t in (tokens, prompts, *penalties, ids, values, allowed) if isinstance(t, torch.Tensor)]
-    if not (device.type == "cuda" and kind is not None
-            and _plain(logits, *(t for t in given if t.dtype.is_floating_point))):
+    kind = _KINDS.get(logits.dtype)
+    given = [t for t in (*penalties, values) if isinstance(t, torch.Tensor)]
+    if not (device.type == "cuda" and kind is not None and _plain(logits, *given)):
         out = _expressions(logits, tokens, plan, prompts, penalties, ids, values, allowed)
         if plan is not None:
             plan._captured(0, False)

@@ -122,6 +122,8 @@ def _int_list(values, what: str) -> List[int]:
     if isinstance(values, int):
         raise ValueError(f"{what} must be a list")
     values = list(values)
+    if set(map(type, values)) <= {int}:
+        return values
     ints = [int(v) for v in values]
     if ints != values:
         raise ValueError(f"{what} must be whole numbers")
@@ -129,9 +131,9 @@ def _int_list(values, what: str) -> List[int]:
 
 
 def _ints(values: Sequence[int]):
-    for v in values:
-        if not -(1 << 31) <= v < 1 << 31:
-            raise ValueError(f"{v} does not fit 32 bits")
+    if values and not -(1 << 31) <= min(values) <= max(values) < 1 << 31:
+        bad = next(v for v in values if not -(1 << 31) <= v < 1 << 31)
+        raise ValueError(f"{bad} does not fit 32 bits")
     return (ctypes.c_int * len(values))(*values)
 
 
@@ -236,12 +238,13 @@ class PagedKVCache:
         other sequences too."""
         seqs = _int_list(seqs, "seqs")
         new = [new_tokens] * len(seqs) if isinstance(new_tokens, int) else _int_list(new_tokens, "new_tokens")
-        kept = [_int_list(k, "kept") for k in kept]
+        kept = [k if type(k) is list else _int_list(k, "kept") for k in kept]
         if len(new) != len(seqs) or len(kept) != len(seqs):
             raise ValueError(f"new_tokens and kept must have one entry per sequence ({len(seqs)})")
+        flat = _int_list([i for k in kept for i in k], "kept")
         self._may_change()
-        _check(_lib().santa_pages_keep(self._pages, _ints(seqs), _ints(new), _ints([i for k in kept for i in k]),
-                                       _ints([len(k) for k in kept]), len(seqs)))
+        _check(_lib().santa_pages_keep(self._pages, _ints(seqs), _ints(new), _ints(flat), _ints([len(k) for k in kept]),
+                                       len(seqs)))
         if self.device.type == "cuda":
             _launch(self.device, _lib().santa_pages_apply_moves, self._pages, self._pools, len(self._pools),
                     self._page_bytes, self._page_bytes)
@@ -653,16 +656,16 @@ def _token_slots(block_table, plan: PagedPlan, page_size: int):
     return token, block_table[seq, pos // page_size].long() * page_size + pos % page_size
 
 
-def _norm(w: Optional[torch.Tensor], heads: int, what: str, like: torch.Tensor) -> Optional[torch.Tensor]:
-    """A norm's weights as [1, D] or [heads, D]."""
+def _norm_rows(w: Optional[torch.Tensor], heads: int, what: str, like: torch.Tensor) -> int:
+    """Rows of a norm's weights [D] or [heads, D]: 1, or one per head."""
     if w is None:
-        return None
-    D = like.shape[2]
-    if w.shape not in ((D,), (heads, D)):
-        raise ValueError(f"{what} must be [{D}] or [{heads}, {D}]; got {tuple(w.shape)}")
-    if w.device != like.device or w.dtype != like.dtype:
+        return 1
+    shape, D = w.shape, like.shape[2]
+    if shape != (D,) and shape != (heads, D):
+        raise ValueError(f"{what} must be [{D}] or [{heads}, {D}]; got {tuple(shape)}")
+    if w.dtype != like.dtype or w.device != like.device:
         raise ValueError(f"{what} must have the device and dtype of qkv")
-    return w.view(1, D) if w.dim() == 1 else w
+    return 1 if len(shape) == 1 else heads
 
 
 def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -690,7 +693,7 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages
     device, dtype = qkv.device, qkv.dtype
     if cos.device != device or sin.device != device or cos.dtype != dtype or sin.dtype != dtype:
         raise ValueError("cos and sin must have the device and dtype of qkv")
-    q_norm, k_norm, eps = _norm(q_norm, H, "q_norm", qkv), _norm(k_norm, KVH, "k_norm", qkv), float(eps)
+    q_rows, k_rows, eps = _norm_rows(q_norm, H, "q_norm", qkv), _norm_rows(k_norm, KVH, "k_norm", qkv), float(eps)
     if not 0.0 <= eps < math.inf:
         raise ValueError(f"eps must be at least 0 and finite; got {eps}")
     norms = [w for w in (q_norm, k_norm) if w is not None]
@@ -712,10 +715,13 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages
                 _launch(device, _lib().santa_paged_rope_append, qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(),
                         q.data_ptr(), *rest)
             else:
-                q_norm, k_norm = (w if w is None else _packed(w) for w in (q_norm, k_norm))
-                weights = [x for w in (q_norm, k_norm) for x in ((None, 1) if w is None else (w.data_ptr(), len(w)))]
+                if q_norm is not None:
+                    q_norm = _packed(q_norm)
+                if k_norm is not None:
+                    k_norm = _packed(k_norm)
                 _launch(device, _lib().santa_paged_heads_append, qkv.data_ptr(), cos.data_ptr(), sin.data_ptr(), R,
-                        int(interleaved), *weights, eps, q.data_ptr(), *rest)
+                        int(interleaved), None if q_norm is None else q_norm.data_ptr(), q_rows,
+                        None if k_norm is None else k_norm.data_ptr(), k_rows, eps, q.data_ptr(), *rest)
             plan._captured(block_table.shape[1] * k_pages.shape[1], True)
         return q
     wide = torch.float64 if qkv.dtype == torch.float64 else torch.float32
@@ -805,6 +811,9 @@ class RopeScaling:
         return [x / self.factor * (1.0 - s) + x * s for x, s in zip(f, left)], magnitude
 
 
+_KINDS = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
 @functools.lru_cache(maxsize=64)
 def _frequencies(dim: int, theta: float, scaling: Optional[RopeScaling]):
     """(Angles per position, the same in turns as a C array, magnitude)."""
@@ -829,7 +838,7 @@ def rope_tables(positions: torch.Tensor, dim: int, *, theta: float = 10000.0, sc
         raise ValueError("the tables have a floating point dtype")
     f, turns, magnitude = _frequencies(int(dim), float(theta), scaling)
     device = positions.device
-    kind = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}.get(dtype)
+    kind = _KINDS.get(dtype)
     if device.type == "cuda" and kind is not None and dim <= 512 and _plain(positions):
         cos, sin = (torch.empty(len(positions), dim, dtype=dtype, device=device) for _ in range(2))
         _launch(device, _lib().santa_rope_tables, positions.data_ptr(), int(positions.dtype == torch.int64),
