@@ -561,6 +561,30 @@ class PagedPlan:
             return list(range(max(0, t - n), t))
         return [] if n < t else [i for i, p in enumerate(parents) if p != -2]
 
+    def accepted(self, drafts: Sequence[int], chosen: Sequence[int]) -> Tuple[List[List[int]], List[int]]:
+        """Which drafted tokens a step accepts: from each sequence's first token on,
+        which is no guess, to the one that follows and is the token chosen behind it
+        (the first such), as far as there is one.  drafts, chosen: the batch's tokens
+        and those chosen behind each, as host integers.  Returns the accepted tokens'
+        numbers for each sequence (``PagedKVCache.keep``) and the token chosen behind
+        the last of them; none and -1 for a sequence without a first token."""
+        drafts, chosen = _int_list(drafts, "drafts"), _int_list(chosen, "chosen")
+        if self.parents is None or None in self.parents:
+            raise ValueError("the plan has sequences without trees")
+        if len(drafts) != self.tokens or len(chosen) != self.tokens:
+            raise ValueError(f"drafts and chosen must have one entry per token ({self.tokens})")
+        kept, following, t0 = [], [], 0
+        for b, parents in enumerate(self.parents):
+            path, at = [], 0 if parents and parents[0] == -1 and self.seq_lens[b] >= len(parents) else -1
+            while at >= 0:
+                path.append(at)
+                want = chosen[t0 + at]
+                at = next((i for i in range(at + 1, len(parents)) if parents[i] == at and drafts[t0 + i] == want), -1)
+            kept.append(path)
+            following.append(chosen[t0 + path[-1]] if path else -1)
+            t0 += len(parents)
+        return kept, following
+
     def _sees(self, b: int) -> torch.Tensor:
         """[t, t]: which of sequence b's drafted tokens its drafted tokens attend to."""
         parents = self.parents[b]

@@ -632,7 +632,7 @@ class RandomLlama:
     @torch.inference_mode()
     def extend(self, tokens: torch.Tensor, cache, seqs: Sequence[int],
                new_tokens: Union[None, int, Sequence[int]] = None, *, backend=None,
-               mlp_chunk: int = 8192) -> torch.Tensor:
+               mlp_chunk: int = 8192, parents=None) -> torch.Tensor:
         """New tokens of sequences of a santa_amd.paged.PagedKVCache: prompts of
         new sequences, more tokens behind what a sequence holds (a prompt behind
         one it was forked from), or one decoded token each.  tokens: [len(seqs),
@@ -642,8 +642,11 @@ class RandomLlama:
         sequence's last token [len(seqs), V] (float32, as prefill's).  Attention
         is exact, tokens that sequences hold in the same pages being read once;
         or, for one new token each, that of a backend with decode_paged (given the
-        step's plan where its decodes_plans is set).  A call that fails leaves
-        the sequences with the tokens that they had."""
+        step's plan where its decodes_plans is set).  parents: the new tokens are
+        drafts that follow one another as trees (santa_amd.paged.PagedPlan), and the
+        logits are those behind every new token [tokens, V]; PagedKVCache.keep then
+        takes back what is not accepted.  A call that fails leaves the sequences with
+        the tokens that they had."""
         from .paged import _int_list
 
         s, D = self.shape, self.shape.head_dim
@@ -662,23 +665,26 @@ class RandomLlama:
             raise ValueError(f"the cache is on {cache.device}, the model on {self.embed.device}")
         if backend is not None and max(new) > 1:
             raise ValueError("a backend decodes one new token per sequence")
+        if backend is not None and parents is not None:
+            raise ValueError("a backend decodes no trees")
         if mlp_chunk < 1:
             raise ValueError(f"mlp_chunk must be at least 1; got {mlp_chunk}")
         h = self.embed[tokens.reshape(-1)]  # [N, hidden]
         cache.extend(seqs, new)
         try:
-            return self._extend(h, cache, seqs, new, backend, mlp_chunk)
+            return self._extend(h, cache, seqs, new, backend, mlp_chunk, parents)
         except BaseException:  # a backend that does not take the model, a GPU without room
             cache._take_back(seqs, new)
             raise
 
-    def _extend(self, h: torch.Tensor, cache, seqs: List[int], new: List[int], backend, mlp_chunk: int) -> torch.Tensor:
+    def _extend(self, h: torch.Tensor, cache, seqs: List[int], new: List[int], backend, mlp_chunk: int,
+                parents) -> torch.Tensor:
         """extend() of embedded tokens h [N, hidden] that the sequences have
         pages for."""
         from .paged import paged_attention, rope_append
 
         s, D = self.shape, self.shape.head_dim
-        plan = cache.plan(seqs, s.heads, new)
+        plan = cache.plan(seqs, s.heads, new, parents=parents)
         cos, sin = _rope_cos_sin(plan.positions, D, s.rope_theta, self.dtype)  # [N, D]
         table = cache.block_table
         planned = getattr(backend, "decodes_plans", False)
@@ -718,7 +724,7 @@ class RandomLlama:
                     hc = h[c:c + mlp_chunk]
                     hc += self._mlp(L, _rms_norm(hc, L["ln2"], s.rms_eps))
             x = _rms_norm(h, self.norm, s.rms_eps)
-        if max(new) > 1:
+        if max(new) > 1 and parents is None:
             last = torch.tensor(new).cumsum(0) - 1
             if x.is_cuda:
                 last = last.pin_memory().to(x.device, non_blocking=True)
