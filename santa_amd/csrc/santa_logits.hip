@@ -505,8 +505,8 @@ extern "C" int santa_adjust_logits(const void* x, int dtype, long long stride, i
   }
   a.out = out;
   a.best = static_cast<unsigned long long*>(workspace);
+  a.rows = std::max(a.rows, (N + 65534) / 65535);  // a grid's second dimension
   const int group = (N + a.rows - 1) / a.rows;
-  if (group > 65535) return set_error(SANTA_ERR_INVALID, "adjust_logits: too many rows");
   const int parts = static_cast<int>(parts_of(V, steps));
   auto launch = [&](auto kernel) {
     hipLaunchKernelGGL(kernel, dim3(static_cast<unsigned>(parts / kWaves), static_cast<unsigned>(group)),

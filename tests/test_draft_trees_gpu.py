@@ -130,6 +130,21 @@ def test_masked_values_stay_out(H, KVH, D, dtype):
         _check(out[~hit], tuple(x[~hit] for x in base), dtype)
 
 
+def test_masked_values_beside_plain_sequences():
+    """The same in a batch whose other sequence has no tree: later tokens stay out there."""
+    print("\n[case] masked values beside a sequence without a tree", flush=True)
+    for H, KVH, D in ((4, 2, 128), (16, 1, 64), (40, 1, 128)):
+        lens, new, trees = [100, 140], [5, 30], [[-1, 0, 0, 1, 2], None]
+        q, k, v, table, plan = _case(lens, new, trees, [], H, KVH, D, 16, BF, H)
+        base = _reference(q, k, v, table, lens, new, trees)
+        v[table[1, 130 // 16].long(), 130 % 16], k[table[1, 130 // 16].long(), 130 % 16] = math.inf, math.nan
+        v[table[0, 98 // 16].long(), 98 % 16] = math.nan
+        out = paged_attention(q, k, v, table, plan)
+        hit = torch.tensor([False, False, False, True, False] + [110 + i >= 130 for i in range(30)]).cuda()
+        assert not torch.isfinite(out[hit]).any()
+        _check(out[~hit], tuple(x[~hit] for x in base), BF)
+
+
 def test_tokens_not_in_use_behind_bad_prefixes():
     """Zeros of tokens not in use, also where the context holds infinities and NaN."""
     print("\n[case] not in use behind infinities", flush=True)

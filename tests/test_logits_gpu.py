@@ -65,11 +65,22 @@ def large(lens, new, V, K, seed, chains=(), dtype=torch.float32, trees=True):
     ([700, 800, 900], [64, 100, 1], 50002, 50, (1,), torch.float16, True),
     ([300 + i for i in range(40)], [40] * 40, 4100, 9, (), torch.float32, True),  # many rows to a workgroup
     ([90] * 600, [1] * 600, 2049, 5, (), torch.float32, False), ([1100], [1024], 1000, 5, (), torch.float32, True),
-    ([60000], [3], 100, 5, (), torch.float32, True),
+    ([60000], [3], 100, 5, (), torch.float32, True), ([9000], [8192], 40, 5, (), torch.float16, True),
 ])
 def test_sizes(lens, new, V, K, chains, dtype, trees):
     print(f"\n[case] sizes lens={lens[:4]} new={new[:4]} V={V} K={K} {dtype}", flush=True)
     same(*large(lens, new, V, K, V, chains, dtype, trees))
+
+
+def test_many_rows():
+    """More rows than a grid has in one dimension, of one sequence each and without any."""
+    print("\n[case] many rows", flush=True)
+    x = torch.randn(140001, 9, device="cuda")
+    assert torch.equal(adjust_logits(x), x) and torch.equal(adjust_logits(x, greedy=True), x.argmax(-1))
+    t = torch.randint(0, 9, (140001, 4), device="cuda", dtype=torch.int32)
+    out = adjust_logits(x, t, [3] * 140001, presence=2.0)
+    seen = torch.zeros_like(x, dtype=torch.bool).scatter_(1, t[:, :3].long(), True)
+    assert torch.equal(out, torch.where(seen, x - 2.0, x))
 
 
 def test_layouts():

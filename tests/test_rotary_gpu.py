@@ -83,7 +83,8 @@ CASES = [
     (128, 24, 4, 2, "both", True, F16), (128, 6, 4, 2, "none", False, BF), (64, 62, 4, 2, "per head", True, BF),
     (16, 16, 2, 1, "both", False, BF), (32, 8, 2, 1, "both", True, F16), (48, 48, 3, 3, "both", False, BF),
     (80, 32, 2, 1, "per head", False, F16), (256, 64, 4, 2, "both", False, BF), (512, 512, 2, 1, "both", True, BF),
-    (96, 96, 2, 1, "q", True, BF), (272, 2, 2, 1, "k", False, F16),
+    (96, 96, 2, 1, "q", True, BF), (272, 2, 2, 1, "k", False, F16), (16, 8, 2, 2, "both", False, BF),
+    (256, 200, 2, 1, "per head", False, F16),
 ]
 
 
