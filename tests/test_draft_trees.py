@@ -125,6 +125,7 @@ PLANS = [
     ([300, 20, 2, 5], [250, 20, 7, 0], (2,), 0.1, [], 7, 1, 32),
     ([2000], [129], (), 0.5, [], 8, 2, 64),
     ([], [], (), 0.0, [], 4, 2, 8),
+    ([700, 900], [40, 60], (), 0.1, [], 8, 1, 16), ([900, 20, 66], [40, 60, 33], (1,), 0.0, [], 8, 1, 16),
 ]
 
 

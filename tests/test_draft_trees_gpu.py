@@ -71,6 +71,10 @@ CASES = [
     ([2000 + i for i in range(20)], [4] * 20, (3, 5), 0.1, [(list(range(20)), 1984)], 32, 8, 128, 16, BF),
     ([700, 650, 300, 66], [90, 40, 0, 2], (0,), 0.0, [([0, 1, 2, 3], 64)], 7, 1, 128, 32, BF),
     ([5000], [25], (), 0.0, [], 32, 8, 128, 16, BF), ([5000, 4000], [31, 17], (), 0.1, [], 28, 4, 64, 32, F16),
+    # several blocks of 256 rows
+    ([3000, 1000, 2500, 64], [64, 40, 50, 60], (), 0.1, [], 64, 8, 128, 16, BF),
+    ([3000, 2900], [64, 80], (), 0.1, [], 32, 4, 64, 64, F16), ([9000], [100], (), 0.0, [], 8, 1, 128, 16, BF),
+    ([9000, 30, 8000], [40, 60, 64], (2,), 0.0, [], 16, 2, 128, 32, F16),
     # one row of bits that no token sets: none in use
     ([100, 200], [6, 3], (), 1.0, [], 4, 2, 128, 16, BF),
 ]
