@@ -110,7 +110,8 @@ struct MoveArgs {
 // every row of a sequence, in order, up to eight read before they are written (a
 // later row never reads what an earlier one wrote, so that a batch of reads may come
 // first), and no thread touches another's pieces: nothing to wait for.  Latency bound:
-// a launch, a read and a write.
+// 64 sequences' paths of up to 8 tokens in 32 pools, 23 MB read and written, are two
+// launches of about 5 us, and 2 us one sequence's in 4 pools.
 template <class T>
 __global__ __launch_bounds__(128) void move_rows_kernel(MoveArgs a) {
   const uint32_t i = blockIdx.x * 128u + threadIdx.x;
@@ -280,6 +281,18 @@ __global__ __launch_bounds__(256) void rope_append_kernel(const uint16_t* __rest
 // a long prompt has both: 64 sequences behind 32k tokens 114 us, 32 with 64 query and
 // 8 KV heads behind 128k 262 us (106 and 215 with rounded probabilities).  Little work: latency, about 10 us for the first
 // loads, one tile, the join of the waves and the output.
+//
+// Trees of drafted tokens (a kernel of its own, kTrees, so that calls without them
+// stay as they are): a row attends to the whole context and, behind it, to the tokens
+// of its bits.  Only the tiles from the context's end on differ, one or two for up to
+// 64 drafts; their scores are masked by a bit each, and all else is the same pass: 16
+// sequences of 1000 to 20 000 tokens with 25 drafts each, 32 query and 8 KV heads, 648
+// MB, 137 us, 4.7 TB/s, and 147 to 157 with the join, where the same tokens in a row
+// take 146 to 150.  Eight of 30 to 131 thousand tokens with 64 drafts, 64 query and 8 KV
+// heads: 1.56 to 1.8 ms, 790 to 915 TFLOP/s.  Their 512 rows are two blocks, and what
+// they wait for is not HBM: with all pages in the L2 1.40 ms, with K and V of zeros, read
+// as ever, 1.25, as the chip holds its clocks then.  Bits in LDS, 4 KiB for the first two
+// tiles of every row: in registers they spill, 27 of them beside probabilities in two parts.
 constexpr int kWaves = 8;
 // Above this a row's reference in log2 units is subtracted from the scores before
 // they are scaled: fma(score, scale, -round(m * scale)) is off by half an ulp of

@@ -40,7 +40,7 @@ int tile_cost(int rows, bool rounded) { return rows > 128 ? (rounded ? 10 : 13) 
 // Whether a sequence's new tokens have the batch's probabilities rounded for the
 // second product (santa_paged_plan_info.rounded, the default): several tokens, as
 // in a prefill, whose second products would cost more than they do behind HBM.
-// 8 sequences of 3000 to 16000 tokens, GH 4, D 128, rounded and in two parts: 8
+// (Trees of drafts follow the same rule.)  8 sequences of 3000 to 16000 tokens, GH 4, D 128, rounded and in two parts: 8
 // tokens (32 rows) 76.8 and 77.5 us, 9 77.6 and 84.2, 32 90.9 and 102.9; a prefill
 // of 1300 tokens 313 and 410.  A single token is never rounded: what it attends to
 // must not depend on how many others read the same pages.

@@ -14,15 +14,17 @@ the same pages until they write:
     seqs = [prompt, *cache.fork(prompt, 63)]
     logits = model.extend(next_tokens, cache, seqs)         # the prompt's K and V are read once for all 64
 
-* ``PagedKVCache`` adds, lengthens, forks, frees and compacts sequences;
-* ``PagedPlan`` cuts up the attention's work for one set of lengths (built on
-  the host once per step, used by every layer);
-* ``rope_append`` rotates new tokens' q and k and writes k and v to their pages;
+* ``PagedKVCache`` adds, lengthens, forks, frees and compacts sequences, and keeps
+  accepted drafts;
+* ``PagedPlan`` cuts up the attention's work for one set of lengths and trees of
+  drafts (built on the host once per step, used by every layer);
+* ``rope_tables`` makes the cos and sin of positions, ``rope_append`` norms and rotates
+  new tokens' q and k and writes k and v to their pages;
 * ``paged_attention`` is exact attention over pages, for one or several new
   tokens per sequence;
 * ``copy_pages`` copies pages within pools.
 
-On a GPU all of them run the library's kernels (santa_paged.hip); torch
+On a GPU all of them run the library's kernels (santa_paged.hip, santa_rotary.hip); torch
 expressions are the CPU path and that of calls that the attention kernel does
 not take (float32, head_dim other than 64 and 128, autograd).
 """
