@@ -221,22 +221,25 @@ __global__ __launch_bounds__(kThreads, kMany || kSteps == kMostSteps ? 4 : 6) vo
       if (tid < drafts) w.path = static_cast<uint32_t>(record[paged::kTreeWords + (tid >> 5)]);
     }
   };
-  int held = -1, upto = 0;       // the words are those of this sequence's first tokens,
-  bool added = false;            // this lane's drafted token where this is set,
-  const int* far = nullptr;      // and those beyond the lanes that this record's token follows
-  int mine = -1, mine_base = -1; // the drafted token, of the tree from this place on
+  int held = -1, upto = 0;   // the words are those of this sequence's first tokens,
+  bool added = false;        // this lane's drafted token where this is set,
+  const int* far = nullptr;  // and those beyond the lanes that this record's token follows,
+  int tree_base = -1;        // of the tree behind this place (-1: none are marked)
+  int mine = -1;             // the drafted token
   int own = -1;                  // the listed token that this lane has the logit of, for the next row
   float own_logit = 0.0f;
   Rules rules{1.0f, 0.0f, 0.0f, bias};
   auto work_on = [&](Ahead<kType, kSteps>& w, int r) {
     const int seq = a.pos ? w.at.y : r, context = !a.tokens ? 0 : a.tree ? w.head.x : w.at.x + 1;
-    const bool used = a.tokens && a.tree && w.head.y >= 0;
+    // a tree's token lies behind the context that it sees, others are the last of theirs
+    const bool drafted = a.tokens && a.tree && w.head.y >= 0 && context <= w.at.x;
     int count = 0;
     if (ruled) {
       const void* row = static_cast<const char*>(a.tokens) + seq * a.tokens_stride * (a.wide ? 8 : 4);
       const int base = context & ~63;
-      const bool anew = seq != held || context < upto;
-      if (anew) upto = 0, mine_base = -1;
+      const bool anew = seq != held || context < upto ||
+                        (tree_base >= 0 && !(drafted && base == tree_base && context == upto));
+      if (anew) upto = 0, tree_base = -1;
       // what is read here is asked for before any of it is used
       int id[kTokenSteps][4], bias_id = -1;
       float bias_value = 0.0f;
@@ -245,10 +248,10 @@ __global__ __launch_bounds__(kThreads, kMany || kSteps == kMostSteps ? 4 : 6) vo
         bias_value = a.bias[seq * a.bias_stride + tid];
       }
       if (context > upto) ask_tokens(a, row, upto, context, id);
-      const bool plant = used && mine_base != base;
+      const bool plant = drafted && tree_base < 0;
       if (plant) {
         mine = tid < drafts && base + tid >= context && base + tid < a.tokens_len ? token_at(a, row, base + tid) : -1;
-        mine_base = base;
+        tree_base = base;
       }
       if (anew) {
         rules.repetition = a.repetition ? a.repetition[seq] : a.repetition_all;
@@ -301,7 +304,7 @@ __global__ __launch_bounds__(kThreads, kMany || kSteps == kMostSteps ? 4 : 6) vo
         for (int i = tid + kThreads; i < drafts && base + i < a.tokens_len; i += kThreads)  // all behind the context
           touch(token_at(a, row, base + i), [](uint32_t* at) { return atomicOr(at, kDrafted); });
       }
-      if (used) {
+      if (drafted) {
         const bool want = (w.path >> (tid & 31) & 1) && base + tid >= context;
         const uint32_t by = want ? 1u : 0xffffffffu;
         if (want != added) touch(mine, [&](uint32_t* at) { return atomicAdd(at, by) | 1u; });

@@ -83,6 +83,27 @@ def test_many_rows():
     assert torch.equal(out, torch.where(seen, x - 2.0, x))
 
 
+def test_the_same_row_twice():
+    """Entries of a batch that read one row of the table, with other lengths, trees or
+    none, one after the other in a workgroup."""
+    print("\n[case] the same row twice", flush=True)
+    r = random.Random(7)
+    lens, new = [130, 70, 66, 200, 66, 500, 66], [30, 6, 2, 9, 30, 1, 5]
+    trees = [random_tree(r, 30, 0.1), random_tree(r, 6), random_tree(r, 2), None, random_tree(r, 30), None, random_tree(r, 5)]
+    rows = [0, 0, 0, 0, 0, 0, 0]
+    g = torch.Generator().manual_seed(0)
+    tokens = torch.randint(0, 50, (1, 520), generator=g, dtype=torch.int32)
+    for V in (50, 128256):
+        logits = torch.randn(sum(new), V, generator=g)
+        plan = PagedPlan(lens, heads=4, kv_heads=2, new_tokens=new, rows=rows, parents=trees, device="cpu")
+        kw = dict(repetition=1.2, frequency=0.1, prompts=torch.tensor([40], dtype=torch.int32))
+        same(logits, tokens, plan, kw)
+    big = [[-1] + [0] * 599, [-1] + [0] * 599]  # drafts beyond a workgroup's lanes
+    plan = PagedPlan([700, 664], heads=4, kv_heads=2, new_tokens=600, rows=[0, 0], parents=big, device="cpu")
+    same(torch.randn(1200, 64, generator=g), torch.randint(0, 64, (1, 700), generator=g, dtype=torch.int32), plan,
+         dict(presence=0.5, frequency=0.25))
+
+
 def test_layouts():
     """Rows that lie apart, columns that do, tables that are views, one row for all."""
     print("\n[case] layouts", flush=True)
