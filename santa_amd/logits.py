@@ -54,9 +54,10 @@ def _lib():
 
 def _penalty(value, what: str, seqs: int, device, positive: bool) -> Union[float, torch.Tensor]:
     if isinstance(value, torch.Tensor):
-        if value.dim() != 1 or value.dtype != torch.float32 or value.device != device or len(value) < seqs:
+        shape = value.shape
+        if len(shape) != 1 or value.dtype != torch.float32 or value.device != device or shape[0] < seqs:
             raise ValueError(f"{what} must be a number or float32 [sequences] on the logits' device, {seqs} or more")
-        return value.contiguous()
+        return value if value.is_contiguous() else value.contiguous()
     value = float(value)
     if not math.isfinite(value) or (positive and value <= 0.0):
         raise ValueError(f"{what} must be {'positive and ' if positive else ''}finite; got {value}")
@@ -65,11 +66,12 @@ def _penalty(value, what: str, seqs: int, device, positive: bool) -> Union[float
 
 def _rows(t: torch.Tensor, count: int, what: str) -> Tuple[torch.Tensor, int]:
     """t [1 or at least count, n] with contiguous rows, and its row stride (0: one row for all)."""
-    if t.dim() != 2 or (t.shape[0] != 1 and t.shape[0] < count):
-        raise ValueError(f"{what} must have one row, or {count}; got {tuple(t.shape)}")
-    if t.shape[1] > 1 and t.stride(1) != 1:
+    shape = t.shape
+    if len(shape) != 2 or (shape[0] != 1 and shape[0] < count):
+        raise ValueError(f"{what} must have one row, or {count}; got {tuple(shape)}")
+    if shape[1] > 1 and t.stride(1) != 1:
         t = t.contiguous()
-    return t, t.stride(0) if t.shape[0] > 1 else 0
+    return t, t.stride(0) if shape[0] > 1 else 0
 
 
 def adjust_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
@@ -119,7 +121,7 @@ def adjust_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
         if tokens.shape[1] > 1 and tokens.stride(1) != 1:
             tokens = tokens.contiguous()
     if prompts is not None and (prompts.dim() != 1 or prompts.dtype != torch.int32 or prompts.device != device
-                                or len(prompts) < seqs):
+                                or prompts.shape[0] < seqs):
         raise ValueError(f"prompts must be int32 [sequences] on the logits' device, {seqs} or more")
     penalties = [_penalty(x, name, seqs, device, name == "repetition")
                  for x, name in ((repetition, "repetition"), (frequency, "frequency"), (presence, "presence"))]
@@ -134,7 +136,7 @@ def adjust_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
         (ids, bias_stride), (values, value_stride) = _rows(ids, seqs, "bias"), _rows(values, seqs, "bias")
         if bias_stride != value_stride:
             ids, values = ids.contiguous(), values.contiguous()
-            bias_stride = ids.stride(0) if len(ids) > 1 else 0
+            bias_stride = ids.stride(0) if ids.shape[0] > 1 else 0
     if allowed is not None:
         if allowed.dtype != torch.int32 or allowed.device != device or allowed.dim() != 2 or \
                 allowed.shape[1] != -(-V // 32):
