@@ -1089,11 +1089,16 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_attention_kernel(AttnArg
     const Item now = it;
     last = now.next < 0;
     if (!last) it = read_item(w, now.next);  // while this one is worked on
-    if (now.rows <= 16) attend<BF16, D, 1, kLanes, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares, first_bits);
-    else if (now.rows <= 32) attend<BF16, D, 1, kParts, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares, first_bits);
-    else if (now.rows <= 64) attend<BF16, D, 2, kParts, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares, first_bits);
-    else if (now.rows <= 128) attend<BF16, D, 4, kParts, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares, first_bits);
-    else attend<BF16, D, 8, kParts, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares, first_bits);
+    if (now.rows <= 16) attend<BF16, D, 1, kLanes, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages,
+                                                     &shares, first_bits);
+    else if (now.rows <= 32) attend<BF16, D, 1, kParts, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages,
+                                                     &shares, first_bits);
+    else if (now.rows <= 64) attend<BF16, D, 2, kParts, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages,
+                                                     &shares, first_bits);
+    else if (now.rows <= 128) attend<BF16, D, 4, kParts, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages,
+                                                     &shares, first_bits);
+    else attend<BF16, D, 8, kParts, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages,
+                                                     &shares, first_bits);
   }
 }
 

@@ -952,8 +952,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     [num_pages, page_size, KVH, D] which hold the tokens themselves already,
     block_table int32 [sequences, pages] -> [tokens, H, D].  A token attends to
     the tokens of its sequence up to itself or, where the plan has a tree of them,
-    to those that it follows in it; one at a negative position gives zeros.  plan: a PagedPlan, or the lengths of the sequences, each with one
-    new token.  scale: of the scores, positive, 1 / sqrt(D) by default.
+    to those that it follows in it; one at a negative position, or not in use, gives
+    zeros.  plan: a PagedPlan, or the lengths of the sequences, each with one new
+    token.  scale: of the scores, positive, 1 / sqrt(D) by default.
 
     bf16 and f16 of head_dim 64 and 128 on a GPU run as one kernel over all
     sequences (and one that joins parts, where the tokens of a sequence are
