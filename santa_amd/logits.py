@@ -52,10 +52,10 @@ def _lib():
     return _lib_ready
 
 
-def _penalty(value, what: str, seqs: int, device, positive: bool) -> Union[float, torch.Tensor]:
+def _penalty(value, what: str, seqs: int, index: int, positive: bool) -> Union[float, torch.Tensor]:
     if isinstance(value, torch.Tensor):
         shape = value.shape
-        if len(shape) != 1 or value.dtype != torch.float32 or value.device != device or shape[0] < seqs:
+        if len(shape) != 1 or value.dtype != torch.float32 or value.get_device() != index or shape[0] < seqs:
             raise ValueError(f"{what} must be a number or float32 [sequences] on the logits' device, {seqs} or more")
         return value if value.is_contiguous() else value.contiguous()
     value = float(value)
@@ -105,7 +105,7 @@ def adjust_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
     if logits.dim() != 2 or not logits.dtype.is_floating_point or logits.shape[1] == 0:
         raise ValueError(f"logits must be [rows, vocabulary] of a floating point dtype; got {tuple(logits.shape)}")
     N, V = logits.shape
-    device = logits.device
+    device, index = logits.device, logits.get_device()
     if tokens is not None and plan is None:
         raise ValueError("a plan, or the sequences' lengths, says which tokens a row has seen")
     if plan is not None and not isinstance(plan, PagedPlan):
@@ -114,22 +114,22 @@ def adjust_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
         raise ValueError(f"the plan is for {plan.tokens} tokens on {plan.device}; got {N} rows on {device}")
     seqs = N if plan is None else plan._info.max_row + 1
     if tokens is not None:
-        if tokens.dim() != 2 or tokens.dtype not in (torch.int32, torch.int64) or tokens.device != device:
+        if tokens.dim() != 2 or tokens.dtype not in (torch.int32, torch.int64) or tokens.get_device() != index:
             raise ValueError("tokens must be [sequences, places] of int32 or int64 on the logits' device")
         if tokens.shape[0] < seqs or tokens.shape[1] < plan._info.max_len:
             raise ValueError(f"tokens must hold {seqs} sequences of {plan._info.max_len} tokens; got {tuple(tokens.shape)}")
         if tokens.shape[1] > 1 and tokens.stride(1) != 1:
             tokens = tokens.contiguous()
-    if prompts is not None and (prompts.dim() != 1 or prompts.dtype != torch.int32 or prompts.device != device
+    if prompts is not None and (prompts.dim() != 1 or prompts.dtype != torch.int32 or prompts.get_device() != index
                                 or prompts.shape[0] < seqs):
         raise ValueError(f"prompts must be int32 [sequences] on the logits' device, {seqs} or more")
-    penalties = [_penalty(x, name, seqs, device, name == "repetition")
+    penalties = [_penalty(x, name, seqs, index, name == "repetition")
                  for x, name in ((repetition, "repetition"), (frequency, "frequency"), (presence, "presence"))]
     ids = values = None
     if bias is not None:
         ids, values = bias
         if ids.shape != values.shape or ids.dtype != torch.int32 or values.dtype != torch.float32 or \
-                ids.device != device or values.device != device:
+                ids.get_device() != index or values.get_device() != index:
             raise ValueError("bias must be (int32 ids, float32 values) of one shape on the logits' device")
         if ids.dim() == 2 and ids.shape[1] > 2046:
             raise ValueError(f"a row has at most 2046 biases; got {ids.shape[1]}")
@@ -138,7 +138,7 @@ def adjust_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
             ids, values = ids.contiguous(), values.contiguous()
             bias_stride = ids.stride(0) if ids.shape[0] > 1 else 0
     if allowed is not None:
-        if allowed.dtype != torch.int32 or allowed.device != device or allowed.dim() != 2 or \
+        if allowed.dtype != torch.int32 or allowed.get_device() != index or allowed.dim() != 2 or \
                 allowed.shape[1] != -(-V // 32):
             raise ValueError(f"allowed must be int32 [1 or {N}, {-(-V // 32)}] on the logits' device")
         allowed, allowed_stride = _rows(allowed, N, "allowed")

@@ -598,7 +598,7 @@ class PagedPlan:
 
 
 def _check_pools(k_pages, v_pages, block_table, plan: PagedPlan, like: torch.Tensor) -> None:
-    shape, device = k_pages.shape, like.device
+    shape, device = k_pages.shape, like.get_device()
     if len(shape) != 4 or shape != v_pages.shape:
         raise ValueError("k_pages and v_pages must be [num_pages, page_size, KVH, D] tensors of one shape")
     if k_pages.dtype != like.dtype or v_pages.dtype != like.dtype:
@@ -606,10 +606,10 @@ def _check_pools(k_pages, v_pages, block_table, plan: PagedPlan, like: torch.Ten
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or (block_table.shape[1] > 1
                                                                       and block_table.stride(1) != 1):
         raise ValueError("block_table must be an int32 [sequences, pages] tensor with contiguous rows")
-    if k_pages.device != device or v_pages.device != device or block_table.device != device:
+    if k_pages.get_device() != device or v_pages.get_device() != device or block_table.get_device() != device:
         raise ValueError("device mismatch")
-    if plan.device != device:
-        raise ValueError(f"the plan is for {plan.device}, the tensors are on {device}")
+    if plan.device != like.device:
+        raise ValueError(f"the plan is for {plan.device}, the tensors are on {like.device}")
     num_pages, page_size, kv_heads, _ = shape
     if page_size < 8 or page_size & (page_size - 1) or page_size > 1 << 20:
         raise ValueError(f"page_size must be a power of two in [8, 1048576]. Got page_size={page_size}")
@@ -689,7 +689,7 @@ def _norm_rows(w: Optional[torch.Tensor], heads: int, what: str, like: torch.Ten
     shape, D = w.shape, like.shape[2]
     if shape != (D,) and shape != (heads, D):
         raise ValueError(f"{what} must be [{D}] or [{heads}, {D}]; got {tuple(shape)}")
-    if w.dtype != like.dtype or w.device != like.device:
+    if w.dtype != like.dtype or w.get_device() != like.get_device():
         raise ValueError(f"{what} must have the device and dtype of qkv")
     return 1 if len(shape) == 1 else heads
 
@@ -716,8 +716,8 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages
     R = cos.shape[1] if cos.dim() == 2 else -1
     if cos.shape != (plan.tokens, R) or sin.shape != cos.shape or R % 2 or not 0 < R <= D:
         raise ValueError(f"cos and sin must be [{plan.tokens}, R], R even and at most {D}")
-    device, dtype = qkv.device, qkv.dtype
-    if cos.device != device or sin.device != device or cos.dtype != dtype or sin.dtype != dtype:
+    device, dtype, index = qkv.device, qkv.dtype, qkv.get_device()
+    if cos.get_device() != index or sin.get_device() != index or cos.dtype != dtype or sin.dtype != dtype:
         raise ValueError("cos and sin must have the device and dtype of qkv")
     q_rows, k_rows, eps = _norm_rows(q_norm, H, "q_norm", qkv), _norm_rows(k_norm, KVH, "k_norm", qkv), float(eps)
     if not 0.0 <= eps < math.inf:
