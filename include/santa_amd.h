@@ -429,7 +429,7 @@ typedef struct santa_paged_plan_info {
   int heads, kv_heads;
   long long records; /* parts: rows of the workspace */
   long long ints, pos_at, merge_at, parts_at, list_at; /* ints of the plan, and where its sections start */
-  int rounded; /* how probabilities enter the second product; the caller's to change (santa_paged_attention) */
+  int rounded; /* 0, 1 or 2: how probabilities enter the second product (santa_paged_attention) */
   int tree_ints;     /* of a token's record in a plan with trees, 0 in others */
   long long tree_at; /* where the records start */
 } santa_paged_plan_info;
@@ -463,10 +463,13 @@ int santa_paged_tree_plan(const int* lens, const int* new_tokens, const int* row
  * numbers are clamped to the pool.
  * Scores, softmax and sums in float32.  The probabilities enter the second
  * product as the sum of two values of the 16-bit type, with a product each, or,
- * where info->rounded is set and more than 16 rows share a pass over a KV head's
- * tokens, rounded to one.  A plan sets rounded where a sequence has several new
- * tokens and more than 32 rows (tokens x query heads per KV head); a copy of info
- * with another value may be given to any call.  workspace:
+ * where info->rounded is 1 and more than 16 rows share a pass over a KV head's
+ * tokens, rounded to one.  A plan sets rounded to 1 where a sequence has several new
+ * tokens and more than 32 rows (tokens x query heads per KV head), and a plan with
+ * trees to 2 then: those of trees are not rounded (but a tree that is one chain and
+ * shares no prefix is the sequence that it is without a tree), and the other sequences'
+ * are where one of these has that many rows.  A copy of info with 0 or 1 may be given to
+ * any call.  workspace:
  * santa_paged_workspace_size(info, D) bytes, 16-byte aligned, no initialization
  * needed. */
 size_t santa_paged_workspace_size(const santa_paged_plan_info* info, int D);

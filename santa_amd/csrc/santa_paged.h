@@ -13,8 +13,13 @@ constexpr int kBlockRows = 256;  // rows per workgroup: 32 for each of its 8 wav
 enum ItemFlags {
   kFromList = 1,  // tok0 indexes the plan's list of tokens; no row is before the item's end
   kDirect = 2,    // the item is all its rows attend to: it writes the output
-  kTree = 4       // what token i attends to from position tree0 on is in its record
+  kTree = 4,      // what token i attends to from position tree0 on is in its record
+  kTwoParts = 8   // in a plan of kByItem: its probabilities are in two parts
 };
+
+// How the probabilities of a plan's items enter the second product
+// (santa_paged_plan_info.rounded).
+enum Rounded { kNever = 0, kAlways = 1, kByItem = 2 };
 
 // A token's record in a plan with trees: the context tokens that it attends to,
 // its position (-1: not in use), and one bit for each position from the last

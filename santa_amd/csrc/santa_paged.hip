@@ -489,6 +489,7 @@ enum class Parts {
   kTwo,    // as the sum of two 16-bit values, each with a product of its own
   kLanes,  // likewise, the second values in lanes that up to 16 rows leave free
   kLanesOfTwo,  // likewise, in a kernel whose other items are kTwo
+  kByItem   // of a kernel: as the item's flag says, kTwo and kLanesOfTwo, or kOne and kLanes
 };
 
 // Probabilities of kTwo are 1 + kMore times as large (cut8); those of kLanesOfTwo,
@@ -1045,13 +1046,26 @@ __device__ __forceinline__ Item read_item(const Loader& w, int i) {
   return it;
 }
 
+// One item, in the form for its number of rows.
+template <bool BF16, int D, Parts kParts, bool kTrees>
+__device__ __forceinline__ void attend_rows(const AttnArgs& a, const Item& it, int kv, const Loader& w, Cursor& c,
+                                            const uint32_t (&lk)[2], const uint32_t (&lv)[2], uint32_t& tile,
+                                            uint32_t& loaded, u32x4* stages, Shares* x, uint32_t* bits) {
+  constexpr Parts kLanes = kParts == Parts::kTwo ? Parts::kLanesOfTwo : Parts::kLanes;
+  if (it.rows <= 16) attend<BF16, D, 1, kLanes, kTrees>(a, it, kv, w, c, lk, lv, tile, loaded, stages, x, bits);
+  else if (it.rows <= 32) attend<BF16, D, 1, kParts, kTrees>(a, it, kv, w, c, lk, lv, tile, loaded, stages, x, bits);
+  else if (it.rows <= 64) attend<BF16, D, 2, kParts, kTrees>(a, it, kv, w, c, lk, lv, tile, loaded, stages, x, bits);
+  else if (it.rows <= 128) attend<BF16, D, 4, kParts, kTrees>(a, it, kv, w, c, lk, lv, tile, loaded, stages, x, bits);
+  else attend<BF16, D, 8, kParts, kTrees>(a, it, kv, w, c, lk, lv, tile, loaded, stages, x, bits);
+}
+
 template <bool BF16, int D, Parts kParts, bool kTrees>
 __global__ __launch_bounds__(64 * kWaves, 2) void paged_attention_kernel(AttnArgs a) {
   using G = Geometry<D>;
   __shared__ u32x4 stages[G::kStages * G::kStage];
   __shared__ Shares shares;
   __shared__ uint32_t first_bits[kTrees ? 4 * kBlockRows : 1];
-  constexpr Parts kLanes = kParts == Parts::kTwo ? Parts::kLanesOfTwo : Parts::kLanes;
+  static_assert(sizeof stages + sizeof shares + (kTrees ? sizeof first_bits : 0) <= 160 * 1024, "a compute unit's LDS");
   const int kv = blockIdx.x % a.KVH, group = blockIdx.x / a.KVH;
   const int lane = threadIdx.x & 63;
   Loader w;
@@ -1089,16 +1103,14 @@ __global__ __launch_bounds__(64 * kWaves, 2) void paged_attention_kernel(AttnArg
     const Item now = it;
     last = now.next < 0;
     if (!last) it = read_item(w, now.next);  // while this one is worked on
-    if (now.rows <= 16) attend<BF16, D, 1, kLanes, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages,
-                                                     &shares, first_bits);
-    else if (now.rows <= 32) attend<BF16, D, 1, kParts, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages,
-                                                     &shares, first_bits);
-    else if (now.rows <= 64) attend<BF16, D, 2, kParts, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages,
-                                                     &shares, first_bits);
-    else if (now.rows <= 128) attend<BF16, D, 4, kParts, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages,
-                                                     &shares, first_bits);
-    else attend<BF16, D, 8, kParts, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages,
-                                                     &shares, first_bits);
+    if constexpr (kParts == Parts::kByItem) {
+      if (now.flags & kTwoParts)
+        attend_rows<BF16, D, Parts::kTwo, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares, first_bits);
+      else
+        attend_rows<BF16, D, Parts::kOne, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares, first_bits);
+    } else {
+      attend_rows<BF16, D, kParts, kTrees>(a, now, kv, w, c, lk, lv, tile, loaded, stages, &shares, first_bits);
+    }
   }
 }
 
@@ -1383,7 +1395,8 @@ extern "C" int santa_paged_attention(const void* q, const void* k_pages, const v
     };
     if (info->groups > 0) {
       if (info->tree_ints > 0) {
-        if (info->rounded) attend(paged_attention_kernel<BF16, kD, Parts::kOne, true>);
+        if (info->rounded == kByItem) attend(paged_attention_kernel<BF16, kD, Parts::kByItem, true>);
+        else if (info->rounded) attend(paged_attention_kernel<BF16, kD, Parts::kOne, true>);
         else attend(paged_attention_kernel<BF16, kD, Parts::kTwo, true>);
       } else {
         if (info->rounded) attend(paged_attention_kernel<BF16, kD, Parts::kOne, false>);

@@ -39,11 +39,15 @@ constexpr int kPieceCost = 20;
 int tile_cost(int rows, bool rounded) { return rows > 128 ? (rounded ? 10 : 13) : rows > 64 ? 7 : 6; }
 // Whether a sequence's new tokens have the batch's probabilities rounded for the
 // second product (santa_paged_plan_info.rounded, the default): several tokens, as
-// in a prefill, whose second products would cost more than they do behind HBM.
-// (Trees of drafts follow the same rule.)  8 sequences of 3000 to 16000 tokens, GH 4, D 128, rounded and in two parts: 8
-// tokens (32 rows) 76.8 and 77.5 us, 9 77.6 and 84.2, 32 90.9 and 102.9; a prefill
-// of 1300 tokens 313 and 410.  A single token is never rounded: what it attends to
-// must not depend on how many others read the same pages.
+// in a prefill, whose second products would cost more than they do behind HBM.  8
+// sequences of 3000 to 16000 tokens, GH 4, D 128, rounded and in two parts: 8 tokens
+// (32 rows) 76.8 and 77.5 us, 9 77.6 and 84.2, 32 90.9 and 102.9; a prefill of 1300
+// tokens 313 and 410.  A single token is never rounded: what it attends to
+// must not depend on how many others read the same pages.  Nor is a tree of drafts,
+// whatever the batch's other sequences are: a step that verifies it stands in for
+// decode steps, and what a draft attends to must not depend on its neighbours.  Only a
+// tree that is one chain, and reads no prefix with others, is the sequence that it is
+// without a tree, bit for bit.
 bool rounds(int new_tokens, int GH) { return new_tokens > 1 && static_cast<long long>(new_tokens) * GH > 32; }
 // The fewest tiles that a block is cut off after.
 constexpr int kLeastCut = 2;
@@ -64,6 +68,12 @@ struct Input {
   int n_groups, heads, kv_heads, fixed;
   const int *parents, *trees;  // NULL: no trees
   bool tree(int b) const { return trees && trees[b]; }
+  // Whether sequence b's new tokens, from `first` on, follow one another.
+  bool chain(int b, int first) const {
+    for (int i = 0; tree(b) && i < new_tokens[b]; ++i)
+      if (parents[first + i] != i - 1) return false;
+    return true;
+  }
 };
 
 // The most drafted tokens that a sequence has in a tree, or an error.
@@ -130,6 +140,9 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
     // the context's last tile and those that the new tokens begin
     info->tree_ints = kTreeWords + 2 * ((std::max(1, most) + 126) / 64);
     if (tokens * info->tree_ints > 1 << 26) return set_error(SANTA_ERR_INVALID, "too many new tokens beside trees");
+    // an update's trees may be chains or none: by item whatever they are, so that a
+    // captured call follows
+    if (info->rounded) info->rounded = kByItem;
   }
 
   // the passes: whole tiles of each group's common tokens for all its rows, and
@@ -137,26 +150,37 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
   std::vector<Block> blocks;
   std::vector<int> list;
   std::vector<int> token_pos(static_cast<size_t>(tokens)), token_row(static_cast<size_t>(tokens));
-  std::vector<int> group_list(static_cast<size_t>(in.n_groups), 0);
+  auto reads_with = [&](int b, int g) {  // whether sequence b's rows are among those of group g
+    return in.group[b] == g && static_cast<long long>(in.new_tokens[b]) * GH < kBlockRows;
+  };
   for (int g = 0; g < in.n_groups; ++g) {
-    const int common = in.shared[g] / kTile * kTile;
-    if (members[g] < 2 || common == 0) {
-      members[g] = 0;
-      continue;
+    if (members[g] < 2 || in.shared[g] < kTile) members[g] = 0;
+    for (int b = 0; b < in.B && members[g]; ++b)
+      if (reads_with(b, g)) prefix[b] = in.shared[g] / kTile * kTile;
+  }
+  // all parts of a row are held alike: its sums are joined
+  const bool by_item = info->rounded == kByItem;
+  auto as_tree = [&](int b) { return in.tree(b) && (prefix[b] > 0 || !in.chain(b, first[b])); };
+  bool others_round = false;
+  for (int b = 0; b < in.B && by_item; ++b) others_round |= rounds(in.new_tokens[b], GH) && !as_tree(b);
+  auto held = [&](bool tree) { return by_item && (tree || !others_round) ? kTwoParts : 0; };
+  for (int g = 0; g < in.n_groups; ++g) {
+    if (!members[g]) continue;
+    for (const bool trees : {false, true}) {
+      const int from = static_cast<int>(list.size());
+      for (int b = 0; b < in.B; ++b)
+        if (reads_with(b, g) && (by_item && in.tree(b)) == trees)
+          for (int i = 0; i < in.new_tokens[b]; ++i) list.push_back(first[b] + i);
+      const int n = static_cast<int>(list.size()) - from;
+      for (int i = 0; i < n; i += block_tokens)
+        blocks.push_back({kFromList | held(trees), lead[g], 0, in.shared[g] / kTile * kTile, from + i,
+                          std::min(block_tokens, n - i), kMaxLen, 0});
     }
-    group_list[g] = static_cast<int>(list.size());
-    for (int b = 0; b < in.B; ++b)
-      if (in.group[b] == g && static_cast<long long>(in.new_tokens[b]) * GH < kBlockRows) {
-        prefix[b] = common;
-        for (int i = 0; i < in.new_tokens[b]; ++i) list.push_back(first[b] + i);
-      }
-    const int n = static_cast<int>(list.size()) - group_list[g];
-    for (int i = 0; i < n; i += block_tokens)
-      blocks.push_back({kFromList, lead[g], 0, common, group_list[g] + i, std::min(block_tokens, n - i), kMaxLen, 0});
   }
   for (int b = 0; b < in.B; ++b) {
     const int n = in.lens[b], t = in.new_tokens[b], row = in.rows ? in.rows[b] : b;
     const bool tree = in.tree(b), vacant = tree && n < t;  // a tree that its sequence does not hold: no token in use
+    const int two = held(as_tree(b));
     for (int i = 0; i < t; ++i) {
       token_pos[first[b] + i] = tree && (vacant || in.parents[first[b] + i] == -2) ? -1 : n - t + i;
       token_row[first[b] + i] = row;
@@ -164,7 +188,8 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
     for (int i = 0; i < t; i += block_tokens) {
       const int k = std::min(block_tokens, t - i);
       const int end = vacant ? 0 : std::max(prefix[b], std::min(n, n - t + i + k));
-      blocks.push_back({tree ? kTree : 0, row, prefix[b], end, first[b] + i, k, n - t + i, tree ? std::max(0, n - t) : 0});
+      blocks.push_back({(tree ? kTree : 0) | two, row, prefix[b], end, first[b] + i, k, n - t + i,
+                        tree ? std::max(0, n - t) : 0});
     }
   }
 
@@ -175,11 +200,12 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
     int block, t0, t1, slot;
   };
   std::vector<Piece> pieces;
+  auto cost_of = [&](const Block& k) { return tile_cost(k.ntok * GH, info->rounded && !(k.flags & kTwoParts)); };
   auto pack = [&](long long budget, bool keep) {
     int slot = 0;
     long long left = budget;
     for (size_t i = 0; i < blocks.size(); ++i) {
-      const int tiles = blocks[i].tiles(), cost = tile_cost(blocks[i].ntok * GH, info->rounded);
+      const int tiles = blocks[i].tiles(), cost = cost_of(blocks[i]);
       for (int t = 0; t < tiles || t == 0;) {
         long long k = std::min<long long>(tiles - t, (left - kPieceCost) / cost);
         if (left < budget && (k < 1 ? tiles > 0 || left < kPieceCost : k < tiles - t && k < kLeastCut)) {
@@ -196,7 +222,7 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
     return true;
   };
   long long total = 0;
-  for (const Block& k : blocks) total += kPieceCost + static_cast<long long>(tile_cost(k.ntok * GH, info->rounded)) * k.tiles();
+  for (const Block& k : blocks) total += kPieceCost + static_cast<long long>(cost_of(k)) * k.tiles();
   long long lo = std::max<long long>(total / slots, kPieceCost + tile_cost(1, true) * kLeastCut), hi = lo;
   while (!pack(hi, false)) lo = hi + 1, hi += std::max(1LL, hi / 4);
   while (lo < hi) {

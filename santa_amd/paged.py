@@ -964,8 +964,11 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     enter it as the sum of two such values, which gives the values of float32
     probabilities and takes up to a third longer where many rows read the same
     tokens.  By default they are rounded where a sequence has several new
-    tokens, and more than 32 rows of them (tokens x query heads per KV head);
-    up to 16 rows that pass over a KV head's tokens together are not rounded
+    tokens, and more than 32 rows of them (tokens x query heads per KV head),
+    for all sequences without a tree; those of trees are not, whatever is beside
+    them, as a step that verifies drafts stands in for decode steps.  (A tree that
+    is one chain, and shares no prefix, is the sequence that it is without one.)
+    Up to 16 rows that pass over a KV head's tokens together are not rounded
     either way.  The expressions for other calls never round them."""
     if q.dim() != 3:
         raise ValueError(f"q must be [tokens, H, D]; got {tuple(q.shape)}")
@@ -997,7 +1000,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     strides = (_L * 8)(*sq, *_strides(k_pages, "k_pages"), *_strides(v_pages, "v_pages"))
     table, row = _table_rows(block_table)
     info = plan._info
-    if rounded is not None and bool(info.rounded) != rounded:
+    if rounded is not None and info.rounded != int(rounded):
         info = _PlanInfo.from_buffer_copy(info)
         info.rounded = int(rounded)
     info = ctypes.byref(info)

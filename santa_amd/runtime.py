@@ -637,7 +637,7 @@ class RandomLlama:
     @torch.inference_mode()
     def extend(self, tokens: torch.Tensor, cache, seqs: Sequence[int],
                new_tokens: Union[None, int, Sequence[int]] = None, *, backend=None,
-               mlp_chunk: int = 8192, parents=None) -> torch.Tensor:
+               mlp_chunk: int = 8192, parents=None, rounded: Optional[bool] = None) -> torch.Tensor:
         """New tokens of sequences of a santa_amd.paged.PagedKVCache: prompts of
         new sequences, more tokens behind what a sequence holds (a prompt behind
         one it was forked from), or one decoded token each.  tokens: [len(seqs),
@@ -650,8 +650,9 @@ class RandomLlama:
         step's plan where its decodes_plans is set).  parents: the new tokens are
         drafts that follow one another as trees (santa_amd.paged.PagedPlan), and the
         logits are those behind every new token [tokens, V]; PagedKVCache.keep then
-        takes back what is not accepted.  A call that fails leaves the sequences with
-        the tokens that they had."""
+        takes back what is not accepted.  rounded: how probabilities are held, as
+        santa_amd.paged.paged_attention takes it.  A call that fails leaves the
+        sequences with the tokens that they had."""
         from .paged import _int_list
 
         s, D = self.shape, self.shape.head_dim
@@ -672,18 +673,20 @@ class RandomLlama:
             raise ValueError("a backend decodes one new token per sequence")
         if backend is not None and parents is not None:
             raise ValueError("a backend decodes no trees")
+        if backend is not None and rounded is not None:
+            raise ValueError("a backend holds probabilities in its own way")
         if mlp_chunk < 1:
             raise ValueError(f"mlp_chunk must be at least 1; got {mlp_chunk}")
         h = self.embed[tokens.reshape(-1)]  # [N, hidden]
         cache.extend(seqs, new)
         try:
-            return self._extend(h, cache, seqs, new, backend, mlp_chunk, parents)
+            return self._extend(h, cache, seqs, new, backend, mlp_chunk, parents, rounded)
         except BaseException:  # a backend that does not take the model, a GPU without room
             cache._take_back(seqs, new)
             raise
 
     def _extend(self, h: torch.Tensor, cache, seqs: List[int], new: List[int], backend, mlp_chunk: int,
-                parents) -> torch.Tensor:
+                parents, rounded: Optional[bool]) -> torch.Tensor:
         """extend() of embedded tokens h [N, hidden] that the sequences have
         pages for."""
         from .paged import paged_attention, rope_append
@@ -704,7 +707,7 @@ class RandomLlama:
             elif backend is not None:
                 a = backend.decode_paged(q, cache.k[li], cache.v[li], tables, plan.seq_lens)
             else:
-                a = paged_attention(q, cache.k[li], cache.v[li], table, plan)
+                a = paged_attention(q, cache.k[li], cache.v[li], table, plan, rounded=rounded)
             return a.reshape(len(q), s.heads * D)
 
         fused = self._fused_layers_take(h)
