@@ -78,8 +78,7 @@ struct Rules {
 __device__ __forceinline__ float apply(float x, uint32_t word, const Rules& r) {
   if (word & (kCount | kInPrompt)) x = x > 0.0f ? x / r.repetition : x * r.repetition;
   const uint32_t count = word & kCount;
-  x = x - r.frequency * static_cast<float>(count);
-  if (count) x = x - r.presence;
+  if (count) x = x - r.frequency * static_cast<float>(count) - r.presence;  // of others not even 0 times an infinity
   if (word >> kBiasShift) x = x + r.bias[(word >> kBiasShift) - 1];
   return x;
 }

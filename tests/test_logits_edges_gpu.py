@@ -1,0 +1,36 @@
+"""Rules on logits on the GPU where their values are out of the ordinary: bit for bit
+against the expressions on the CPU, NaN for NaN.  Every case prints its name before
+touching the GPU."""
+import math
+
+import pytest
+import torch
+
+from santa_amd.logits import adjust_logits
+from santa_amd.paged import PagedPlan
+from test_logits_gpu import cuda
+
+pytestmark = pytest.mark.gpu
+
+
+def alike(out, want):
+    return torch.equal(out.isnan(), want.isnan()) and torch.equal(out.nan_to_num(0.0), want.nan_to_num(0.0))
+
+
+@pytest.mark.parametrize("what", ["repetition", "frequency", "presence"])
+@pytest.mark.parametrize("value", [math.inf, -math.inf, math.nan, 3e38])
+def test_penalties_that_are_not_finite(what, value):
+    """They reach the tokens that they are for: those of the answer, or all that the
+    row has seen; not those of the prompt, of a bias or of no rule."""
+    print(f"\n[case] {what} {value}", flush=True)
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(3, 50, generator=g)
+    tokens = torch.tensor([[1, 2, 2, 3, 4, 4], [5, 6, 7, 8, 9, 9], [0, 0, 0, 0, 0, 0]], dtype=torch.int32)
+    kw = {what: torch.tensor([value, 1.5, value]), "prompts": torch.tensor([3, 2, 6], dtype=torch.int32),
+          "bias": (torch.tensor([[1, 10, 4]], dtype=torch.int32), torch.tensor([[0.5, -1.0, 2.0]]))}
+    want = adjust_logits(x, tokens, [6, 6, 5], **kw)
+    out = adjust_logits(x.cuda(), tokens.cuda(), [6, 6, 5], **{k: cuda(v) for k, v in kw.items()})
+    assert alike(out.cpu(), want)
+    if what != "repetition" and not math.isfinite(value):  # of the third row all tokens are the prompt's
+        assert torch.isfinite(want[2]).all() and torch.isfinite(want[0, [1, 2, 10]]).all()
+        assert not torch.isfinite(want[0, 3])
