@@ -31,7 +31,7 @@ constexpr uint32_t kDrafted = 0x100000u;    // whether it is a drafted token, of
 constexpr int kBiasShift = 21;              // above: its bias's number, and one
 constexpr int kMostBiases = 2046;
 constexpr int kMostTokens = 0x7ffff;
-constexpr uint32_t kUntouched = 0x7fc0feedu;  // a NaN; a logit with these bits is its own result
+constexpr uint32_t kUntouched = 0x7fc0feedu;  // a NaN; a result with these bits is written as another one
 
 struct Args {
   const void* x;
@@ -324,7 +324,8 @@ __global__ __launch_bounds__(kThreads, kMany || kSteps == kMostSteps ? 4 : 6) vo
       for (int i = tid; i < count; i += kThreads) {
         const int at = list[i];
         const float x = i == tid && at == own ? own_logit : logit(r, at);
-        results[at] = __float_as_uint(apply(x, words[at], rules));
+        const uint32_t result = __float_as_uint(apply(x, words[at], rules));
+        results[at] = result == kUntouched ? 0x7fc00000u : result;
       }
       __syncthreads();
     }

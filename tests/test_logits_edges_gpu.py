@@ -34,3 +34,24 @@ def test_penalties_that_are_not_finite(what, value):
     if what != "repetition" and not math.isfinite(value):  # of the third row all tokens are the prompt's
         assert torch.isfinite(want[2]).all() and torch.isfinite(want[0, [1, 2, 10]]).all()
         assert not torch.isfinite(want[0, 3])
+
+
+def test_any_nan():
+    """A bias or a penalty of any NaN gives one, with whatever bits."""
+    print("\n[case] NaN of any bits", flush=True)
+    nans = torch.tensor([0x7fc0feed, 0x7fc00000, -1, 0x7f800001], dtype=torch.int32).view(torch.float32)
+    x, ids = torch.randn(4, 9), torch.tensor([[5]] * 4, dtype=torch.int32)
+    tokens = torch.tensor([[2, 2]] * 4, dtype=torch.int32)
+    want = x.clone()
+    want[:, 5] = math.nan
+    out = adjust_logits(x.cuda(), bias=(ids.cuda(), nans[:, None].cuda()))
+    assert alike(out.cpu(), want)
+    for name in ("repetition", "frequency", "presence"):
+        want = x.clone()
+        want[:, 2] = math.nan
+        assert alike(adjust_logits(x.cuda(), tokens.cuda(), [2] * 4, **{name: nans.cuda()}).cpu(), want)
+    x[:, 5] = nans  # of the logits themselves, with a rule and without
+    want = x.clone()
+    assert alike(adjust_logits(x.cuda()).cpu(), want)
+    assert alike(adjust_logits(x.cuda(), bias=(ids.cuda(), torch.ones(4, 1).cuda())).cpu(), want)
+    assert adjust_logits(x.cuda(), greedy=True).tolist() == [5] * 4
