@@ -144,6 +144,9 @@ def adjust_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
         allowed, allowed_stride = _rows(allowed, N, "allowed")
     if plan is not None and tokens is not None and plan._info.max_len >= 1 << 19:
         raise ValueError(f"at most {(1 << 19) - 1} tokens are counted; got {plan._info.max_len}")
+    if tokens is None and plan is None and (prompts is not None or any(
+            isinstance(p, torch.Tensor) or p != none for p, none in zip(penalties, (1.0, 0.0, 0.0)))):
+        raise ValueError("penalties and prompts are for tokens that a row has seen: without tokens there are none")
     kind = _KINDS.get(logits.dtype)
     given = [t for t in (*penalties, values) if isinstance(t, torch.Tensor)]
     if not (device.type == "cuda" and kind is not None and _plain(logits, *given)):
