@@ -74,6 +74,14 @@ def _rows(t: torch.Tensor, count: int, what: str) -> Tuple[torch.Tensor, int]:
     return t, t.stride(0) if shape[0] > 1 else 0
 
 
+def _bare(*ts: Optional[torch.Tensor]) -> bool:
+    """Tensors with memory of their own: no subclasses, none under functorch transforms."""
+    for t in ts:
+        if t is not None and (type(t) is not torch.Tensor or torch._C._functorch.is_functorch_wrapped_tensor(t)):
+            return False
+    return True
+
+
 def adjust_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
                   plan: Union[None, PagedPlan, Sequence[int]] = None, *, prompts: Optional[torch.Tensor] = None,
                   repetition: Union[float, torch.Tensor] = 1.0, frequency: Union[float, torch.Tensor] = 0.0,
@@ -149,7 +157,8 @@ def adjust_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
         raise ValueError("penalties and prompts are for tokens that a row has seen: without tokens there are none")
     kind = _KINDS.get(logits.dtype)
     given = [t for t in (*penalties, values) if isinstance(t, torch.Tensor)]
-    if not (device.type == "cuda" and kind is not None and _plain(logits, *given)):
+    if not (device.type == "cuda" and kind is not None and _plain(logits, *given)
+            and _bare(tokens, prompts, ids, allowed)):
         out = _expressions(logits, tokens, plan, prompts, penalties, ids, values, allowed)
         if plan is not None:
             plan._captured(0, False)
@@ -201,33 +210,36 @@ def _expressions(logits, tokens, plan, prompts, penalties, ids, values, allowed)
     rows = list(range(N)) if plan is None else [row for row, t in zip(plan.rows, plan.new_tokens) for _ in range(t)]
     at = torch.tensor(rows, dtype=torch.int64, device=device)
     repetition, frequency, presence = (p[at][:, None].to(x.dtype) if isinstance(p, torch.Tensor) else p for p in penalties)
-    if tokens is not None:
-        seen = torch.zeros(N, V + 1, dtype=torch.bool, device=device)  # the last column: no token of the vocabulary
-        count = torch.zeros(N, V + 1, dtype=torch.int64, device=device)
-        r = 0
+    if tokens is not None and N > 0:
+        none = torch.zeros(V + 1, dtype=torch.int64, device=device)  # the last one: no token of the vocabulary
+        all_seen, counts = [], []
         for b, (row, n, t) in enumerate(zip(plan.rows, plan.seq_lens, plan.new_tokens)):
             ids_b = tokens[row, :n].long()
             ids_b = torch.where((ids_b >= 0) & (ids_b < V), ids_b, V)
-            answer = torch.arange(n, device=device) >= (0 if prompts is None else prompts[row])
+            answer = (torch.arange(n, device=device) >= (0 if prompts is None else prompts[row])).long()
             tree = plan.parents is not None and plan.parents[b] is not None
-            sees = plan._sees(b).to(device) if tree else None
-            for i in plan._in_use(b):
-                context = n - t if tree else n - t + i + 1
-                seen[r + i, ids_b[:context]] = True
-                count[r + i].index_add_(0, ids_b[:context], answer[:context].long())
+            if tree:
+                sees = plan._sees(b)
+                answer = torch.cat([answer[:max(0, n - t)], answer.new_ones(min(n, t))])  # a tree's are the answer's
+            used = set(plan._in_use(b))
+            for i in range(t):
+                if i not in used:
+                    all_seen.append(none > 0), counts.append(none)
+                    continue
+                places = torch.arange(n - t + i + 1, device=device)
                 if tree:
-                    drafted = ids_b[n - t:][sees[i]]
-                    seen[r + i, drafted] = True
-                    count[r + i].index_add_(0, drafted, torch.ones_like(drafted))
-            r += t
-        seen, count = seen[:, :V], count[:, :V]
+                    places = torch.cat([places[:n - t], n - t + sees[i].nonzero()[:, 0].to(device)])
+                here = ids_b[places]
+                all_seen.append(none.scatter_add(0, here, torch.ones_like(here)) > 0)
+                counts.append(none.scatter_add(0, here, answer[places]))
+        seen, count = torch.stack(all_seen)[:, :V], torch.stack(counts)[:, :V]
         x = torch.where(seen, torch.where(x > 0, x / repetition, x * repetition), x)
         x = torch.where(count > 0, x - frequency * count.to(x.dtype) - presence, x)
     if ids is not None and ids.shape[1]:
         each = torch.arange(ids.shape[1], device=device).expand(ids.shape)
         inside = (ids >= 0) & (ids < V)
         last = torch.full((len(ids), V + 1), -1, dtype=torch.int64, device=device)
-        last.scatter_reduce_(1, torch.where(inside, ids, V).long(), torch.where(inside, each, -1), "amax")
+        last = last.scatter_reduce(1, torch.where(inside, ids, V).long(), torch.where(inside, each, -1), "amax")
         last = last[:, :V].expand(N, V) if len(ids) == 1 else last[at, :V]
         row_values = values.expand(N, -1) if len(values) == 1 else values[at]
         x = torch.where(last >= 0, x + row_values.gather(1, last.clamp(min=0)).to(x.dtype), x)

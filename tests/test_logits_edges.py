@@ -16,3 +16,38 @@ def test_penalties_without_tokens(kw):
         adjust_logits(x, greedy=True, **kw)
     assert torch.equal(adjust_logits(x, repetition=1.0, frequency=0.0, presence=-0.0), x)
     assert torch.equal(adjust_logits(x, None, [4, 5, 6], **kw), x)  # a plan, whose rows have seen none
+
+
+def under_vmap(device):
+    """What is mapped alone -> (values, those of calls one by one)."""
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(3, 40, generator=g).to(device)
+    i = lambda lo, hi, *s: torch.randint(lo, hi, s, generator=g, dtype=torch.int64).to(torch.int32).to(device)  # noqa: E731
+    tokens, prompts, ids, bits = i(0, 40, 2, 3, 6), i(0, 6, 2, 3), i(-1, 41, 2, 3, 4), i(-(1 << 31), 1 << 31, 2, 3, 2)
+    values, lens = torch.randn(2, 3, 4, generator=g).to(device), [4, 5, 6]
+    penalties = torch.rand(2, 3, generator=g).to(device) + 0.5
+    calls = {
+        "logits": (torch.stack([x, -x]), lambda y: adjust_logits(y, tokens[0], lens, repetition=2.0)),
+        "tokens": (tokens, lambda t: adjust_logits(x, t, lens, repetition=2.0, frequency=0.5)),
+        "prompts": (prompts, lambda p: adjust_logits(x, tokens[0], lens, prompts=p, frequency=0.5)),
+        "ids": (ids, lambda b: adjust_logits(x, bias=(b, values[0]))),
+        "values": (values, lambda b: adjust_logits(x, bias=(ids[0], b))),
+        "allowed": (bits, lambda b: adjust_logits(x, allowed=b)),
+        "penalty": (penalties, lambda p: adjust_logits(x, tokens[0], lens, repetition=p)),
+        "tree": (tokens, lambda t: adjust_logits(x, t, _tree(device), presence=0.5)),
+        "token": (bits, lambda b: adjust_logits(x, allowed=b, greedy=True)),
+    }
+    return {k: (torch.vmap(f)(mapped), torch.stack([f(y) for y in mapped])) for k, (mapped, f) in calls.items()}
+
+
+def _tree(device):
+    from santa_amd.paged import PagedPlan
+
+    return PagedPlan([6], heads=1, kv_heads=1, new_tokens=[3], parents=[[-1, 0, 0]], device=device)
+
+
+def test_vmap():
+    """Under vmap over one argument alone, whichever it is, a call gives what it
+    gives for each."""
+    for what, (out, want) in under_vmap("cpu").items():
+        assert torch.equal(out, want), what

@@ -7,7 +7,7 @@ import pytest
 import torch
 
 from santa_amd.logits import adjust_logits
-from santa_amd.paged import PagedPlan
+from test_logits_edges import under_vmap
 from test_logits_gpu import cuda
 
 pytestmark = pytest.mark.gpu
@@ -55,3 +55,12 @@ def test_any_nan():
     assert alike(adjust_logits(x.cuda()).cpu(), want)
     assert alike(adjust_logits(x.cuda(), bias=(ids.cuda(), torch.ones(4, 1).cuda())).cpu(), want)
     assert adjust_logits(x.cuda(), greedy=True).tolist() == [5] * 4
+
+
+def test_vmap():
+    """Tensors that a transform wraps have no memory for a kernel to read: whichever
+    argument it is alone, the expressions take it."""
+    print("\n[case] vmap", flush=True)
+    for what, (out, want) in under_vmap("cuda").items():
+        # torch's quotient by a number is a product with its inverse on a GPU: a rounding more
+        assert (out == want).all() or ((out - want).abs() <= 2.0 ** -22 * want.abs()).all(), what
