@@ -546,7 +546,8 @@ typedef struct santa_logit_rules {
  * penalty; then the bias is added; one that may not come is -inf.  Either out [N, V]
  * (float32, contiguous) is written or token [N]: the index of the row's maximum, NaN
  * above any number, the first one among equal values.  info, plan: those of a
- * santa_paged_plan of N tokens, or NULL.  At most 2^19 - 1 tokens are counted.
+ * santa_paged_plan of N tokens, plan 16-byte aligned, or NULL; all other arrays are
+ * aligned to their elements.  At most 2^19 - 1 tokens are counted.
  * workspace (for token): santa_adjust_logits_workspace_size bytes for these N, V and
  * rules->sequences, 8-byte aligned, no initialization needed. */
 size_t santa_adjust_logits_workspace_size(int N, int V, int sequences);

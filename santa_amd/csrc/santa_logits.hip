@@ -464,6 +464,18 @@ extern "C" int santa_adjust_logits(const void* x, int dtype, long long stride, i
     return set_error(SANTA_ERR_INVALID, "bad adjust_logits arguments");
   if (dtype != SANTA_BF16 && dtype != SANTA_F16 && dtype != SANTA_F32)
     return set_error(SANTA_ERR_UNSUPPORTED, "adjust_logits: logits are bf16, f16 or float32");
+  // what the kernels read in one piece: pairs of the plan's, one element of all else
+  const auto aligned = [](const void* p, size_t to) { return reinterpret_cast<uintptr_t>(p) % to == 0; };
+  if (info && !aligned(plan, 16))
+    return set_error(SANTA_ERR_INVALID, "adjust_logits: the plan must be 16-byte aligned");
+  if (!aligned(x, dtype == SANTA_F32 ? 4 : 2) || !aligned(out, 4) || !aligned(token, 8))
+    return set_error(SANTA_ERR_INVALID, "adjust_logits: logits and output must be aligned to their elements");
+  for (const void* p : {static_cast<const void*>(rules->prompts), static_cast<const void*>(rules->repetition),
+                        static_cast<const void*>(rules->frequency), static_cast<const void*>(rules->presence),
+                        static_cast<const void*>(rules->bias_ids), static_cast<const void*>(rules->bias),
+                        static_cast<const void*>(rules->allowed)})
+    if (!aligned(p, 4))
+      return set_error(SANTA_ERR_INVALID, "adjust_logits: the rules' arrays must be aligned to their elements");
   if (info && info->tokens != N)
     return set_error(SANTA_ERR_INVALID, "adjust_logits: the plan is for %d rows; got %d", info->tokens, N);
   if (rules->tokens) {
@@ -473,7 +485,7 @@ extern "C" int santa_adjust_logits(const void* x, int dtype, long long stride, i
                        info->max_len - 1, info->max_row, rules->tokens_rows, rules->tokens_len);
     if (info->max_len > kMostTokens)
       return set_error(SANTA_ERR_UNSUPPORTED, "adjust_logits counts up to %d tokens. Got %d", kMostTokens, info->max_len);
-    if (reinterpret_cast<uintptr_t>(rules->tokens) % (rules->tokens_wide ? 8 : 4) != 0)
+    if (!aligned(rules->tokens, rules->tokens_wide ? 8 : 4))
       return set_error(SANTA_ERR_INVALID, "adjust_logits: tokens must be aligned");
   }
   if (rules->biases < 0 || (rules->biases > 0 && (!rules->bias_ids || !rules->bias)))

@@ -1,8 +1,12 @@
 """Rules on logits, on the CPU, at the edges of what a call may say."""
+import ctypes
+
 import pytest
 import torch
 
+from santa_amd import logits as L
 from santa_amd.logits import adjust_logits
+from santa_amd.paged import PagedPlan
 
 
 @pytest.mark.parametrize("kw", [{"repetition": 2.0}, {"frequency": 0.5}, {"presence": -0.5}, {"repetition": torch.ones(3)},
@@ -41,8 +45,6 @@ def under_vmap(device):
 
 
 def _tree(device):
-    from santa_amd.paged import PagedPlan
-
     return PagedPlan([6], heads=1, kv_heads=1, new_tokens=[3], parents=[[-1, 0, 0]], device=device)
 
 
@@ -51,3 +53,25 @@ def test_vmap():
     gives for each."""
     for what, (out, want) in under_vmap("cpu").items():
         assert torch.equal(out, want), what
+
+
+def test_library_refuses_what_is_not_aligned():
+    """The plan, which kernels read in pairs, and every array of the call."""
+    lib, info = L._lib(), PagedPlan([20, 9], heads=4, kv_heads=2, device="cpu")._info
+
+    def call(x=4096, dtype=2, plan=4096, out=4096, token=None, **kw):
+        rules = L._Rules(**{"tokens": 4096, "tokens_rows": 2, "tokens_len": 20, "tokens_stride": 20, "biases": 3,
+                            "bias_ids": 4096, "bias": 4096, **kw})
+        rc = lib.santa_adjust_logits(x, dtype, 100, 2, 100, ctypes.byref(rules), ctypes.byref(info), plan, out, token,
+                                     4096, 0, None)
+        assert rc != 0
+        return lib.santa_last_error().decode()
+
+    for off in (4, 8):  # without it the refusal is the one of the workspace, which comes last
+        assert "the plan must be 16-byte aligned" in call(plan=4096 + off, out=None, token=4096)
+    assert "workspace" in call(out=None, token=4096)
+    for kw in ({"x": 4098}, {"x": 4097, "dtype": 0}, {"out": 4098}, {"out": None, "token": 4100}):
+        assert "aligned to their elements" in call(**kw)
+    for name in ("prompts", "repetition", "frequency", "presence", "bias_ids", "bias", "allowed"):
+        assert "rules' arrays" in call(out=None, token=4096, **{name: 4098})
+    assert "aligned" in call(out=None, token=4096, tokens=4100, tokens_wide=1)
