@@ -22,7 +22,7 @@ from typing import Optional, Sequence, Tuple, Union
 
 import torch
 
-from .paged import _KINDS, PagedPlan, _launch, _PlanInfo
+from .paged import _KINDS, PagedPlan, _elsewhere, _launch, _PlanInfo
 from .runtime import _FusedOps, _plain
 
 __all__ = ["adjust_logits"]
@@ -120,6 +120,12 @@ def adjust_logits(logits: torch.Tensor, tokens: Optional[torch.Tensor] = None,
         plan = PagedPlan(plan, heads=1, kv_heads=1, device=device)
     if plan is not None and (plan.tokens != N or plan.device != device):
         raise ValueError(f"the plan is for {plan.tokens} tokens on {plan.device}; got {N} rows on {device}")
+    if index < 0:  # CPU and meta tensors have one number
+        for name, t in (("tokens", tokens), ("prompts", prompts), ("repetition", repetition), ("frequency", frequency),
+                        ("presence", presence), ("bias", None if bias is None else bias[0]),
+                        ("bias", None if bias is None else bias[1]), ("allowed", allowed)):
+            if isinstance(t, torch.Tensor) and _elsewhere(logits, t):
+                raise ValueError(f"{name} must be on the logits' device; got {t.device}")
     seqs = N if plan is None else plan._info.max_row + 1
     if tokens is not None:
         if tokens.dim() != 2 or tokens.dtype not in (torch.int32, torch.int64) or tokens.get_device() != index:

@@ -115,6 +115,13 @@ def _device(device) -> torch.device:
     return device
 
 
+def _elsewhere(like: torch.Tensor, *ts: Optional[torch.Tensor]) -> bool:
+    """Whether one of ts is on another device than `like`.  GPUs are told apart by
+    get_device() first, which costs less; all other devices, CPU and meta among them,
+    have -1 there."""
+    return any(t is not None and t.device != like.device for t in ts)
+
+
 def _int_list(values, what: str) -> List[int]:
     """Host integers: a list, a range, an array or a CPU tensor."""
     if isinstance(values, torch.Tensor):
@@ -606,7 +613,8 @@ def _check_pools(k_pages, v_pages, block_table, plan: PagedPlan, like: torch.Ten
     if block_table.dtype != torch.int32 or block_table.dim() != 2 or (block_table.shape[1] > 1
                                                                       and block_table.stride(1) != 1):
         raise ValueError("block_table must be an int32 [sequences, pages] tensor with contiguous rows")
-    if k_pages.get_device() != device or v_pages.get_device() != device or block_table.get_device() != device:
+    if k_pages.get_device() != device or v_pages.get_device() != device or block_table.get_device() != device or (
+            device < 0 and _elsewhere(like, k_pages, v_pages, block_table)):
         raise ValueError("device mismatch")
     if plan.device != like.device:
         raise ValueError(f"the plan is for {plan.device}, the tensors are on {like.device}")
@@ -689,7 +697,8 @@ def _norm_rows(w: Optional[torch.Tensor], heads: int, what: str, like: torch.Ten
     shape, D = w.shape, like.shape[2]
     if shape != (D,) and shape != (heads, D):
         raise ValueError(f"{what} must be [{D}] or [{heads}, {D}]; got {tuple(shape)}")
-    if w.dtype != like.dtype or w.get_device() != like.get_device():
+    index = like.get_device()
+    if w.dtype != like.dtype or w.get_device() != index or (index < 0 and _elsewhere(like, w)):
         raise ValueError(f"{what} must have the device and dtype of qkv")
     return 1 if len(shape) == 1 else heads
 
@@ -717,7 +726,8 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages
     if cos.shape != (plan.tokens, R) or sin.shape != cos.shape or R % 2 or not 0 < R <= D:
         raise ValueError(f"cos and sin must be [{plan.tokens}, R], R even and at most {D}")
     device, dtype, index = qkv.device, qkv.dtype, qkv.get_device()
-    if cos.get_device() != index or sin.get_device() != index or cos.dtype != dtype or sin.dtype != dtype:
+    if cos.get_device() != index or sin.get_device() != index or cos.dtype != dtype or sin.dtype != dtype or (
+            index < 0 and _elsewhere(qkv, cos, sin)):
         raise ValueError("cos and sin must have the device and dtype of qkv")
     q_rows, k_rows, eps = _norm_rows(q_norm, H, "q_norm", qkv), _norm_rows(k_norm, KVH, "k_norm", qkv), float(eps)
     if not 0.0 <= eps < math.inf:
