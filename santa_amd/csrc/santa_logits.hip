@@ -232,12 +232,14 @@ __global__ __launch_bounds__(kThreads, kMany || kSteps == kMostSteps ? 4 : 6) vo
     const int seq = a.pos ? w.at.y : r, context = !a.tokens ? 0 : a.tree ? w.head.x : w.at.x + 1;
     // a tree's token lies behind the context that it sees, others are the last of theirs
     const bool drafted = a.tokens && a.tree && w.head.y >= 0 && context <= w.at.x;
+    // a tree's token that is not in use has seen nothing; the words stay those of the rows around it
+    const bool unused = a.tokens && a.tree && w.head.y < 0;
     int count = 0;
     if (ruled) {
       const void* row = static_cast<const char*>(a.tokens) + seq * a.tokens_stride * (a.wide ? 8 : 4);
       const int base = context & ~63;
-      const bool anew = seq != held || context < upto ||
-                        (tree_base >= 0 && !(drafted && base == tree_base && context == upto));
+      const bool anew = seq != held || (!unused && (context < upto || (tree_base >= 0 && !(drafted && base == tree_base &&
+                                                                                           context == upto))));
       if (anew) upto = 0, tree_base = -1;
       // what is read here is asked for before any of it is used
       int id[kTokenSteps][4], bias_id = -1;
@@ -324,7 +326,8 @@ __global__ __launch_bounds__(kThreads, kMany || kSteps == kMostSteps ? 4 : 6) vo
       for (int i = tid; i < count; i += kThreads) {
         const int at = list[i];
         const float x = i == tid && at == own ? own_logit : logit(r, at);
-        const uint32_t result = __float_as_uint(apply(x, words[at], rules));
+        const uint32_t word = unused ? words[at] & ~(kCount | kInPrompt) : words[at];
+        const uint32_t result = __float_as_uint(apply(x, word, rules));
         results[at] = result == kUntouched ? 0x7fc00000u : result;
       }
       __syncthreads();

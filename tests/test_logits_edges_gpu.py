@@ -2,13 +2,16 @@
 against the expressions on the CPU, NaN for NaN.  Every case prints its name before
 touching the GPU."""
 import math
+import random
 
 import pytest
 import torch
 
 from santa_amd.logits import adjust_logits
+from santa_amd.paged import PagedPlan
+from test_draft_trees import random_tree
 from test_logits_edges import under_vmap
-from test_logits_gpu import cuda
+from test_logits_gpu import cuda, same
 
 pytestmark = pytest.mark.gpu
 
@@ -64,3 +67,23 @@ def test_vmap():
     for what, (out, want) in under_vmap("cuda").items():
         # torch's quotient by a number is a product with its inverse on a GPU: a rounding more
         assert (out == want).all() or ((out - want).abs() <= 2.0 ** -22 * want.abs()).all(), what
+
+
+@pytest.mark.parametrize("V", [37, 5000, 128256])
+def test_tokens_not_in_use_among_others(V):
+    """Rows of tokens not in use have the biases alone, wherever they are in a tree,
+    and the rows around them what their own paths have seen."""
+    print(f"\n[case] not in use among others V={V}", flush=True)
+    r, g = random.Random(V), torch.Generator().manual_seed(V)
+    every = [-1 if i == 0 else max(0, i - 2) if i % 2 == 0 else -2 for i in range(40)]
+    trees = [every, [-2] * 9 + [-1, 9, -2, 10], [-2, -1, -2, -2, 1], [-2] * 3, None, random_tree(r, 70, 0.5), [-2, -1], [-1, -2],
+             [-1] + [0 if i % 3 else -2 for i in range(1, 600)], random_tree(r, 5, 0.4)]
+    new = [40, 13, 5, 3, 6, 70, 2, 2, 600, 5]
+    lens, rows = [3000, 70, 64, 40, 90, 700, 66, 30, 700, 3], [0, 1, 2, 3, 4, 5, 5, 5, 6, 7]  # the last: shorter than its tree
+    tokens = torch.randint(0, min(V, 300), (8, 3000), generator=g, dtype=torch.int32)
+    for some in (slice(0, 10), slice(0, 3), slice(5, 8), slice(8, 10)):
+        plan = PagedPlan(lens[some], heads=4, kv_heads=2, new_tokens=new[some], rows=rows[some], parents=trees[some], device="cpu")
+        ids = torch.randint(0, V, (8, 7), generator=g, dtype=torch.int32)
+        same(torch.randn(plan.tokens, V, generator=g), tokens, plan,
+             dict(repetition=1.2, frequency=torch.rand(8, generator=g), presence=0.25, bias=(ids, torch.randn(8, 7, generator=g)),
+                  prompts=torch.arange(8, dtype=torch.int32) * 30))
