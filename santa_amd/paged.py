@@ -557,7 +557,10 @@ class PagedPlan:
     @property
     def positions(self) -> torch.Tensor:
         """The position of every token of the batch, int32 [tokens] on the device
-        (-1: a drafted token not in use)."""
+        (-1: a drafted token not in use): the plan's own memory, which a captured
+        call that reads it holds as the kernels' calls do."""
+        self._used()
+        self._captured(1 << 30, True)
         at, step = self._info.pos_at, 2
         if self._info.tree_ints:
             at, step = self._info.tree_at + 1, self._info.tree_ints
