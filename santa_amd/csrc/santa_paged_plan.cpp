@@ -153,10 +153,11 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
   auto reads_with = [&](int b, int g) {  // whether sequence b's rows are among those of group g
     return in.group[b] == g && static_cast<long long>(in.new_tokens[b]) * GH < kBlockRows;
   };
-  for (int g = 0; g < in.n_groups; ++g) {
+  for (int g = 0; g < in.n_groups; ++g)
     if (members[g] < 2 || in.shared[g] < kTile) members[g] = 0;
-    for (int b = 0; b < in.B && members[g]; ++b)
-      if (reads_with(b, g)) prefix[b] = in.shared[g] / kTile * kTile;
+  for (int b = 0; b < in.B && in.group; ++b) {
+    const int g = in.group[b];
+    if (g >= 0 && members[g] && reads_with(b, g)) prefix[b] = in.shared[g] / kTile * kTile;
   }
   // all parts of a row are held alike: its sums are joined
   const bool by_item = info->rounded == kByItem;
@@ -166,14 +167,14 @@ int build(const Input& in, santa_paged_plan_info* info, int* plan, long long pla
   auto held = [&](bool tree) { return by_item && (tree || !others_round) ? kTwoParts : 0; };
   for (int g = 0; g < in.n_groups; ++g) {
     if (!members[g]) continue;
-    for (const bool trees : {false, true}) {
+    for (int trees = 0; trees <= by_item; ++trees) {
       const int from = static_cast<int>(list.size());
       for (int b = 0; b < in.B; ++b)
-        if (reads_with(b, g) && (by_item && in.tree(b)) == trees)
+        if (reads_with(b, g) && (!by_item || in.tree(b) == (trees > 0)))
           for (int i = 0; i < in.new_tokens[b]; ++i) list.push_back(first[b] + i);
       const int n = static_cast<int>(list.size()) - from;
       for (int i = 0; i < n; i += block_tokens)
-        blocks.push_back({kFromList | held(trees), lead[g], 0, in.shared[g] / kTile * kTile, from + i,
+        blocks.push_back({kFromList | held(trees > 0), lead[g], 0, in.shared[g] / kTile * kTile, from + i,
                           std::min(block_tokens, n - i), kMaxLen, 0});
     }
   }
