@@ -265,7 +265,10 @@ __global__ __launch_bounds__(256) void rope_append_kernel(const uint16_t* __rest
 // as the prefill over contiguous caches does.  Elsewhere they enter it as two
 // values of that type, with a product each, so that a decode step has the values of
 // float32 probabilities, however many sequences read the same pages: free up to
-// 32 rows, up to a third more time above (both sides in santa_paged_plan.cpp).
+// 32 rows, up to a third more time above (both sides in santa_paged_plan.cpp).  So
+// they do for trees of drafts, which stand in for decode steps: a plan with trees and
+// that many rows says so item by item (kByItem, both forms in one kernel, which takes
+// what that of two parts alone does).
 //
 // What bounds it, at D 128 in bf16.  Few rows: HBM, 5.6 TB/s over 16-token pages
 // (16 sequences of 1000 to 40 000 tokens, 32 query and 8 KV heads, 1.55 GB:
@@ -287,12 +290,14 @@ __global__ __launch_bounds__(256) void rope_append_kernel(const uint16_t* __rest
 // of its bits.  Only the tiles from the context's end on differ, one or two for up to
 // 64 drafts; their scores are masked by a bit each, and all else is the same pass: 16
 // sequences of 1000 to 20 000 tokens with 25 drafts each, 32 query and 8 KV heads, 648
-// MB, 137 us, 4.7 TB/s, and 147 to 157 with the join, where the same tokens in a row
-// take 146 to 150.  Eight of 30 to 131 thousand tokens with 64 drafts, 64 query and 8 KV
-// heads: 1.56 to 1.8 ms, 790 to 915 TFLOP/s.  Their 512 rows are two blocks, and what
-// they wait for is not HBM: with all pages in the L2 1.40 ms, with K and V of zeros, read
-// as ever, 1.25, as the chip holds its clocks then.  Bits in LDS, 4 KiB for the first two
-// tiles of every row: in registers they spill, 27 of them beside probabilities in two parts.
+// MB, 172 us a call in a run of them, 7 of which the join (3.9 TB/s without it), and 150
+// with rounded probabilities, as the same tokens in a row take.  Eight of 30 to 131
+// thousand tokens with 64 drafts, 64 query and 8 KV heads: 2.24 ms, 640 TFLOP/s without the
+// second product's second half and 960 with it, and 1.72 ms rounded.  Their 512 rows are
+// two blocks.  Both HBM and the products' power hold them up: with all pages in the L2
+// 1.96 ms, with K and V of zeros, read as ever, 1.66, as the chip holds its clocks then
+// (rounded 1.45 and 1.28).  Bits in LDS, 4 KiB for the first two tiles of every row, with
+// which D 128 fills it: in registers 27 spill beside probabilities in two parts, so 21 to 23.
 constexpr int kWaves = 8;
 // Above this a row's reference in log2 units is subtracted from the scores before
 // they are scaled: fma(score, scale, -round(m * scale)) is off by half an ulp of

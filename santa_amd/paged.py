@@ -712,7 +712,8 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages
     """RoPE of the batch's tokens with their write into pages: qkv [tokens, H +
     2 KVH, D], cos and sin [tokens, R], R even and at most D: the first R dims of
     a head are rotated, dims d and d + R / 2 together (rotate-half convention) or,
-    interleaved, 2d and 2d + 1.  The k heads are rotated and written to k_pages,
+    interleaved, 2d and 2d + 1.  Tables hold a pair's angle for both of its dims: one
+    of D / 2 columns rotates half of a head.  The k heads are rotated and written to k_pages,
     the v heads to v_pages, at the tokens' positions; returns the rotated q heads
     [tokens, H, D].  q_norm, k_norm: weights [D], or [H, D] and [KVH, D], of an
     RMS norm of each q and k head before its rotation, x / sqrt(mean(x^2) + eps) *
@@ -866,7 +867,8 @@ def rope_tables(positions: torch.Tensor, dim: int, *, theta: float = 10000.0, sc
     """cos and sin [tokens, dim] of integer positions [tokens] (``plan.positions``)
     for ``rope_append``: the angle positions x theta^(-2i / dim), scaled as
     `scaling` says, in dims i and i + dim / 2 or, interleaved, 2i and 2i + 1.  dim:
-    the number of rotated dims, even.  Angles are float64: far positions lose nothing."""
+    the number of rotated dims, even.  Angles are float64, far positions lose nothing;
+    on a GPU cos and sin are float32's, rounded once more to the dtype."""
     if positions.dim() != 1 or positions.dtype not in (torch.int32, torch.int64):
         raise ValueError("positions must be [tokens] of int32 or int64")
     if dim <= 0 or dim % 2:
