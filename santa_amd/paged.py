@@ -1015,9 +1015,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     strides = (_L * 8)(*sq, *_strides(k_pages, "k_pages"), *_strides(v_pages, "v_pages"))
     table, row = _table_rows(block_table)
     info = plan._info
-    if rounded is not None and info.rounded != int(rounded):
+    if rounded is not None and info.rounded != bool(rounded):
         info = _PlanInfo.from_buffer_copy(info)
-        info.rounded = int(rounded)
+        info.rounded = bool(rounded)
     info = ctypes.byref(info)
     lib = _lib()
     workspace = torch.empty(lib.santa_paged_workspace_size(info, D), dtype=torch.uint8, device=device)
