@@ -39,9 +39,9 @@ __device__ __forceinline__ _Float16 rounded<_Float16>(float x) { return static_c
 // in float64, of which the whole ones leave nothing.  What remains, r, is a float32 h
 // and what that leaves, l, of at most 2^-26 turns: with e = 2 pi l, cos(2 pi r) = cos(2
 // pi h) - e sin(2 pi h), sin(2 pi r) = sin(2 pi h) + e cos(2 pi h), up to e^2 / 2 < 2^-47.
-// Bound by sincospif's vector work
-// beside the stores: 27 thousand positions of 64 pairs in float32, 28 MB, 9.9 us (9.8
-// without l, 10.3 with a pair a thread); 64 positions are the launch (2.6 us).
+// Bound by sincospif's vector work beside the stores: 27 thousand positions of 64 pairs
+// in float32, 28 MB, 9.9 us (9.8 without l, 10.3 with a pair a thread); 64 positions are
+// the launch (2.6 us).
 template <class T, int kMore, bool kInterleaved>
 __global__ __launch_bounds__(256) void rope_tables_kernel(const void* __restrict__ positions, int wide,
                                                           long long stride, Frequencies f, int pairs,

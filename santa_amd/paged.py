@@ -713,9 +713,9 @@ def rope_append(qkv: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor, k_pages
     2 KVH, D], cos and sin [tokens, R], R even and at most D: the first R dims of
     a head are rotated, dims d and d + R / 2 together (rotate-half convention) or,
     interleaved, 2d and 2d + 1.  Tables hold a pair's angle for both of its dims: one
-    of D / 2 columns rotates half of a head.  The k heads are rotated and written to k_pages,
-    the v heads to v_pages, at the tokens' positions; returns the rotated q heads
-    [tokens, H, D].  q_norm, k_norm: weights [D], or [H, D] and [KVH, D], of an
+    of D / 2 columns rotates half of a head.  The k heads are rotated and written to
+    k_pages, the v heads to v_pages, at the tokens' positions; returns the rotated q
+    heads [tokens, H, D].  q_norm, k_norm: weights [D], or [H, D] and [KVH, D], of an
     RMS norm of each q and k head before its rotation, x / sqrt(mean(x^2) + eps) *
     weight.  float32 arithmetic, rounded once.  Two tokens of one position and page
     (sequences that share a page they write to) leave one of the two there:
